@@ -359,6 +359,111 @@ int pqkv_prefill_attn(const void *q, int q_dtype, const float *R,
                       void *out, int out_dtype,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- a cache under a budget ------------------------------------------------
+ * No counterpart in the reference, whose token importance only assigns widths
+ * (src/polarquant_kv_cuda/token_importance.py:17-40): attention that also says
+ * how much weight each cached position got, the choice of the positions that
+ * stay, the move of their vectors, and rotary positions for queries and keys
+ * (a position's slot in such a cache no longer says where it stood). */
+
+/* pqkv_decode_attn that also gives the weights: for t < S
+ *   weights_out[b][h][t] = weights_in[b][h][t] (0 where weights_in is NULL)
+ *                          + sum over kv head h's query heads of softmax(s)_t,
+ * fp32, summed in a fixed order. Entries of weights_out from S on are left as
+ * they are. weights_in / weights_out: stream (b, h) starts (b * Hkv + h) *
+ * weights_*_stride floats in (a stride of at least S); weights_out may be
+ * weights_in with the same stride, and may not overlap it otherwise. Keys and
+ * values of one width n_bits (2 or 4), no per-head widths; S = 0 writes zeros
+ * to out and no weights. S < 2^24. The output equals pqkv_decode_attn's bit
+ * for bit. */
+size_t pqkv_decode_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int d);
+int pqkv_decode_attn_weights(const void *q, int q_dtype, const float *R,
+                             const uint8_t *k_cache, const uint8_t *v_cache,
+                             const float *k_codebook, const float *v_codebook, int n_bits,
+                             const uint8_t *qjl_signs, const float *p_rot, int m,
+                             int B, int Hq, int Hkv, int S, int S_max, int d, float scale,
+                             void *out, int out_dtype,
+                             const float *weights_in, int64_t weights_in_stride,
+                             float *weights_out, int64_t weights_out_stride,
+                             void *workspace, size_t workspace_bytes, void *stream);
+/* The same on a paged cache (as pqkv_decode_attn_paged). */
+int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
+                                   const uint8_t *const *k_pages, const uint8_t *const *v_pages,
+                                   int page_tokens, int max_pages,
+                                   const float *k_codebook, const float *v_codebook, int n_bits,
+                                   const uint8_t *const *qjl_pages, const float *p_rot, int m,
+                                   int B, int Hq, int Hkv, int S, int d, float scale,
+                                   void *out, int out_dtype,
+                                   const float *weights_in, int64_t weights_in_stride,
+                                   float *weights_out, int64_t weights_out_stride,
+                                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* The weights alone, of Sq query tokens per sequence at positions q_start ..
+ * q_start + Sq - 1 (causal as pqkv_prefill_attn): weights_out[b][h][t] =
+ * weights_in[b][h][t] + sum over kv head h's query heads and the Sq tokens of
+ * softmax(s)_t, arguments as pqkv_prefill_attn and pqkv_decode_attn_weights
+ * (keys only: no values are read). Sq = 0 copies weights_in (or writes zeros);
+ * S = 0 writes nothing. Any group size Hq / Hkv. The workspace needs no
+ * initialisation; its size does not grow past about 600 MB plus the rotated
+ * queries (long chunks run in passes). */
+size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d);
+int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
+                      int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,
+                      int B, int Hq, int Hkv, int Sq, int q_start, int S, int S_max, int d, float scale, int causal,
+                      const float *weights_in, int64_t weights_in_stride,
+                      float *weights_out, int64_t weights_out_stride,
+                      void *workspace, size_t workspace_bytes, void *stream);
+int pqkv_attn_weights_paged(const void *q, int q_dtype, const float *R, const uint8_t *const *k_pages,
+                            int page_tokens, int max_pages, const float *k_codebook, int n_bits,
+                            const uint8_t *const *qjl_pages, const float *p_rot, int m,
+                            int B, int Hq, int Hkv, int Sq, int q_start, int S, int d, float scale, int causal,
+                            const float *weights_in, int64_t weights_in_stride,
+                            float *weights_out, int64_t weights_out_stride,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
+/* The positions that stay: of each of n_streams rows of S weights (row s at
+ * weights + s * weights_stride), the first min(sink, S) and last
+ * min(recent, S) positions and the largest of the others, `keep` in all, equal
+ * weights by the lowest index, NaN below every weight; written in ascending
+ * order to kept[n_streams][keep]. min(S, sink + recent) <= keep <= S. */
+int pqkv_evict_select(const float *weights, int64_t weights_stride, int64_t n_streams, int S, int keep, int sink,
+                      int recent, int32_t *kept, void *stream);
+
+/* The move: for each of n_arrays arrays (at most PQKV_MAX_GATHER) row i of
+ * stream s in dst = row kept[s * keep + i] of stream s in src, in one launch.
+ * A row is row_bytes[a] bytes (a multiple of 4). An array is contiguous (rows
+ * of stream s from base + s * stride bytes on) or, with `pages`, paged as the
+ * caches above (row t in the page pages[s * max_pages + t / page_tokens];
+ * base and stride unused). Paged results also get zeros in rows keep ..
+ * fill - 1 (fill >= keep; contiguous results end at keep). A kept position
+ * outside 0 .. S - 1 gives a row of zeros. Bases, strides and pages are 4-byte
+ * aligned (pages 16-byte, as everywhere). dst must not overlap src. */
+#define PQKV_MAX_GATHER 6
+typedef struct pqkv_row_array {
+    const void *base;
+    const uint8_t *const *pages;
+    int64_t stride;
+    int page_tokens, max_pages;
+} pqkv_row_array;
+int pqkv_gather_rows(int n_arrays, const pqkv_row_array *src, const pqkv_row_array *dst, const int *row_bytes,
+                     const int32_t *kept, int64_t n_streams, int S, int keep, int fill, void *stream);
+
+/* Rotary positions: pair i of the first rot_dim coordinates of every head
+ * turns by positions[b][t] * freqs[i] radians and is scaled by `amplitude`;
+ * the other coordinates are copied. Pairs are (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) with interleaved = 1. inverse = 1 turns back by the same angle
+ * (with the same amplitude): the gradient. q [B][Hq][T][d] and k [B][Hkv][T][d]
+ * with element strides {sequence, head, token} (any, also 0; the last
+ * dimension is dense); q_out and k_out contiguous, and equal to q / k only
+ * where those are contiguous too. Hkv = 0: no keys. dtype PQKV_F32, PQKV_F16 or
+ * PQKV_BF16 (one for all four). positions: int64, sequence b's at positions +
+ * b * positions_stride (0: one row for all); freqs: rot_dim / 2 doubles. Angles
+ * are reduced in 64 bits. 2 <= rot_dim <= d <= 1024, rot_dim even. */
+int pqkv_rotary(const void *q, const int64_t q_strides[3], void *q_out, int Hq, const void *k,
+                const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
+                int64_t positions_stride, const double *freqs, int B, int T, int d, int rot_dim, int interleaved,
+                float amplitude, int inverse, void *stream);
+
 /* ---- dequantise -----------------------------------------------------------
  * out = (r16 c[code]) R for n block-encoded vectors: the stored radius times
  * the centroids, rotated back to the original space, each output one fp32

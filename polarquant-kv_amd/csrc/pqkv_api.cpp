@@ -513,7 +513,7 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
                     const int *k_head_bits, const int *v_head_bits, const uint8_t *qjl_signs, const float *p_rot,
                     int m, int B, int Hq, int Hkv, int S, int S_max, int d, float scale, void *out, int out_dtype,
                     void *workspace, size_t workspace_bytes, bool plan_sized, const SoaCache *soa,
-                    void *stream, const PagedCache *pg) {
+                    void *stream, const PagedCache *pg, const DecodeWeights *wt) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || S < 0 || S_max < S)
     return fail(PQKV_ERR_INVALID, "decode: B=%d Hq=%d Hkv=%d S=%d S_max=%d", B, Hq, Hkv, S, S_max);
   if (Hq % Hkv) return fail(PQKV_ERR_INVALID, "decode: Hq=%d not a multiple of Hkv=%d", Hq, Hkv);
@@ -539,6 +539,8 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(PQKV_ERR_INVALID, "decode: scale must be > 0");
   if (pg && (mixed || soa || k_bits != v_bits))
     return fail(PQKV_ERR_UNSUPPORTED, "decode: paged caches take uniform widths with k_bits == v_bits");
+  if (wt && (mixed || soa || k_bits != v_bits))
+    return fail(PQKV_ERR_UNSUPPORTED, "decode: weights take uniform widths with k_bits == v_bits");
   if (!q || (!R && !soa) || !out) return fail(PQKV_ERR_INVALID, "decode: null pointer");
   if ((uintptr_t)R % 16) return fail(PQKV_ERR_INVALID, "decode: R must be 16-byte aligned");
   if (soa && (mixed || k_bits != 4 || v_bits != 4 || qjl_signs || soa->levels < 1 || soa->levels > 16 ||
@@ -553,8 +555,8 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
   // is sized for the largest launch: all kv heads, or with mixed widths the
   // largest group of heads sharing (k bits, v bits). Heads that are all 4/4
   // (one shared codebook) or 2/2 run as one launch.
-  // (the paged and SoA modes exist only in the matrix-core kernel)
-  const bool mfma = use_mfma() || soa != nullptr || pg != nullptr;
+  // (the paged and SoA modes and the logits exist only in the matrix-core kernel)
+  const bool mfma = use_mfma() || soa != nullptr || pg != nullptr || wt != nullptr;
   int group = Hkv;
   bool pair = false;
   if (mixed) {
@@ -629,6 +631,10 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
   a.tokens_per_split = tps;
   a.split_base = 0;
   a.split_stride = splits;
+  if (wt) {
+    a.logits = wt->logits;
+    a.logit_stride = wt->logit_stride;
+  }
 
   // Query heads of a kv head in launches of at most kMaxGroup (the matrix
   // tile holds 8 heads): the group is cut into equal parts where it divides,
@@ -659,7 +665,8 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
       const int t = prof_begin("decode_split", st, true);
       hipError_t r = hipSuccess;
       for (int rep = 0, nrep = prof_repeats(); rep < nrep && r == hipSuccess; ++rep)
-        r = pg     ? launch_decode_mfma_paged(a, k_bits, st)
+        r = wt     ? launch_decode_mfma_logits(a, k_bits, st)
+            : pg   ? launch_decode_mfma_paged(a, k_bits, st)
             : soa  ? launch_decode_mfma_soa(a, st)
             : mfma ? launch_decode_mfma(a, k_bits, v_bits, st)
                    : launch_decode_split(a, k_bits, v_bits, st);
@@ -733,7 +740,11 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
   for (int rep = 0, nrep = prof_repeats(); rep < nrep && e == hipSuccess; ++rep)
     e = launch_decode_merge(part, R, out, out_dtype, B * Hq, splits, d, st);
   prof_end(tok, st);
-  return hip_status(e, "decode merge launch");
+  if (e != hipSuccess || !wt) return hip_status(e, "decode merge launch");
+  tok = prof_begin("decode_weights", st);
+  e = launch_decode_weights(a, *wt, st);
+  prof_end(tok, st);
+  return hip_status(e, "decode weights launch");
 }
 
 // Split plans of the segments of a segmented decode call (B * Hkv streams
@@ -1047,7 +1058,7 @@ int prefill_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *
 
 // ---- paged caches ----
 
-namespace {
+namespace pqkv {
 
 // log2 of a page size that is a power of two in [64, 65536], else -1
 int page_shift_of(int page_tokens) {
@@ -1072,7 +1083,7 @@ int paged_validate(const char *what, int page_tokens, int max_pages, int64_t pos
   return shift;
 }
 
-}  // namespace
+}  // namespace pqkv
 
 extern "C" {
 
@@ -1082,7 +1093,7 @@ int pqkv_encode_paged(const void *x, int x_dtype, int64_t x_outer_stride, const 
                       uint8_t *const *qjl_pages, void *stream) {
   if (start < 0) return fail(PQKV_ERR_INVALID, "encode_paged: start=%lld", (long long)start);
   if (n_streams < 0 || n_tokens < 0) return fail(PQKV_ERR_INVALID, "encode_paged: negative count");
-  const int shift = paged_validate("encode_paged", page_tokens, max_pages, start + n_tokens);
+  const int shift = pqkv::paged_validate("encode_paged", page_tokens, max_pages, start + n_tokens);
   if (shift < 0) return shift;
   // the row checks of pqkv_encode with the page tables standing in for the
   // block and sign rows
@@ -1128,7 +1139,7 @@ int pqkv_decode_attn_paged(const void *q, int q_dtype, const float *R, const uin
                            const float *v_codebook, int n_bits, const uint8_t *const *qjl_pages, const float *p_rot,
                            int m, int B, int Hq, int Hkv, int S, int d, float scale, void *out, int out_dtype,
                            void *workspace, size_t workspace_bytes, void *stream) {
-  const int shift = paged_validate("decode_paged", page_tokens, max_pages, S);
+  const int shift = pqkv::paged_validate("decode_paged", page_tokens, max_pages, S);
   if (shift < 0) return shift;
   const pqkv::PagedCache pg{k_pages, v_pages, qjl_pages, shift, max_pages};
   return pqkv::decode_attn_run(q, q_dtype, R, nullptr, nullptr, k_codebook, v_codebook, n_bits, n_bits, nullptr,
@@ -1142,7 +1153,7 @@ int pqkv_prefill_attn_paged(const void *q, int q_dtype, const float *R, const ui
                             int m, int B, int Hq, int Hkv, int Sq, int q_start, int S, int d, float scale,
                             int causal, void *out, int out_dtype, void *workspace, size_t workspace_bytes,
                             void *stream) {
-  const int shift = paged_validate("prefill_paged", page_tokens, max_pages, S);
+  const int shift = pqkv::paged_validate("prefill_paged", page_tokens, max_pages, S);
   if (shift < 0) return shift;
   const pqkv::PagedCache pg{k_pages, v_pages, qjl_pages, shift, max_pages};
   return pqkv::prefill_attn_run(q, q_dtype, R, nullptr, nullptr, k_codebook, v_codebook, n_bits, n_bits, nullptr,

@@ -337,18 +337,22 @@ struct DecodeSmem {
 // tokens (>= 64, so a 64-token chunk lies in one page) found through the
 // page tables a.k_pages / a.v_pages / a.s_pages; each chunk's loads go
 // through a buffer over its own page.
+// WS (decode with weights): every token's logit (exp2 domain) also goes to
+// a.logits, from the registers in which the softmax holds it: a lane holds
+// four consecutive tokens of one head, one 16-byte store.
 // FREE: the steady-state iteration has no scheduling fences between its
 // table reads, softmax weights and products (the mixed-width pair kernel and
 // the ggml layout, 3.5 % and 2.4 % faster that way; the other kernels are as
 // fast or faster with them).
 template <int D, int G, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GG = false, bool HW = false,
-          bool PG = false, bool FREE = false>
+          bool PG = false, bool FREE = false, bool WS = false>
 __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem<D, G, KB, VBITS, QJL, VSH> &sm,
                                                  const int split, const int bh) {
   static_assert(!SOA || (KB == 4 && VBITS == 4 && !QJL), "the SoA layout carries 4-bit codes and no QJL signs");
   static_assert(!GG || (!SOA && !QJL), "the ggml layout has block-encoded keys and values and no QJL signs");
   static_assert(!HW || GG, "one kv head per wave is a mode of the ggml layout (fp16 block radii, no listed heads)");
   static_assert(!PG || (!SOA && !GG), "paged caches hold block-encoded vectors, one token per vector slot");
+  static_assert(!WS || (!SOA && !GG), "the logits are written for block-encoded caches");
   constexpr int VBK = SOA ? D / 2 : vector_bytes(D, KB), VBV = SOA ? D / 2 : vector_bytes(D, VBITS);
   constexpr int KK = D / 16;     // score MFMAs per 16-token tile
   constexpr int NB = D / 16;     // value n-tiles
@@ -422,6 +426,24 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     } else {
       rel = t0;
       return whole;
+    }
+  };
+
+  // WS: the logit rows of this launch's heads; a lane's store starts
+  // l_off + 4 t0 bytes in (past the end, so dropped, where it holds no head)
+  __amdgpu_buffer_rsrc_t lres = kres;
+  uint32_t l_off = 0;
+  if constexpr (WS) {
+    const uint32_t row_bytes = (uint32_t)a.logit_stride * 4u;
+    lres = stream_rsrc((const uint8_t *)(a.logits + (int64_t)(b * a.Hq + h * a.gq + a.q_off) * a.logit_stride),
+                       (uint32_t)G * row_bytes);
+    const int head = kCompact ? (col & 3) : col;
+    l_off = head < G ? (uint32_t)head * row_bytes + 16u * grp + (kCompact ? 64u * (col >> 2) : 0u) : 0xFFFFFFF0u;
+  }
+  auto store_logits = [&](int t0, int sub, float4_t v) {
+    if constexpr (WS) {
+      const uint32_t off = l_off == 0xFFFFFFF0u ? l_off : l_off + 4u * (uint32_t)t0 + 64u * (uint32_t)sub;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), lres, (int)off, 0, 0);
     }
   };
 
@@ -714,9 +736,9 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     uint32_t top[kCompact ? 4 : 1], bot[kCompact ? 4 : 1];  // compact weights: (p_hi, 0), (p_lo, p_hi)
   };
   // rks (kRawScores): this lane's loaded key radius of the chunk in sc; mk
-  // (GG): its mask words of that chunk.
+  // (GG): its mask words of that chunk; t0: its first position.
   auto fbegin = [&](float (&sv)[NSUB][4], const float4_t (&sc)[NSUB], int ntok, bool partial, float rvl, float rks,
-                    const uint32_t (&mk)[MC]) {
+                    const uint32_t (&mk)[MC], int t0) {
     FState f;
     float cmax;
     float cv[4];
@@ -739,6 +761,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
         if constexpr (GG) c = __builtin_fmaf(mask_val(mk, i), kLog2eF, c);  // the logits are in the exp2 domain
         cv[i] = partial && kSub * (col >> 2) + 4 * grp + i >= ntok ? -INFINITY : c;
       }
+      store_logits(t0, 0, (float4_t){cv[0], cv[1], cv[2], cv[3]});
       cmax = fmaxf(fmaxf(cv[0], cv[1]), fmaxf(cv[2], cv[3]));
       cmax = fmaxf(cmax, __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, cmax), 0x124, 0xF, 0xF, true)));
       cmax = fmaxf(cmax, __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, cmax), 0x128, 0xF, 0xF, true)));
@@ -754,6 +777,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
           for (int i = 0; i < 4; ++i)
             if (kSub * st + 4 * grp + i >= ntok) sv[st][i] = -INFINITY;
       }
+#pragma unroll
+      for (int st = 0; st < NSUB; ++st) store_logits(t0, st, (float4_t){sv[st][0], sv[st][1], sv[st][2], sv[st][3]});
       cmax = sv[0][0];
 #pragma unroll
       for (int st = 0; st < NSUB; ++st)
@@ -869,10 +894,10 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   };
   // Softmax update and value product of a whole chunk (the last one).
   auto finish = [&](const CV &v, const float4_t (&sc)[NSUB], float rks, const uint32_t (&mks)[MC],
-                    int ntok, bool partial) {
+                    int ntok, bool partial, int t0) {
     float sv[NSUB][4];
     const float rvl = rad(v.r);
-    FState f = fbegin(sv, sc, ntok, partial, rvl, rks, mks);
+    FState f = fbegin(sv, sc, ntok, partial, rvl, rks, mks, t0);
     VTile vt[2];
     vread(v, 0, vt[0]);
 #pragma unroll
@@ -888,11 +913,12 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   // tiles' table reads are issued first, the softmax weights are computed
   // while they are in flight, then the two products run.
   // One iteration; k and v are reloaded in place with the chunks at tk and
-  // tv. With kPieceLoads the pieces go out as the iteration consumes them
+  // tv (the chunk after the one it finishes). With kPieceLoads the pieces go out as the iteration consumes them
   // (loads complete in order, so the next iteration's first reads wait only
   // for the first loads: config 4 28.3 -> 27.3 us); the QJL kernels with
   // G > 4 would spill with that schedule and reload after the iteration.
   constexpr bool kPieceLoads = !QJL || G <= 4;
+  constexpr int kStep = HW ? kChunk : kMWaves * kChunk;   // from one of the wave's chunks to the next
   auto step = [&](CK &k, CV &v, const float4_t (&sc)[NSUB], float rks, const uint32_t (&mks)[MC],
                   float4_t (&sn)[NSUB], float &rkn, uint32_t (&mkn)[MC], int tk, int tv) {
     float sv[NSUB][4];
@@ -907,7 +933,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     }
 #pragma unroll
     for (int j = 0; j < MC; ++j) mkn[j] = k.mw[j];
-    FState f = fbegin(sv, sc, kChunk, false, rvl, rks, mks);
+    FState f = fbegin(sv, sc, kChunk, false, rvl, rks, mks, tv - kStep);
 #pragma unroll
     for (int j = 0; j < NSUB; ++j) {
       KTile kt;
@@ -948,7 +974,6 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   // work. The key registers are reloaded with chunk i + 2 and the value
   // registers with chunk i + 1. Only the last chunk can be partial; it is
   // finished after the loop.
-  constexpr int kStep = HW ? kChunk : kMWaves * kChunk;
   // (PG: through a scalar register, so that the chunk positions and with
   // them the page addresses are known to be wave-uniform)
   const int first = t_begin + (HW ? 0 : (PG ? __builtin_amdgcn_readfirstlane(wave) : wave) * kChunk);
@@ -976,7 +1001,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
       for (int j = 0; j < MC; ++j) mks[j] = mkn[j];
     }
     const int tlast = first + (nch - 1) * kStep;
-    finish(cv, sacc, rks, mks, min(kChunk, t_end - tlast), true);
+    finish(cv, sacc, rks, mks, min(kChunk, t_end - tlast), true, tlast);
   }
 
   // ---------------- per-wave results ----------------
@@ -1055,14 +1080,14 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
 // HW: workgroup row y takes the pairs 4y .. 4y + 3, one per wave (n_heads a
 // multiple of 4, so the four share the batch row).
 template <int D, int G, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GG = false, bool HW = false,
-          bool PG = false>
+          bool PG = false, bool WS = false>
 __global__ void __launch_bounds__(256, kMfmaBlocksPerCU) decode_mfma_kernel(const DecodeArgs a) {
   __shared__ DecodeSmem<D, G, KB, VBITS, QJL, VSH> sm;
   // (read through a scalar register: the buffer resources built from the
   // pair must be wave-uniform, or every load becomes a loop over lanes)
   const int bh = HW ? __builtin_amdgcn_readfirstlane((int)blockIdx.y * kMWaves + (int)(threadIdx.x >> 6))
                     : (int)blockIdx.y;
-  decode_mfma_body<D, G, KB, VBITS, QJL, VSH, SOA, GG, HW, PG, GG>(a, sm, blockIdx.x, bh);
+  decode_mfma_body<D, G, KB, VBITS, QJL, VSH, SOA, GG, HW, PG, GG, WS>(a, sm, blockIdx.x, bh);
 }
 
 // Mixed widths whose kv heads are either 4-bit keys and values (a4, one
@@ -1102,25 +1127,25 @@ __global__ void __launch_bounds__(256, kMfmaBlocksPerCU) decode_mfma_pair_kernel
   }
 
 template <int D, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GGML = false, bool HW = false,
-          bool PG = false>
+          bool PG = false, bool WS = false>
 static void launch_dm(const DecodeArgs &a, int G, hipStream_t s) {
   dim3 grid(a.splits, HW ? a.B * a.n_heads / kMWaves : a.B * a.n_heads);
-#define PQKV_DM_ONE(GG, ...) decode_mfma_kernel<D, GG, KB, VBITS, QJL, VSH, SOA, GGML, HW, PG><<<grid, 256, 0, s>>>(a)
+#define PQKV_DM_ONE(GG, ...) decode_mfma_kernel<D, GG, KB, VBITS, QJL, VSH, SOA, GGML, HW, PG, WS><<<grid, 256, 0, s>>>(a)
   PQKV_DM_G_SWITCH(PQKV_DM_ONE, 0)
 #undef PQKV_DM_ONE
 }
 
 // One width pair on both head dims, with or without QJL (PG: paged caches,
-// whose QJL signs come through a.s_pages).
-template <int KB, int VBITS, bool VSH = false, bool PG = false>
+// whose QJL signs come through a.s_pages; WS: the logits written too).
+template <int KB, int VBITS, bool VSH = false, bool PG = false, bool WS = false>
 static hipError_t launch_dm_widths(const DecodeArgs &a, hipStream_t s) {
   const bool qjl = PG ? a.s_pages != nullptr : a.qjl != nullptr;
   if (a.d == 128) {
-    if (qjl) launch_dm<128, KB, VBITS, true, VSH, false, false, false, PG>(a, a.g, s);
-    else launch_dm<128, KB, VBITS, false, VSH, false, false, false, PG>(a, a.g, s);
+    if (qjl) launch_dm<128, KB, VBITS, true, VSH, false, false, false, PG, WS>(a, a.g, s);
+    else launch_dm<128, KB, VBITS, false, VSH, false, false, false, PG, WS>(a, a.g, s);
   } else {
-    if (qjl) launch_dm<64, KB, VBITS, true, VSH, false, false, false, PG>(a, a.g, s);
-    else launch_dm<64, KB, VBITS, false, VSH, false, false, false, PG>(a, a.g, s);
+    if (qjl) launch_dm<64, KB, VBITS, true, VSH, false, false, false, PG, WS>(a, a.g, s);
+    else launch_dm<64, KB, VBITS, false, VSH, false, false, false, PG, WS>(a, a.g, s);
   }
   return hipGetLastError();
 }
@@ -1136,5 +1161,12 @@ hipError_t launch_dm_k2v2(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_paged_k4v4_shared(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_paged_k4v4_own(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_paged_k2v2(const DecodeArgs &a, hipStream_t s);
+// The same six with the logits written.
+hipError_t launch_dm_logits_k4v4_shared(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_logits_k4v4_own(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_logits_k2v2(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_logits_paged_k4v4_shared(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_logits_paged_k4v4_own(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_logits_paged_k2v2(const DecodeArgs &a, hipStream_t s);
 
 }  // namespace pqkv

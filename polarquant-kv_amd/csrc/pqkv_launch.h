@@ -90,6 +90,10 @@ struct DecodeArgs {
   // pages s_pages, alike); page_shift >= 6, so a 64-token chunk lies in one page.
   const uint8_t *const *k_pages, *const *v_pages, *const *s_pages;
   int page_shift, max_pages;
+  // The kernels' WS mode: the logits (exp2 domain) of every token, row
+  // b * Hq + head of logit_stride floats (a multiple of 64, at least S).
+  float *logits;
+  int64_t logit_stride;
   int16_t heads[kMaxListHeads];
   int64_t k_head_off[kMaxListHeads], v_head_off[kMaxListHeads];
 };
@@ -146,6 +150,16 @@ struct PagedCache {
   const uint8_t *const *k_pages, *const *v_pages, *const *s_pages;
   int page_shift, max_pages;
 };
+// The weights a decode call also gives (pqkv_decode_attn_weights): room for
+// the logits, and the accumulated weights of every cached position.
+struct DecodeWeights {
+  float *logits;
+  int64_t logit_stride;
+  const float *in;            // or null
+  int64_t in_stride;          // floats between (batch, kv-head) streams
+  float *out;
+  int64_t out_stride;
+};
 // The validated decode call behind pqkv_decode_attn (plan_sized = false: the
 // workspace must hold pqkv_decode_workspace_bytes) and the allocation-free
 // entry point (plan_sized = true: the workspace must hold this call's plan).
@@ -156,7 +170,7 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
                     const int *k_head_bits, const int *v_head_bits, const uint8_t *qjl_signs, const float *p_rot,
                     int m, int B, int Hq, int Hkv, int S, int S_max, int d, float scale, void *out, int out_dtype,
                     void *workspace, size_t workspace_bytes, bool plan_sized, const SoaCache *soa,
-                    void *stream, const PagedCache *pg = nullptr);
+                    void *stream, const PagedCache *pg = nullptr, const DecodeWeights *wt = nullptr);
 // The validated call behind pqkv_prefill_attn (pg: pqkv_prefill_attn_paged).
 int prefill_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const uint8_t *v_cache,
                      const float *k_codebooks, const float *v_codebooks, int k_bits, int v_bits,
@@ -179,6 +193,10 @@ int decode_segments_run(const void *q, int q_dtype, const float *R, int n_seg, c
 int report_hip_error(hipError_t e, const char *what);
 // Sets the thread's error message (printf format); returns code.
 int fail_status(int code, const char *fmt, ...);
+// Shared checks of the paged entry points: the page size, and a table wide
+// enough for `positions` tokens per stream. Returns the page shift, or a
+// negative status.
+int paged_validate(const char *what, int page_tokens, int max_pages, int64_t positions);
 // The matrix-core decode kernel's split plan for `streams` (batch, kv-head)
 // streams of S tokens: one balanced round of workgroups.
 void mfma_split_plan(int64_t streams, int S, int *splits, int *tps);
@@ -253,6 +271,12 @@ hipError_t launch_decode_mfma(const DecodeArgs &a, int k_bits, int v_bits, hipSt
 // Paged caches (a.k_pages, a.v_pages, a.s_pages; uniform widths, keys and
 // values of `bits` each).
 hipError_t launch_decode_mfma_paged(const DecodeArgs &a, int bits, hipStream_t s);
+// The same kernels writing a.logits (keys and values of `bits` each, contiguous
+// or, with a.k_pages, paged).
+hipError_t launch_decode_mfma_logits(const DecodeArgs &a, int bits, hipStream_t s);
+// weights_out = weights_in + the softmax weights of a decode call, summed over
+// each kv head's query heads, from its logits and its splits' partials.
+hipError_t launch_decode_weights(const DecodeArgs &a, const DecodeWeights &w, hipStream_t s);
 // Mixed widths with kv heads of exactly two kinds, 4-bit K and V sharing one
 // codebook (a4) and 2-bit K and V (a2): one launch over both head lists.
 hipError_t launch_decode_mfma_pair(const DecodeArgs &a4, const DecodeArgs &a2, hipStream_t s);
@@ -352,6 +376,68 @@ hipError_t launch_prefill_planes(PrefillArgs a, int k_bits, int v_bits, const Pr
                                  hipStream_t s);
 // Joins a split launch's partials into a.o (streams stream0 .. + ns - 1).
 hipError_t launch_prefill_merge(const PrefillArgs &a, int stream0, int ns, int rows, hipStream_t s);
+// Weights of a chunk's rows (pqkv_attn_weights): row i * G + g of stream
+// (b, kv head) is query token i of the group's head g.
+struct AttnWeightsArgs {
+  const float *q, *pq;           // [B][Hq][Sq][d] fp32, rotated, times scale*log2(e); projections (QJL) or null
+  const uint8_t *k_cache;        // [B][Hkv][S_max] vectors, or pages as in DecodeArgs
+  const uint8_t *qjl;
+  const uint8_t *const *k_pages, *const *s_pages;
+  int page_shift, max_pages;
+  const float *codebook;         // [16]
+  int bits, B, Hq, Hkv, G, Sq, q_start, S, S_max, d, causal;
+  int row0, rows;                // this pass's rows of every stream (row0 a multiple of G)
+  int tblocks, chunks;           // token blocks; row chunks of kWeightRows rows
+  float2 *part;                  // [stream][tblock][rows]: maximum and sum over the block's tokens
+  float2 *stat;                  // [stream][rows]: maximum and 1 / sum over all tokens
+  float *col;                    // [stream][chunk][tblocks * kWeightTokens]: sums over a chunk's rows
+  const float *in;
+  int64_t in_stride;
+  float *out;
+  int64_t out_stride;
+};
+constexpr int kWeightTokens = 256;   // tokens per workgroup
+constexpr int kWeightRows = 2048;    // rows per workgroup
+hipError_t launch_attn_weights(const AttnWeightsArgs &a, hipStream_t s);
+// out = in (or zeros) for S tokens of every stream.
+hipError_t launch_weights_copy(const float *in, int64_t in_stride, float *out, int64_t out_stride, int64_t streams,
+                               int S, hipStream_t s);
+
+// Rotary positions (pqkv_rotary); strides in elements between sequences,
+// heads and tokens.
+struct RotaryArgs {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_stride[3], k_stride[3];
+  const int64_t *positions;
+  int64_t pos_batch_stride;
+  const double *freqs;
+  int B, Hq, Hkv, T, d, rot_dim, interleaved, inverse;
+  float amplitude;
+};
+hipError_t launch_rotary(const RotaryArgs &a, int dtype, hipStream_t s);
+
+// Eviction: selection, and the move of up to PQKV_MAX_GATHER arrays' rows.
+hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_streams, int S, int keep, int sink,
+                               int recent, int *kept, hipStream_t s);
+struct GatherPart {
+  const uint8_t *src;
+  const uint8_t *const *src_pages;   // or null: contiguous
+  uint8_t *dst;
+  uint8_t *const *dst_pages;
+  int64_t src_stride, dst_stride;    // bytes between streams
+  int src_shift, src_max_pages, dst_shift, dst_max_pages;
+  int row_bytes, unit;
+};
+constexpr int kMaxGather = PQKV_MAX_GATHER;
+struct GatherArgs {
+  GatherPart part[kMaxGather];
+  int n_parts;
+  const int *kept;                   // [stream][keep]
+  int S, keep, fill;                 // source positions; result rows; rows written (those past keep with zeros)
+};
+hipError_t launch_gather_rows(const GatherArgs &a, int64_t n_streams, hipStream_t s);
+
 // Query rows per prefill workgroup (the QJL kernel holds 16 rows per wave
 // instead of 32, to make room for the projection operands).
 int prefill_rows_per_block(bool qjl);

@@ -7,6 +7,7 @@ fallback for the hot path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -23,6 +24,16 @@ c_void_p, c_int, c_int64, c_float, c_size_t = (ctypes.c_void_p, ctypes.c_int, ct
 c_int_p, c_float_p = ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_float)
 c_int64_4, c_size_4 = ctypes.c_int64 * 4, ctypes.c_size_t * 4      # ggml ne / nb arrays
 c_int64_p, c_size_p = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_size_t)
+
+
+
+class RowArray(ctypes.Structure):
+    """pqkv_row_array: one array of rows, contiguous or paged."""
+    _fields_ = [("base", c_void_p), ("pages", c_void_p), ("stride", c_int64), ("page_tokens", c_int),
+                ("max_pages", c_int)]
+
+
+MAX_GATHER = 6                          # PQKV_MAX_GATHER
 
 # name -> (restype, argtypes); the full exported surface of include/pqkv.h
 SIGNATURES = {
@@ -92,6 +103,28 @@ SIGNATURES = {
                                      c_int64, c_int, c_void_p]),
     "pqkv_soa_to_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "pqkv_blocks_to_soa": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "pqkv_decode_attn_weights_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "pqkv_decode_attn_weights": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                         c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t,
+                                         c_void_p]),
+    "pqkv_decode_attn_weights_paged": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                                               c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                               c_int, c_float, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                               c_void_p, c_size_t, c_void_p]),
+    "pqkv_attn_weights_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "pqkv_attn_weights": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                  c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                                  c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "pqkv_attn_weights_paged": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p,
+                                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                        c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "pqkv_evict_select": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "pqkv_gather_rows": (c_int, [c_int, ctypes.POINTER(RowArray), ctypes.POINTER(RowArray), c_int_p, c_void_p, c_int64,
+                                 c_int, c_int, c_int, c_void_p]),
+    "pqkv_rotary": (c_int, [c_void_p, c_int64_p, c_void_p, c_int, c_void_p, c_int64_p, c_void_p, c_int, c_int,
+                            c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                            c_void_p]),
     "pqkv_profile_enable": (c_int, [c_int]),
     "pqkv_profile_repeat": (c_int, [c_int]),
     "pqkv_profile_stream_read": (c_int, [c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
@@ -178,6 +211,22 @@ def require_device(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("GPU entry points take device tensors (the hot path has no CPU fallback)")
+
+
+def require_one_device(*tensors) -> None:
+    """The tensors a call reads and writes are on one device."""
+    where = [t.device for t in tensors if t is not None]
+    if any(d != where[0] for d in where):
+        raise ValueError(f"tensors on several devices: {sorted({str(d) for d in where})}")
+
+
+def on_device(t):
+    """Context in which kernels launch on the tensor's device, whichever is
+    current."""
+    import torch
+    if torch.cuda.current_device() == t.device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def workspace(best: int, least, device):

@@ -149,6 +149,126 @@ def _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype
     return out
 
 
+def _weights_args(B, H, S, previous, into, device):
+    """(previous, into, result) of a call that gives weights: the tensors it
+    reads and writes, rows [B, H] one stride apart, and the [B, H, S] result."""
+    from .eviction import _check_rows
+    for name, t in (("previous", previous), ("into", into)):
+        if t is None:
+            continue
+        if t.dim() != 3 or t.shape[:2] != (B, H) or t.shape[2] < S or t.dtype != torch.float32:
+            raise ValueError(f"{name} must be [{B}, {H}, >= {S}] float32, got {tuple(t.shape)} {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the query on {device}")
+    if previous is not None:
+        previous = _check_rows(previous, "previous")
+    if into is None:
+        into = torch.empty(B, H, S, dtype=torch.float32, device=device)
+    elif _check_rows(into, "into") is not into:
+        raise ValueError("into must have dense rows one stride apart")
+    return previous, into, into[:, :, :S]
+
+
+def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix: torch.Tensor,
+                             scale: float | None = None, jl_rot: torch.Tensor | None = None,
+                             out_dtype: torch.dtype | None = None, previous: torch.Tensor | None = None,
+                             into: torch.Tensor | None = None):
+    """decode_attention, and the softmax weight of each cached position summed
+    over its kv head's query heads: -> (out [B, Hq, d], weights [B, Hkv, S]
+    float32). previous ([B, Hkv, >= S] float32) is added to the weights; into
+    (same shape; may be previous itself) receives them, positions from S on
+    left as they are. keys / values: PQCache or PagedPQCache of one and the
+    same width (pqkv_decode_attn_weights, _paged)."""
+    from .eviction import _row_stride
+    if query.dim() != 3:
+        raise ValueError(f"query must be [B, Hq, d], got {tuple(query.shape)}")
+    B, Hq, d = query.shape
+    paged = isinstance(keys, PagedPQCache) or isinstance(values, PagedPQCache)
+    Hkv = (check_paged if paged else check_shapes)(B, Hq, d, keys, values, rotation_matrix)
+    if keys.mixed or values.mixed or keys.n_bits != values.n_bits:
+        raise ValueError("weights take keys and values of one and the same width")
+    _lib.require_device(query, rotation_matrix, jl_rot)
+    _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks)
+    if jl_rot is not None and keys.qjl_signs is None:
+        raise ValueError("QJL correction requested but the key cache has no signs")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    out_dtype = query.dtype if out_dtype is None else out_dtype
+    S = keys.seq_len
+    previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
+    q = query.contiguous()
+    R = rotation_matrix.to(torch.float32).contiguous()
+    P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    out = torch.empty(B, Hq, d, dtype=out_dtype, device=q.device)
+    lib = _lib.lib()
+    ws = torch.empty(lib.pqkv_decode_attn_weights_workspace_bytes(B, Hq, Hkv, max(S, 1), d), dtype=torch.uint8,
+                     device=q.device)
+    kcb, vcb = (keys.codebooks, values.codebooks) if paged else _codebook_tables(keys, values, False, Hkv)
+    tail = (_lib.ptr(previous), 0 if previous is None else _row_stride(previous), into.data_ptr(), _row_stride(into),
+            ws.data_ptr(), ws.numel(), _lib.stream_of(q))
+    with _lib.on_device(q):
+        if paged:
+            _lib.check(lib.pqkv_decode_attn_weights_paged(
+                q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),
+                keys.page_tokens, keys.max_pages, kcb.data_ptr(), vcb.data_ptr(), keys.n_bits,
+                keys.sign_table.data_ptr() if P is not None else None, _lib.ptr(P), d if P is not None else 0, B, Hq,
+                Hkv, S, d, scale, out.data_ptr(), _lib.dtype_code(out_dtype), *tail))
+        else:
+            _lib.check(lib.pqkv_decode_attn_weights(
+                q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.blocks.data_ptr(), values.blocks.data_ptr(),
+                kcb.data_ptr(), vcb.data_ptr(), keys.n_bits, keys.qjl_signs.data_ptr() if P is not None else None,
+                _lib.ptr(P), d if P is not None else 0, B, Hq, Hkv, S, keys.max_seq_len, d, scale, out.data_ptr(),
+                _lib.dtype_code(out_dtype), *tail))
+    return out, result
+
+
+def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, q_start: int, causal: bool = True,
+                      scale: float | None = None, jl_rot: torch.Tensor | None = None,
+                      previous: torch.Tensor | None = None, into: torch.Tensor | None = None) -> torch.Tensor:
+    """The softmax weight that a chunk of query tokens [B, Hq, Sq, d] at
+    positions q_start .. gives each cached position, summed over the tokens and
+    the kv head's query heads: -> [B, Hkv, S] float32, plus previous, into
+    `into` where given (both as decode_attention_weights takes them). keys:
+    PQCache (one width) or PagedPQCache that already holds the chunk; causal as
+    prefill_attention (pqkv_attn_weights, _paged)."""
+    from .eviction import _row_stride
+    if query.dim() != 4:
+        raise ValueError(f"query must be [B, Hq, Sq, d], got {tuple(query.shape)}")
+    B, Hq, Sq, d = query.shape
+    paged = isinstance(keys, PagedPQCache)
+    Hkv = (check_paged if paged else check_shapes)(B, Hq, d, keys, keys, rotation_matrix)
+    if keys.mixed:
+        raise ValueError("weights take keys of one width")
+    _lib.require_device(query, rotation_matrix, jl_rot)
+    _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks)
+    if jl_rot is not None and keys.qjl_signs is None:
+        raise ValueError("QJL correction requested but the key cache has no signs")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    S = keys.seq_len
+    previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
+    q = query.contiguous()
+    R = rotation_matrix.to(torch.float32).contiguous()
+    P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    lib = _lib.lib()
+    ws = torch.empty(max(1, lib.pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d)), dtype=torch.uint8,
+                     device=q.device)
+    tail = (scale, int(causal), _lib.ptr(previous), 0 if previous is None else _row_stride(previous), into.data_ptr(),
+            _row_stride(into), ws.data_ptr(), ws.numel(), _lib.stream_of(q))
+    head = (q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr())
+    with _lib.on_device(q):
+        if paged:
+            _lib.check(lib.pqkv_attn_weights_paged(
+                *head, keys.table.data_ptr(), keys.page_tokens, keys.max_pages, keys.codebooks.data_ptr(), keys.n_bits,
+                keys.sign_table.data_ptr() if P is not None else None, _lib.ptr(P), d if P is not None else 0, B, Hq,
+                Hkv, Sq, q_start, S, d, *tail))
+        else:
+            cb = keys.codebooks.contiguous()
+            _lib.check(lib.pqkv_attn_weights(
+                *head, keys.blocks.data_ptr(), cb.data_ptr(), keys.n_bits,
+                keys.qjl_signs.data_ptr() if P is not None else None, _lib.ptr(P), d if P is not None else 0, B, Hq,
+                Hkv, Sq, q_start, S, keys.max_seq_len, d, *tail))
+    return result
+
+
 def decode_attention_segments(query: torch.Tensor, segments: list, rotation_matrix: torch.Tensor,
                               scale: float | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """query [B, Hq, d] against the tokens of several (keys, values) cache

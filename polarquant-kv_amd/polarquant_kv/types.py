@@ -183,6 +183,31 @@ class PagedPQCache:
                 self.sign_groups.append(sg)
                 self.sign_table[:, p] = sg.data_ptr() + streams * (P * (self.jl_dim // 8))
 
+    def reserve(self, positions: int) -> None:
+        """The pages of a cache that has none yet, for `positions` positions, in
+        one allocation whose bytes are not set: for a writer that fills every
+        page to its end."""
+        import torch
+        if self._adopted is not None or self.groups:
+            raise ValueError("reserve() is for a cache without pages")
+        n = -(-int(positions) // self.page_tokens)
+        if n == 0:
+            return
+        self._widen(n)
+        B, H, P = self.batch, self.num_heads, self.page_tokens
+
+        def pages(row_bytes, table):
+            g = torch.empty(n, B, H, P, row_bytes, dtype=torch.uint8, device=self.device)
+            size = P * row_bytes
+            # page p of stream s: page number p * B * H + s
+            at = torch.arange(g.data_ptr(), g.data_ptr() + n * B * H * size, size, device=self.device)
+            table[:, :n] = at.view(n, B * H).t()
+            return list(g.unbind(0))
+
+        self.groups = pages(self.vector_bytes, self.table)
+        if self.sign_table is not None:
+            self.sign_groups = pages(self.jl_dim // 8, self.sign_table)
+
     def memory_bytes(self) -> int:
         """Device bytes of the allocated pages (and the page tables)."""
         n = sum(g.numel() for g in self.groups) + sum(g.numel() for g in self.sign_groups)
