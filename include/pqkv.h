@@ -374,7 +374,7 @@ int pqkv_prefill_attn(const void *q, int q_dtype, const float *R,
  * weights_*_stride floats in (a stride of at least S); weights_out may be
  * weights_in with the same stride, and may not overlap it otherwise. Keys and
  * values of one width n_bits (2 or 4), no per-head widths; S = 0 writes zeros
- * to out and no weights. S < 2^24. The output equals pqkv_decode_attn's bit
+ * to out and no weights. S < 2^24, groups Hq / Hkv of up to 1024. The output equals pqkv_decode_attn's bit
  * for bit. */
 size_t pqkv_decode_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int d);
 int pqkv_decode_attn_weights(const void *q, int q_dtype, const float *R,
@@ -403,10 +403,10 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * weights_in[b][h][t] + sum over kv head h's query heads and the Sq tokens of
  * softmax(s)_t, arguments as pqkv_prefill_attn and pqkv_decode_attn_weights
  * (keys only: no values are read). Sq = 0 copies weights_in (or writes zeros);
- * S = 0 writes nothing. Any group size Hq / Hkv. The workspace needs no
- * initialisation; its size does not grow past about 600 MB plus the rotated
- * queries (long chunks run in passes). */
-size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d);
+ * S = 0 writes nothing. Groups Hq / Hkv of up to 1024, S < 2^24. The workspace
+ * (qjl: with signs) needs no initialisation; past the rotated queries it stays
+ * below 1 GB (long chunks run in passes). */
+size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
                       int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,
                       int B, int Hq, int Hkv, int Sq, int q_start, int S, int S_max, int d, float scale, int causal,

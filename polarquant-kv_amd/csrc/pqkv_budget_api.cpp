@@ -67,35 +67,47 @@ int decode_weights_run(const void *q, int q_dtype, const float *R, const uint8_t
                                stream, pg, &wt);
 }
 
-// Workspace of a chunk's weights: rotated queries and projections, then what
-// one pass over `rows` rows of every stream needs.
+// One pass of a chunk's weights over `rows` rows of every stream, and its
+// workspace: rotated queries (and projections), the rows' records and factors,
+// the token blocks' partials, the rows' statistics, the row chunks' sums.
 struct WeightsPlan {
-  int tblocks, rows, chunks;
-  size_t q, part, stat, col;
-  size_t bytes() const { return 2 * q + part + stat + col; }
+  int tblocks, rows, chunk_rows;
+  size_t q, pq, records, factor, part, stat, col;
+  size_t bytes() const { return q + pq + records + factor + part + stat + col; }
+  int chunks(int r) const { return (r + chunk_rows - 1) / chunk_rows; }
 };
-WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d) {
+int row_tiles(int rows) { return (rows + 31) / 32 * 2; }
+WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl) {
   WeightsPlan p;
-  const int64_t streams = (int64_t)B * Hkv;
-  const int G = Hq / Hkv;
-  p.tblocks = (S + pqkv::kWeightTokens - 1) / pqkv::kWeightTokens;
-  // rows of a pass: the token blocks' partials stay within 256 MB
-  int64_t rows = (256 << 20) / (streams * p.tblocks * (int64_t)sizeof(float2)) / G * G;
-  rows = std::max<int64_t>(rows, G);
-  p.rows = (int)std::min<int64_t>(rows, (int64_t)Sq * G);
-  p.chunks = (p.rows + pqkv::kWeightRows - 1) / pqkv::kWeightRows;
+  const int64_t streams = (int64_t)B * Hkv, total = (int64_t)Sq * (Hq / Hkv);
+  const int tokens = pqkv::weight_tokens(qjl);
+  p.tblocks = (S + tokens - 1) / tokens;
+  // rows of a pass: partials within 256 MB, records within 512 MB
+  const int64_t rec_row = (int64_t)d * (qjl ? 8 : 4);
+  int64_t rows = std::min((int64_t)(256 << 20) / (streams * p.tblocks * (int64_t)sizeof(float2)),
+                          (int64_t)(512 << 20) / (streams * rec_row));
+  rows = std::max<int64_t>(rows / 32 * 32, 32);
+  p.rows = (int)std::min(rows, total);
+  // rows of a workgroup: about 2048 workgroups (four rounds of two per compute
+  // unit); at least 128 rows, under which decoding the keys is most of the work,
+  // at most 2048, whose records (1 MB at d = 128) a group of workgroups shares in L2
+  const int64_t want = p.rows * streams * p.tblocks / 2048;
+  p.chunk_rows = (int)std::min<int64_t>(std::max<int64_t>((want + 31) / 32 * 32, 128), 2048);
   p.q = align256((size_t)B * Hq * Sq * d * 4);
+  p.pq = qjl ? p.q : 0;
+  p.records = align256((size_t)streams * row_tiles(p.rows) * 16 * rec_row);
+  p.factor = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float));
   p.part = align256((size_t)streams * p.tblocks * p.rows * sizeof(float2));
   p.stat = align256((size_t)streams * p.rows * sizeof(float2));
-  p.col = align256((size_t)streams * p.chunks * p.tblocks * pqkv::kWeightTokens * sizeof(float));
+  p.col = align256((size_t)streams * p.chunks(p.rows) * p.tblocks * tokens * sizeof(float));
   return p;
 }
 
 bool weights_shape_ok(int B, int Hq, int Hkv, int Sq, int S, int d) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || S <= 0 || Hq % Hkv || (d != 64 && d != 128)) return false;
   const int G = Hq / Hkv;
-  const int64_t tblocks = ((int64_t)S + pqkv::kWeightTokens - 1) / pqkv::kWeightTokens;
-  // grids and row numbers within 31 bits
+  const int64_t tblocks = ((int64_t)S + 127) / 128;
+  // grids, row numbers and positions within 31 bits
   return S < kMaxTokens && G <= kMaxGroupWeights && (int64_t)Sq * G < INT_MAX / 2 &&
          (int64_t)B * Hkv * tblocks <= (1 << 24) && (int64_t)B * Hq * Sq <= ((int64_t)1 << 40) / d;
 }
@@ -135,12 +147,17 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
     return fail_status(PQKV_ERR_INVALID, "attn_weights: null pointer");
   if ((uintptr_t)R % 16 || (uintptr_t)p_rot % 16)
     return fail_status(PQKV_ERR_INVALID, "attn_weights: R and p_rot must be 16-byte aligned");
-  const WeightsPlan p = weights_plan(B, Hq, Hkv, Sq, S, d);
+  const WeightsPlan p = weights_plan(B, Hq, Hkv, Sq, S, d, has_qjl);
   if (!ws || ws_bytes < p.bytes())
     return fail_status(PQKV_ERR_WORKSPACE, "attn_weights: workspace %zu < %zu bytes", ws_bytes, p.bytes());
   if ((uintptr_t)ws % 16) return fail_status(PQKV_ERR_INVALID, "attn_weights: workspace must be 16-byte aligned");
   char *w = (char *)ws;
-  float *q32 = (float *)w, *pq32 = (float *)(w + p.q);
+  auto take = [&](size_t bytes) {
+    char *at = w;
+    w += bytes;
+    return at;
+  };
+  float *q32 = (float *)take(p.q), *pq32 = (float *)take(p.pq);
   const int64_t nvec = (int64_t)B * Hq * Sq;
   const float qs = scale * 1.4426950408889634f;
   int tok = pqkv::prof_begin("weights_rotate", st);
@@ -173,16 +190,20 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
   a.d = d;
   a.causal = causal ? 1 : 0;
   a.tblocks = p.tblocks;
-  a.part = (float2 *)(w + 2 * p.q);
-  a.stat = (float2 *)(w + 2 * p.q + p.part);
-  a.col = (float *)(w + 2 * p.q + p.part + p.stat);
+  a.chunk_rows = p.chunk_rows;
+  a.records = (uint8_t *)take(p.records);
+  a.row_factor = (float *)take(p.factor);
+  a.part = (float2 *)take(p.part);
+  a.stat = (float2 *)take(p.stat);
+  a.col = (float *)take(p.col);
   a.out = out;
   a.out_stride = out_stride;
   const int total = Sq * a.G;
   for (int row0 = 0; row0 < total; row0 += p.rows) {
     a.row0 = row0;
     a.rows = std::min(p.rows, total - row0);
-    a.chunks = (a.rows + pqkv::kWeightRows - 1) / pqkv::kWeightRows;
+    a.row_tiles = row_tiles(a.rows);
+    a.chunks = p.chunks(a.rows);
     a.in = row0 ? out : in;
     a.in_stride = row0 ? out_stride : in_stride;
     tok = pqkv::prof_begin("attn_weights", st);
@@ -229,9 +250,9 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R, c
                             weights_out_stride, workspace, workspace_bytes, stream, &pg);
 }
 
-size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d) {
+size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl) {
   if (!weights_shape_ok(B, Hq, Hkv, Sq, S, d)) return 0;
-  return weights_plan(B, Hq, Hkv, Sq, S, d).bytes();
+  return weights_plan(B, Hq, Hkv, Sq, S, d, qjl != 0).bytes();
 }
 
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,

@@ -386,18 +386,20 @@ struct AttnWeightsArgs {
   int page_shift, max_pages;
   const float *codebook;         // [16]
   int bits, B, Hq, Hkv, G, Sq, q_start, S, S_max, d, causal;
-  int row0, rows;                // this pass's rows of every stream (row0 a multiple of G)
-  int tblocks, chunks;           // token blocks; row chunks of kWeightRows rows
-  float2 *part;                  // [stream][tblock][rows]: maximum and sum over the block's tokens
+  int row0, rows;                // this pass's rows of every stream
+  int row_tiles;                 // their 16-row records, an even count
+  int tblocks, chunks, chunk_rows;   // token blocks; row chunks of chunk_rows (a multiple of 32)
+  uint8_t *records;              // [stream][row_tiles] the rows as matrix operands
+  float *row_factor;             // [stream][16 row_tiles]: undoes each row's power of two
+  float2 *part;                  // [stream][tblocks][rows]: maximum and sum over the block's tokens
   float2 *stat;                  // [stream][rows]: maximum and 1 / sum over all tokens
-  float *col;                    // [stream][chunk][tblocks * kWeightTokens]: sums over a chunk's rows
+  float *col;                    // [stream][chunk][tblocks * weight_tokens]: sums over a chunk's rows
   const float *in;
   int64_t in_stride;
   float *out;
   int64_t out_stride;
 };
-constexpr int kWeightTokens = 256;   // tokens per workgroup
-constexpr int kWeightRows = 2048;    // rows per workgroup
+constexpr int weight_tokens(bool qjl) { return qjl ? 128 : 256; }   // tokens per workgroup
 hipError_t launch_attn_weights(const AttnWeightsArgs &a, hipStream_t s);
 // out = in (or zeros) for S tokens of every stream.
 hipError_t launch_weights_copy(const float *in, int64_t in_stride, float *out, int64_t out_stride, int64_t streams,

@@ -1,12 +1,32 @@
 // The attention weight that each cached position gets: after a decode call,
 // from the logits it wrote (decode_weights_kernel), and for a chunk of query
 // tokens (attn_weights_kernel).
+#include <type_traits>
+
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
 namespace pqkv {
 
 namespace {
+
+// The same lane position of the four 16-lane groups, combined (gfx950 swaps).
+__device__ __forceinline__ float rows4_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
+}
+__device__ __forceinline__ float rows4_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
+}
 
 // ---- after a decode call ----
 //
@@ -71,146 +91,435 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const DecodeArgs a,
 //
 // Row r = i G + g of a (batch, kv head) stream is query token i of the
 // group's head g. The softmax needs each row's maximum and sum before any
-// column can be summed, so the scores are computed twice, from keys that a
-// workgroup decodes once and keeps: kWeightTokens tokens, against kWeightRows
-// rows that pass by.
+// column can be summed, so the scores are computed twice, by a workgroup that
+// decodes its tokens' keys once, keeps them as matrix operands in registers and
+// lets the rows pass by:
 //   STATS: per row, the maximum and the sum over the workgroup's tokens
 //   (attn_stats_kernel joins the token blocks'),
 //   sums:  per token, sum over the rows of exp2(s - M) / L
 //   (weights_join_kernel joins the row chunks' in order, so nothing depends on
 //   which workgroup ends first).
 // A causal row at position p meets only the blocks that start at or before p.
-template <int D, bool QJL, bool STATS>
-__global__ void __launch_bounds__(256) attn_weights_kernel(const AttnWeightsArgs a) {
-  constexpr int NR = 8;
-  __shared__ __align__(16) float qs[NR][D], ps[QJL ? NR : 1][D];
-  __shared__ float red[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t blk = blockIdx.x;
-  const int chunk = blk % (uint32_t)a.chunks;
-  blk /= (uint32_t)a.chunks;
-  const int tb = blk % (uint32_t)a.tblocks;
-  const int64_t stream = blk / (uint32_t)a.tblocks;
+//
+// Products are v_mfma_f32_16x16x32_f16 on fp32 operands split hi / lo, three of
+// them (hi hi + hi lo + lo hi) into one fp32 accumulator. A = 16 tokens' keys
+// r c[code], B = 16 rows' queries, so accumulator i of lane (col, grp) is token
+// 4 grp + i of row col: a row's statistics reduce over a lane's registers and
+// the four lane groups, a column's sum stays in its register until the end.
+// Powers of two keep the parts in fp16's range: a row's largest query value at
+// 2^8 (queries per row, undone by a factor per lane), the block's largest key at
+// 2^8 (per workgroup). With QJL the signs join the same accumulator as +- the
+// keys' power of two against the projections (two more products; +-0 where the
+// sketch is all ones, a zero residual).
+constexpr int kWW = 4;      // waves of a workgroup
+constexpr int kStage = 32;  // rows of a stage
+
+struct WeightsKernelArgs {
+  AttnWeightsArgs a;
+  FastDiv group;             // by G
+  int xcd_groups;            // > 0: (stream, chunk) groups dealt to the XCDs
+};
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) const half8_t lds_chalf8;
+
+template <int D, bool QJL>
+struct RowRec {                                    // 16 rows as B operands
+  static constexpr int KS = D / 32;
+  static constexpr int PARTS = QJL ? 4 : 2;        // q hi, q lo (, projections hi, lo)
+  static constexpr int BYTES = KS * PARTS * 1024;  // segment (ks, part): 64 lanes x 16 bytes
+};
+
+// (x in a register of its own: where it is a product, the conversion may
+// otherwise be fused with it and round the unrounded product, while the
+// remainder is taken from the rounded one: a step of the high part lost on
+// values next to a tie)
+__device__ __forceinline__ void split_parts(float x, half_t *hi, half_t *lo) {
+  asm("" : "+v"(x));
+  const half_t h = (half_t)x;
+  *hi = h;
+  *lo = (half_t)(x - (float)h);
+}
+
+// The power of two that brings `most` to [2^8, 2^9); 0 if it is zero, subnormal or not finite.
+__device__ __forceinline__ int scale_exponent(float most, int largest) {
+  const int ex = (int)((__builtin_bit_cast(uint32_t, most) >> 23) & 0xFF);
+  return ex == 0 || ex == 255 ? 0 : min(135 - ex, largest);
+}
+
+// Rotated queries (and projections) -> records of 16 rows, and each row's
+// factor. Rows past the pass's last one are zeros.
+template <int D, bool QJL>
+__global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernelArgs k) {
+  using Rec = RowRec<D, QJL>;
+  __shared__ float most[D / 8][16];
+  const AttnWeightsArgs &a = k.a;
+  const int tid = threadIdx.x, rl = tid & 15, j = tid >> 4;   // row of the tile; its eight coordinates
+  const uint32_t tiles = (uint32_t)a.row_tiles;
+  const int64_t stream = blockIdx.x / tiles;
+  const int tile = (int)(blockIdx.x - (uint32_t)stream * tiles), r = tile * 16 + rl;
   const int b = (int)(stream / a.Hkv), h = (int)(stream - (int64_t)b * a.Hkv);
-  const int t0 = tb * kWeightTokens, t = t0 + tid;
-  int r_begin = chunk * kWeightRows;
-  const int r_end = min(r_begin + kWeightRows, a.rows);
+  float x[QJL ? 2 : 1][8];
+  float mx = 0.0f;
+  const uint32_t tok = k.group.div((uint32_t)(min(r, a.rows - 1) + a.row0));
+  const int64_t row = ((int64_t)b * a.Hq + h * a.G + (min(r, a.rows - 1) + a.row0 - (int)tok * a.G)) * a.Sq + tok;
+#pragma unroll
+  for (int p = 0; p < (QJL ? 2 : 1); ++p) {
+    const float *src = (p ? a.pq : a.q) + row * D + 8 * j;
+    const float4 u = *(const float4 *)src, v = *(const float4 *)(src + 4);
+    const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[p][i] = r < a.rows ? e[i] : 0.0f;
+      mx = fmaxf(mx, fabsf(x[p][i]));
+    }
+  }
+  most[j][rl] = mx;
+  __syncthreads();
+  for (int i = 0; i < D / 8; ++i) mx = fmaxf(mx, most[i][rl]);
+  const int sh = scale_exponent(mx, 100);
+  if (j == 0) a.row_factor[stream * tiles * 16 + r] = __builtin_ldexpf(1.0f, -sh);
+  uint8_t *rec = a.records + (stream * tiles + tile) * Rec::BYTES;
+  const float sc = __builtin_ldexpf(1.0f, sh);
+#pragma unroll
+  for (int p = 0; p < (QJL ? 2 : 1); ++p) {
+    half8_t hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      half_t u, v;
+      split_parts(x[p][i] * sc, &u, &v);
+      hi[i] = u;
+      lo[i] = v;
+    }
+    uint8_t *seg = rec + ((j >> 2) * Rec::PARTS + 2 * p) * 1024 + ((j & 3) * 16 + rl) * 16;
+    *(half8_t *)seg = hi;
+    *(half8_t *)(seg + 1024) = lo;
+  }
+}
+
+template <int D, bool QJL, bool STATS>
+__global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const WeightsKernelArgs k) {
+  using Rec = RowRec<D, QJL>;
+  constexpr int KS = Rec::KS, TT = weight_tokens(QJL) / (16 * kWW), RT = kStage / 16;
+  constexpr int SEGS = RT * Rec::BYTES / 1024;
+  __shared__ __attribute__((aligned(16))) uint8_t qb[2][RT * Rec::BYTES];
+  __shared__ float2 pair_tab[256];                 // 4-bit: byte -> two centroids; 2-bit: nibble
+  __shared__ float red[kWW];
+  __shared__ float2 st[STATS ? 2 : 1][kWW][kStage];
+  const AttnWeightsArgs &a = k.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+
+  // Workgroup -> (stream, chunk, token block), the blocks of one (stream,
+  // chunk) group side by side: they read the same rows. With groups enough for
+  // every XCD (workgroup n runs on XCD n % 8) a group stays on one, whose L2
+  // then holds its rows. Later chunks first: a causal chunk meets more blocks.
+  uint32_t blk = blockIdx.x;
+  uint32_t gi, tbu;
+  if (k.xcd_groups) {
+    const uint32_t j = blk >> 3;
+    tbu = j % (uint32_t)a.tblocks;
+    gi = (j / (uint32_t)a.tblocks) * 8 + (blk & 7);
+    if (gi >= (uint32_t)k.xcd_groups) return;
+  } else {
+    tbu = blk % (uint32_t)a.tblocks;
+    gi = blk / (uint32_t)a.tblocks;
+  }
+  const uint32_t n_streams = (uint32_t)(a.B * a.Hkv);
+  const int chunk = a.chunks - 1 - (int)(gi / n_streams), tb = (int)tbu;
+  const int64_t stream = gi % n_streams;
+  const int t0 = tb * weight_tokens(QJL), tw0 = t0 + 16 * TT * wave, tw1 = tw0 + 16 * TT - 1;
+  int r_begin = chunk * a.chunk_rows;
+  const int r_end = min(r_begin + a.chunk_rows, a.rows);
   if (a.causal) {   // the first row that sees token t0
     const int64_t first = (int64_t)(t0 - a.q_start) * a.G - a.row0;
-    if (first >= r_end) return;
+    if (first >= r_end) {
+      if (!STATS && a.chunks == 1)   // no row sees the block: what there was stays
+        for (int t = t0 + tid; t < min(t0 + weight_tokens(QJL), a.S); t += 64 * kWW)
+          a.out[stream * a.out_stride + t] = a.in ? a.in[stream * a.in_stride + t] : 0.0f;
+      return;
+    }
     if (first > r_begin) r_begin = (int)first;
   }
-  float c[D], radius = 0.0f;
-  uint32_t sg[QJL ? D / 32 : 1];
-  bool zero_res = true;
+
+  const uint8_t *records = a.records + stream * a.row_tiles * (int64_t)Rec::BYTES;
+  const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
+      (void *)records, (short)0, (int)((int64_t)a.row_tiles * Rec::BYTES), 0x00020000);
+  const float *factor = a.row_factor + stream * a.row_tiles * 16;
+  auto copy_stage = [&](int s) {
+    const int at = __builtin_amdgcn_readfirstlane(s * RT * Rec::BYTES);
+#pragma unroll
+    for (int j = 0; j < SEGS / kWW; ++j) {
+      const int sg = wave + kWW * j;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (lds_void *)(qb[s & 1] + 1024 * sg), 16, 16 * lane, at + 1024 * sg,
+                                               0, 0);
+    }
+  };
+  const int s0 = r_begin / kStage, s1 = (r_end + kStage - 1) / kStage;
+  copy_stage(s0);
+
+  // ---- this wave's keys, 16 TT tokens: lane (col, grp) holds coordinates
+  // 32 ks + 8 grp .. + 7 of token 16 tt + col ----
   const int vb = vector_bytes(D, a.bits);
-  if (t < a.S) {
-    const uint8_t *kv, *sv;
+  const uint8_t *kv[TT], *sv[TT];
+  float radius[TT], rmax = 0.0f;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    const int t = min(tw0 + 16 * tt + col, a.S - 1);
     if (a.k_pages) {
       const int64_t pg = stream * a.max_pages + (t >> a.page_shift);
       const int64_t at = t & ((1 << a.page_shift) - 1);
-      kv = a.k_pages[pg] + at * vb;
-      sv = QJL ? a.s_pages[pg] + at * (D / 8) : nullptr;
+      kv[tt] = a.k_pages[pg] + at * vb;
+      sv[tt] = QJL ? a.s_pages[pg] + at * (D / 8) : nullptr;
     } else {
-      kv = a.k_cache + (stream * a.S_max + t) * vb;
-      sv = QJL ? a.qjl + (stream * a.S_max + t) * (D / 8) : nullptr;
+      kv[tt] = a.k_cache + (stream * a.S_max + t) * vb;
+      sv[tt] = QJL ? a.qjl + (stream * a.S_max + t) * (D / 8) : nullptr;
     }
-    radius = half_bits_to_float(*(const uint16_t *)kv);
-    for (int k = 0; k < D; ++k) {
-      const int byte = kv[qs_offset(k * a.bits / 8, a.bits)];
-      c[k] = a.codebook[(byte >> (k * a.bits % 8)) & ((1 << a.bits) - 1)];
-    }
-    if constexpr (QJL)
-      for (int k = 0; k < D / 32; ++k) {
-        uint32_t w = 0;
-        for (int j = 0; j < 4; ++j) w |= (uint32_t)sv[4 * k + j] << (8 * j);
-        sg[k] = w;
-        zero_res = zero_res && w == 0xFFFFFFFFu;
-      }
-  } else {
-    for (int k = 0; k < D; ++k) c[k] = 0.0f;
-    if constexpr (QJL)
-      for (int k = 0; k < D / 32; ++k) sg[k] = 0;
+    const float r = half_bits_to_float(*(const uint16_t *)kv[tt]);
+    radius[tt] = tw0 + 16 * tt + col < a.S ? r : 0.0f;
+    rmax = fmaxf(rmax, fabsf(radius[tt]));
   }
-  float col = 0.0f;
-  for (int r0 = r_begin; r0 < r_end; r0 += NR) {
-    __syncthreads();
-    for (int i = tid; i < NR * D; i += 256) {
-      const int r = min(r0 + i / D, r_end - 1) + a.row0;
-      const int64_t row = ((int64_t)b * a.Hq + h * a.G + r % a.G) * a.Sq + r / a.G;
-      qs[i / D][i % D] = a.q[row * D + i % D];
-      if constexpr (QJL) ps[i / D][i % D] = a.pq[row * D + i % D];
+  uint32_t code[TT][KS];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint8_t *p = kv[tt] + qs_offset((32 * ks + 8 * grp) * a.bits / 8, a.bits);
+      code[tt][ks] = *(const uint16_t *)p;
+      if (a.bits == 4) code[tt][ks] |= (uint32_t)((const uint16_t *)p)[1] << 16;
     }
-    __syncthreads();
-    for (int rr = 0; rr < min(NR, r_end - r0); ++rr) {
-      const int r = r0 + rr;
-      float s = 0.0f;
-      for (int k = 0; k < D; ++k) s = __builtin_fmaf(qs[rr][k], c[k], s);
-      s *= radius;
-      if constexpr (QJL) {
-        float x = 0.0f;
-        for (int k = 0; k < D; ++k) x += (sg[k / 32] >> (k % 32)) & 1u ? ps[rr][k] : -ps[rr][k];
-        s = zero_res ? s : s + x;
+  float cmax = 0.0f;
+  for (int i = 0; i < (1 << a.bits); ++i) cmax = fmaxf(cmax, fabsf(a.codebook[i]));
+  {
+    const int sh = a.bits == 4 ? 4 : 2, m = (1 << a.bits) - 1;
+    pair_tab[tid] = make_float2(a.codebook[tid & m], a.codebook[(tid >> sh) & m]);
+  }
+  rmax = wave_max(rmax);
+  if (lane == 0) red[wave] = rmax;
+  __syncthreads();
+  rmax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int ksh = max(scale_exponent(rmax * cmax, 14), -24);
+  const float kscale = __builtin_ldexpf(1.0f, ksh), kundo = __builtin_ldexpf(1.0f, -ksh);
+  half8_t kh[TT][KS], kl[TT][KS], sg[QJL ? TT : 1][KS];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    const float rs = radius[tt] * kscale;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 c = pair_tab[a.bits == 4 ? (code[tt][ks] >> (8 * i)) & 255 : (code[tt][ks] >> (4 * i)) & 15];
+        half_t u, v;
+        split_parts(c.x * rs, &u, &v);
+        kh[tt][ks][2 * i] = u;
+        kl[tt][ks][2 * i] = v;
+        split_parts(c.y * rs, &u, &v);
+        kh[tt][ks][2 * i + 1] = u;
+        kl[tt][ks][2 * i + 1] = v;
       }
-      const int pos = a.q_start + (r + a.row0) / a.G;
-      const bool valid = t < a.S && (!a.causal || t <= pos);
+    if constexpr (QJL) {
+      uint32_t w[D / 32];
+      bool ones = true;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        __builtin_memcpy(&w[i], sv[tt] + 4 * i, 4);
+        ones = ones && w[i] == 0xFFFFFFFFu;
+      }
+      const half_t one = (half_t)(ones || tw0 + 16 * tt + col >= a.S ? 0.0f : kscale);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sg[tt][ks][i] = (w[ks] >> (8 * grp + i)) & 1u ? one : -one;
+    }
+  }
+
+  // ---- the rows, a stage at a time ----
+  struct RowInfo {
+    float f[RT];
+    float2 x[RT];
+  };
+  auto row_info = [&](int s) {
+    RowInfo o;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = kStage * s + 16 * rt + col;
+      o.f[rt] = factor[r] * kundo;
+      if constexpr (!STATS) o.x[rt] = r < a.rows ? a.stat[stream * a.rows + r] : make_float2(INFINITY, 0.0f);
+    }
+    return o;
+  };
+  float csum[TT][4];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) csum[tt][i] = 0.0f;
+
+  auto compute = [&](int s, const RowInfo &info, auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
+    const lds_chalf8 *q = (const lds_chalf8 *)(qb[s & 1] + 16 * lane);
+    float4_t acc[RT][TT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const half8_t bh = q[((rt * KS + ks) * Rec::PARTS) * 64], bl = q[((rt * KS + ks) * Rec::PARTS + 1) * 64];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[tt][ks], bh, acc[rt][tt], 0, 0, 0);
+          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bl, acc[rt][tt], 0, 0, 0);
+          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bh, acc[rt][tt], 0, 0, 0);
+        }
+        if constexpr (QJL) {
+          const half8_t ph = q[((rt * KS + ks) * Rec::PARTS + 2) * 64], pl = q[((rt * KS + ks) * Rec::PARTS + 3) * 64];
+#pragma unroll
+          for (int tt = 0; tt < TT; ++tt) {
+            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], pl, acc[rt][tt], 0, 0, 0);
+            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], ph, acc[rt][tt], 0, 0, 0);
+          }
+        }
+      }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      int last = a.S - 1;   // the last token the lane's row sees
+      if (kMasked && a.causal)
+        last = min(last, a.q_start + (int)k.group.div((uint32_t)(kStage * s + 16 * rt + col + a.row0)));
+      const int rel = last - tw0 - 4 * grp;
       if constexpr (STATS) {
-        const float v = valid ? s : -INFINITY;
-        float m = wave_max(v);
-        __syncthreads();
-        if (lane == 0) red[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float l = wave_sum(valid ? __builtin_amdgcn_exp2f(v - m) : 0.0f);
-        __syncthreads();
-        if (lane == 0) red[wave] = l;
-        __syncthreads();
-        if (tid == 0)
-          a.part[(stream * a.tblocks + tb) * a.rows + r] = make_float2(m, red[0] + red[1] + red[2] + red[3]);
+        float m = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (kMasked && 16 * tt + i > rel) acc[rt][tt][i] = -INFINITY;
+            m = fmaxf(m, acc[rt][tt][i]);
+          }
+        m = rows4_max(m) * info.f[rt];      // the factor is positive: the maximum stays where it is
+        const float ref = kMasked && m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], info.f[rt], -ref));
+        l = rows4_sum(l);
+        if (grp == 0) st[s & 1][wave][16 * rt + col] = make_float2(m, l);
       } else {
-        const float2 x = a.stat[stream * a.rows + r];
-        if (valid) col = __builtin_fmaf(__builtin_amdgcn_exp2f(s - x.x), x.y, col);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], info.f[rt], -info.x[rt].x));
+            if (kMasked && 16 * tt + i > rel) e = 0.0f;
+            csum[tt][i] = __builtin_fmaf(e, info.x[rt].y, csum[tt][i]);
+          }
       }
     }
+  };
+  // STATS: the four waves' statistics of stage s, joined and written
+  auto write_stats = [&](int s) {
+    const int r = kStage * s + lane;
+    if (wave != (s & (kWW - 1)) || lane >= kStage || r < r_begin || r >= r_end) return;
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWW; ++w) m = fmaxf(m, st[s & 1][w][lane].x);
+#pragma unroll
+    for (int w = 0; w < kWW; ++w) {
+      const float2 x = st[s & 1][w][lane];
+      if (x.x != -INFINITY) l = __builtin_fmaf(x.y, __builtin_amdgcn_exp2f(x.x - m), l);
+    }
+    a.part[(stream * a.tblocks + tb) * a.rows + r] = make_float2(m, l);
+  };
+  RowInfo info = row_info(s0);
+  for (int s = s0; s < s1; ++s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // stage s has arrived (this wave's part)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // everyone's; stage s - 1 has been read
+    RowInfo next = info;
+    if (s + 1 < s1) {
+      copy_stage(s + 1);
+      next = row_info(s + 1);
+    }
+    if (STATS && s > s0) write_stats(s - 1);
+    const int p_first = a.q_start + (int)k.group.div((uint32_t)(kStage * s + a.row0));
+    const int p_last = a.q_start + (int)k.group.div((uint32_t)(kStage * s + kStage - 1 + a.row0));
+    if (tw0 >= a.S || (a.causal && p_last < tw0)) {
+      if (STATS && lane < kStage) st[s & 1][wave][lane] = make_float2(-INFINITY, 0.0f);   // none of its tokens
+    } else if (tw1 >= a.S || (a.causal && p_first < tw1)) {
+      compute(s, info, std::true_type{});
+    } else {
+      compute(s, info, std::false_type{});
+    }
+    info = next;
   }
-  if constexpr (!STATS)
-    a.col[((stream * a.chunks + chunk) * a.tblocks + tb) * kWeightTokens + tid] = col;
+  if constexpr (STATS) {
+    __syncthreads();
+    write_stats(s1 - 1);
+    return;
+  }
+  // each token's sum over the 16 row columns
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v = csum[tt][i];
+#pragma unroll
+      for (int sft = 1; sft < 16; sft <<= 1) v += shfl_xor_f(v, sft);
+      const int t = tw0 + 16 * tt + 4 * grp + i;
+      if (col == 0) {
+        if (a.chunks > 1) a.col[((stream * a.chunks + chunk) * a.tblocks + tb) * weight_tokens(QJL) + t - t0] = v;
+        else if (t < a.S)
+          a.out[stream * a.out_stride + t] = (a.in ? a.in[stream * a.in_stride + t] : 0.0f) + v;
+      }
+    }
 }
 
-// Joins the token blocks' maxima and sums of one row.
-__global__ void __launch_bounds__(256) attn_stats_kernel(const AttnWeightsArgs a) {
-  const uint32_t tiles = (uint32_t)(a.rows + 255) / 256;
+// Joins the token blocks' maxima and sums of 32 rows, eight threads per row.
+__global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs k, int tokens) {
+  __shared__ float2 sub[8][32];
+  const AttnWeightsArgs &a = k.a;
+  const uint32_t tiles = (uint32_t)(a.rows + 31) / 32;
   const int64_t stream = blockIdx.x / tiles;
-  const int r = (int)(blockIdx.x - (uint32_t)stream * tiles) * 256 + threadIdx.x;
-  if (r >= a.rows) return;
-  const int last = a.causal ? min(a.q_start + (r + a.row0) / a.G, a.S - 1) : a.S - 1;
-  const int n = last / kWeightTokens + 1;
-  const float2 *p = a.part + stream * a.tblocks * a.rows + r;
+  const int rl = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int r = (int)(blockIdx.x - (uint32_t)stream * tiles) * 32 + rl;
+  const int rr = min(r, a.rows - 1);
+  const int last = a.causal ? min(a.q_start + (int)k.group.div((uint32_t)(rr + a.row0)), a.S - 1) : a.S - 1;
+  const int n = last / tokens + 1;
+  const float2 *p = a.part + stream * a.tblocks * a.rows + rr;
   float m = -INFINITY, l = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const float2 x = p[(int64_t)i * a.rows];
+  auto join = [&](float2 x) {
     const float mn = fmaxf(m, x.x);
-    if (mn == -INFINITY) continue;
+    if (mn == -INFINITY) return;
     l = l * __builtin_amdgcn_exp2f(m - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
     m = mn;
-  }
+  };
+#pragma unroll 8
+  for (int i = q; i < n; i += 8) join(p[(int64_t)i * a.rows]);
+  sub[q][rl] = make_float2(m, l);
+  __syncthreads();
+  if (q != 0 || r >= a.rows) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) join(sub[i][rl]);
   a.stat[stream * a.rows + r] = make_float2(m, 1.0f / l);
 }
 
 // out = in + the row chunks' sums of one token, in the chunks' order.
-__global__ void __launch_bounds__(256) weights_join_kernel(const AttnWeightsArgs a) {
-  const int64_t stream = blockIdx.x / (uint32_t)a.tblocks;
-  const int tb = (int)(blockIdx.x - (uint32_t)stream * a.tblocks);
-  const int t = tb * kWeightTokens + threadIdx.x;
+__global__ void __launch_bounds__(256) weights_join_kernel(const AttnWeightsArgs a, int tokens) {
+  const uint32_t tiles = (uint32_t)(a.S + 255) / 256;
+  const int64_t stream = blockIdx.x / tiles;
+  const int t = (int)(blockIdx.x - (uint32_t)stream * tiles) * 256 + threadIdx.x;
   if (t >= a.S) return;
+  const int tb = t / tokens;
   int c0 = 0;
   if (a.causal) {   // chunks that end before the first row that sees the block were not computed
-    const int64_t first = (int64_t)(tb * kWeightTokens - a.q_start) * a.G - a.row0;
+    const int64_t first = (int64_t)(tb * tokens - a.q_start) * a.G - a.row0;
     if (first >= a.rows) c0 = a.chunks;
-    else if (first > 0) c0 = (int)(first / kWeightRows);
+    else if (first > 0) c0 = (int)(first / a.chunk_rows);
   }
   float sum = 0.0f;
-  for (int c = c0; c < a.chunks; ++c) sum += a.col[((stream * a.chunks + c) * a.tblocks + tb) * kWeightTokens + threadIdx.x];
+#pragma unroll 4
+  for (int c = c0; c < a.chunks; ++c) sum += a.col[((stream * a.chunks + c) * a.tblocks) * (int64_t)tokens + t];
   a.out[stream * a.out_stride + t] = (a.in ? a.in[stream * a.in_stride + t] : 0.0f) + sum;
 }
 
@@ -224,11 +533,17 @@ __global__ void __launch_bounds__(256) weights_copy_kernel(const float *in, int6
 
 template <int D, bool QJL>
 void launch_passes(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
-  const unsigned grid = (unsigned)(streams * a.tblocks * a.chunks);
-  attn_weights_kernel<D, QJL, true><<<grid, 256, 0, s>>>(a);
-  attn_stats_kernel<<<(unsigned)(streams * ((a.rows + 255) / 256)), 256, 0, s>>>(a);
-  attn_weights_kernel<D, QJL, false><<<grid, 256, 0, s>>>(a);
-  weights_join_kernel<<<(unsigned)(streams * a.tblocks), 256, 0, s>>>(a);
+  constexpr int tokens = weight_tokens(QJL);
+  WeightsKernelArgs k{a, FastDiv((uint32_t)a.G), 0};
+  const int64_t groups = streams * a.chunks;
+  if (groups % 8 == 0 || groups >= 64) k.xcd_groups = (int)groups;
+  const unsigned grid = (unsigned)((k.xcd_groups ? (groups + 7) / 8 * 8 : groups) * a.tblocks);
+  weights_rows_kernel<D, QJL><<<(unsigned)(streams * a.row_tiles), 2 * D, 0, s>>>(k);
+  attn_weights_kernel<D, QJL, true><<<grid, 64 * kWW, 0, s>>>(k);
+  attn_stats_kernel<<<(unsigned)(streams * ((a.rows + 31) / 32)), 256, 0, s>>>(k, tokens);
+  attn_weights_kernel<D, QJL, false><<<grid, 64 * kWW, 0, s>>>(k);
+  if (a.chunks > 1)   // (one chunk: the sums are the result)
+    weights_join_kernel<<<(unsigned)(streams * ((a.S + 255) / 256)), 256, 0, s>>>(a, tokens);
 }
 
 }  // namespace

@@ -249,7 +249,7 @@ def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, 
     R = rotation_matrix.to(torch.float32).contiguous()
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
     lib = _lib.lib()
-    ws = torch.empty(max(1, lib.pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d)), dtype=torch.uint8,
+    ws = torch.empty(max(1, lib.pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d, int(P is not None))), dtype=torch.uint8,
                      device=q.device)
     tail = (scale, int(causal), _lib.ptr(previous), 0 if previous is None else _row_stride(previous), into.data_ptr(),
             _row_stride(into), ws.data_ptr(), ws.numel(), _lib.stream_of(q))

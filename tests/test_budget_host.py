@@ -69,10 +69,11 @@ def test_attn_weights_refusals(kw, expect):
 def test_attn_weights_nothing_to_do():
     assert _weights(S=0, S_max=0, q_start=0, Sq=0, wo=None) == 0
     assert _weights(Sq=0, wi=FAKE, wis=16) == 0              # in place: the weights stay as they are
-    assert _lib.lib().pqkv_attn_weights_workspace_bytes(1, 8, 3, 4, 16, 128) == 0
+    assert _lib.lib().pqkv_attn_weights_workspace_bytes(1, 8, 3, 4, 16, 128, 0) == 0
     # the partials of a long chunk over a long cache stay bounded
-    n = _lib.lib().pqkv_attn_weights_workspace_bytes(8, 32, 8, 8192, 131072, 128)
-    assert n < (600 << 20) + 2 * 8 * 32 * 8192 * 128 * 4
+    for qjl in (0, 1):
+        n = _lib.lib().pqkv_attn_weights_workspace_bytes(8, 32, 8, 8192, 131072, 128, qjl)
+        assert n < (1 << 30) + (1 + qjl) * 8 * 32 * 8192 * 128 * 4
 
 
 def test_paged_calls_check_the_table():
