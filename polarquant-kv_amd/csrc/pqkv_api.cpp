@@ -736,15 +736,17 @@ int decode_attn_run(const void *q, int q_dtype, const float *R, const uint8_t *k
         }
     }
   }
+  if (wt) {   // (not repeated: the weights may add up in place)
+    tok = prof_begin("decode_merge_weights", st);
+    e = launch_decode_merge_weights(a, *wt, R, out, out_dtype, st);
+    prof_end(tok, st);
+    return hip_status(e, "decode merge launch");
+  }
   tok = prof_begin("decode_merge", st, true);
   for (int rep = 0, nrep = prof_repeats(); rep < nrep && e == hipSuccess; ++rep)
     e = launch_decode_merge(part, R, out, out_dtype, B * Hq, splits, d, st);
   prof_end(tok, st);
-  if (e != hipSuccess || !wt) return hip_status(e, "decode merge launch");
-  tok = prof_begin("decode_weights", st);
-  e = launch_decode_weights(a, *wt, st);
-  prof_end(tok, st);
-  return hip_status(e, "decode weights launch");
+  return hip_status(e, "decode merge launch");
 }
 
 // Split plans of the segments of a segmented decode call (B * Hkv streams

@@ -12,13 +12,13 @@
 #include "pqkv_launch.h"
 
 using pqkv::fail_status;
+using pqkv::kMaxGroupWeights;
 using pqkv::report_hip_error;
 
 namespace {
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 constexpr int kMaxTokens = 1 << 24;      // 32-bit byte offsets into 8 rows of logits
-constexpr int kMaxGroupWeights = 1024;   // query heads per kv head
 constexpr int64_t kMaxGrid = INT_MAX;
 
 // The weights' strides against the shape; returns PQKV_OK or the failure.
@@ -51,7 +51,7 @@ int decode_weights_run(const void *q, int q_dtype, const float *R, const uint8_t
     return fail_status(PQKV_ERR_INVALID, "decode_weights: B=%d Hq=%d Hkv=%d S=%d", B, Hq, Hkv, S);
   if (S >= kMaxTokens) return fail_status(PQKV_ERR_UNSUPPORTED, "decode_weights: S=%d", S);
   if (Hq / Hkv > kMaxGroupWeights) return fail_status(PQKV_ERR_UNSUPPORTED, "decode_weights: group size %d", Hq / Hkv);
-  if ((int64_t)B * Hkv * (S / 1024 + 1) > kMaxGrid) return fail_status(PQKV_ERR_UNSUPPORTED, "decode_weights: size");
+  if ((int64_t)B * Hkv * (S / 1024 + 1) + (int64_t)B * Hq > kMaxGrid) return fail_status(PQKV_ERR_UNSUPPORTED, "decode_weights: size");
   const int c = check_weights("decode_weights", in, in_stride, w_out, w_stride, B, Hkv, S);
   if (c != PQKV_OK) return c;
   const size_t base = S > 0 ? align256(pqkv_decode_workspace_bytes(B, Hq, Hkv, S, d)) : 0;
@@ -71,35 +71,42 @@ int decode_weights_run(const void *q, int q_dtype, const float *R, const uint8_t
 // workspace: rotated queries (and projections), the rows' records and factors,
 // the token blocks' partials, the rows' statistics, the row chunks' sums.
 struct WeightsPlan {
-  int tblocks, rows, chunk_rows;
+  int tokens, tblocks, rows, chunk_rows;
   size_t q, pq, records, factor, part, stat, col;
   size_t bytes() const { return q + pq + records + factor + part + stat + col; }
   int chunks(int r) const { return (r + chunk_rows - 1) / chunk_rows; }
 };
-int row_tiles(int rows) { return (rows + 31) / 32 * 2; }
+// Rows of a stream up to which a workgroup takes 128 tokens, not 256: three
+// waves per SIMD instead of two hide the decoding of the keys, which is then a
+// larger part of the work (32 query / 8 kv heads, d = 128: 256 rows on 32768
+// tokens 129 us against 156, 2048 rows on 16512 tokens 384 against 411); with
+// more rows each operand read serves four tiles instead of two (32764 rows on
+// 8191 tokens 1.48 ms against 1.54).
+constexpr int kFewRows = 2048;
+int row_tiles(int rows) { return (rows + 63) / 64 * 4; }
 WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl) {
   WeightsPlan p;
   const int64_t streams = (int64_t)B * Hkv, total = (int64_t)Sq * (Hq / Hkv);
-  const int tokens = pqkv::weight_tokens(qjl);
-  p.tblocks = (S + tokens - 1) / tokens;
+  p.tokens = qjl || total <= kFewRows ? 128 : 256;
+  p.tblocks = (S + p.tokens - 1) / p.tokens;
   // rows of a pass: partials within 256 MB, records within 512 MB
   const int64_t rec_row = (int64_t)d * (qjl ? 8 : 4);
   int64_t rows = std::min((int64_t)(256 << 20) / (streams * p.tblocks * (int64_t)sizeof(float2)),
                           (int64_t)(512 << 20) / (streams * rec_row));
-  rows = std::max<int64_t>(rows / 32 * 32, 32);
+  rows = std::max<int64_t>(rows / 64 * 64, 64);
   p.rows = (int)std::min(rows, total);
   // rows of a workgroup: about 2048 workgroups (four rounds of two per compute
   // unit); at least 128 rows, under which decoding the keys is most of the work,
   // at most 2048, whose records (1 MB at d = 128) a group of workgroups shares in L2
   const int64_t want = p.rows * streams * p.tblocks / 2048;
-  p.chunk_rows = (int)std::min<int64_t>(std::max<int64_t>((want + 31) / 32 * 32, 128), 2048);
+  p.chunk_rows = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, 128), 1024);
   p.q = align256((size_t)B * Hq * Sq * d * 4);
   p.pq = qjl ? p.q : 0;
   p.records = align256((size_t)streams * row_tiles(p.rows) * 16 * rec_row);
   p.factor = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float));
   p.part = align256((size_t)streams * p.tblocks * p.rows * sizeof(float2));
-  p.stat = align256((size_t)streams * p.rows * sizeof(float2));
-  p.col = align256((size_t)streams * p.chunks(p.rows) * p.tblocks * tokens * sizeof(float));
+  p.stat = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float2));
+  p.col = align256((size_t)streams * p.chunks(p.rows) * p.tblocks * p.tokens * sizeof(float));
   return p;
 }
 
@@ -190,6 +197,7 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
   a.d = d;
   a.causal = causal ? 1 : 0;
   a.tblocks = p.tblocks;
+  a.tokens = p.tokens;
   a.chunk_rows = p.chunk_rows;
   a.records = (uint8_t *)take(p.records);
   a.row_factor = (float *)take(p.factor);
@@ -307,7 +315,7 @@ int pqkv_gather_rows(int n_arrays, const pqkv_row_array *src, const pqkv_row_arr
   if (n_arrays == 0 || n_streams == 0 || fill == 0) return PQKV_OK;
   if (!src || !dst || !row_bytes || (keep > 0 && !kept))
     return fail_status(PQKV_ERR_INVALID, "gather_rows: null pointer");
-  if (n_streams * (((int64_t)fill + 255) / 256) > kMaxGrid)
+  if (n_streams > kMaxGrid || n_streams * (((int64_t)fill + 63) / 64) > kMaxGrid)
     return fail_status(PQKV_ERR_UNSUPPORTED, "gather_rows: n_streams=%lld fill=%d", (long long)n_streams, fill);
   pqkv::GatherArgs a;
   memset(&a, 0, sizeof(a));

@@ -8,8 +8,12 @@
 // digit (11 + 11 + 10 bits, most significant first): a histogram of the digit
 // over the keys that match the digits found so far, then the bin that holds
 // the rank. Counts and indices are whole numbers, so no order of the atomic
-// additions changes the result. One workgroup per stream: the stream's weights
-// are read from HBM once and from L2 afterwards.
+// additions changes the result. One workgroup per stream, its keys in registers
+// up to 65536 positions (KPT per thread), so that the weights are read once and
+// all their loads are in flight together; longer streams are read again in each
+// pass, from L2. Weights crowd into few exponents, so the first digit's
+// additions meet in few bins: there each bin has eight counters, a lane's by its
+// number. Bound by the instructions of one compute unit per stream.
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
@@ -32,10 +36,12 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+constexpr int kCopies = 8;   // counters per bin
+
 struct SelectSmem {
-  uint32_t hist[kBins];
+  uint32_t hist[kBins * kCopies];
   uint32_t wave_sum[kSelWaves], wave_above[kSelWaves], wave_tie[kSelWaves];
-  uint32_t digit, rank;
+  uint32_t digit, rank, count;
 };
 
 // Inclusive prefix sum of v over the wave's lanes.
@@ -48,141 +54,228 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v, int lane) {
   return v;
 }
 
+template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float *__restrict__ weights, int64_t stride,
                                                                    int S, int keep, int sink, int recent,
                                                                    int *__restrict__ kept) {
-  __shared__ SelectSmem sm;
+  __shared__ __align__(16) SelectSmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float *w = weights + blockIdx.x * stride;
   int *out = kept + (int64_t)blockIdx.x * keep;
   // each wave takes one contiguous run of whole 64-position steps
   const int steps = (S + kSelThreads - 1) / kSelThreads;
   const int begin = wave * steps * kWave, end = min(S, begin + steps * kWave);
-  auto key_at = [&](int i) { return i < sink || i >= S - recent ? 0xFFFFFFFFu : weight_key(w[i]); };
+  auto key_of = [&](int i, float x) { return i < sink || i >= S - recent ? 0xFFFFFFFFu : weight_key(x); };
+  uint32_t keys[KPT > 0 ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+      const int i = begin + j * kWave + lane;
+      keys[j] = __builtin_bit_cast(uint32_t, j < steps && i < end ? w[i] : 0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) keys[j] = key_of(begin + j * kWave + lane, __builtin_bit_cast(float, keys[j]));
+  }
+  // f(key, position, whether there is one) for the wave's positions, step by step
+  auto each = [&](auto f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) {
+        if (j >= steps) break;
+        const int i = begin + j * kWave + lane;
+        f(keys[j], i, i < end);
+      }
+    } else {
+      constexpr int U = 16;   // loads in flight
+      for (int i0 = begin + lane; i0 - lane < end; i0 += U * kWave) {
+        float x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = i0 + u * kWave < end ? w[i0 + u * kWave] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(key_of(i0 + u * kWave, x[u]), i0 + u * kWave, i0 + u * kWave < end);
+      }
+    }
+  };
 
-  uint32_t found = 0, mask = 0, rank = (uint32_t)keep;   // rank: of the wanted key among those matching `found`
-#pragma unroll 1
+  // rank: of the wanted key among those matching `found`; on_border: keys equal to it
+  uint32_t found = 0, mask = 0, rank = (uint32_t)keep, on_border = 0;
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const int copies = pass == 0 ? kCopies : 1;
     const uint32_t low = (1u << bits) - 1;
-    for (int i = tid; i < kBins; i += kSelThreads) sm.hist[i] = 0;
+    for (int i = tid; i < kBins * copies / 4; i += kSelThreads) ((u32x4 *)sm.hist)[i] = (u32x4){0u, 0u, 0u, 0u};
     __syncthreads();
-    for (int i = begin + lane; i < end; i += kWave) {
-      const uint32_t key = key_at(i);
-      if ((key & mask) == found) atomicAdd(&sm.hist[(key >> shift) & low], 1u);
-    }
+    each([&](uint32_t key, int, bool there) {
+      if (there && (key & mask) == found)
+        atomicAdd(&sm.hist[((key >> shift) & low) * copies + (lane & (copies - 1))], 1u);
+    });
     __syncthreads();
     // thread t: bins 2047 - 2t and 2046 - 2t, counted from the top
     const int b1 = kBins - 1 - 2 * tid;
-    const uint32_t c1 = sm.hist[b1], c0 = sm.hist[b1 - 1];
+    uint32_t c0, c1;
+    if (pass == 0) {
+      const u32x4 *h = (const u32x4 *)(sm.hist + (b1 - 1) * kCopies);
+      const u32x4 x0 = h[0] + h[1], x1 = h[2] + h[3];
+      c0 = x0.x + x0.y + x0.z + x0.w;
+      c1 = x1.x + x1.y + x1.z + x1.w;
+    } else {
+      c0 = sm.hist[b1 - 1];
+      c1 = sm.hist[b1];
+    }
     const uint32_t incl = wave_prefix(c1 + c0, lane);
     if (lane == 63) sm.wave_sum[wave] = incl;
     __syncthreads();
     uint32_t before = incl - c1 - c0;
-    for (int i = 0; i < wave; ++i) before += sm.wave_sum[i];
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) before += i < wave ? sm.wave_sum[i] : 0u;
     if (before < rank && rank <= before + c1 + c0) {
       const bool first = rank <= before + c1;
       sm.digit = (uint32_t)(first ? b1 : b1 - 1);
       sm.rank = rank - before - (first ? 0u : c1);
+      sm.count = first ? c1 : c0;
     }
     __syncthreads();
     found |= sm.digit << shift;
     mask |= low << shift;
     rank = sm.rank;
+    on_border = sm.count;
+  }
+  // `found` is the border key; of the positions on it the first `rank` stay.
+  // Where all of them do (no equal weights across the border), one comparison
+  // says what stays; else the ties are counted beside the keys above.
+  auto lead = [&](uint32_t above, uint32_t ties, uint32_t &n_above, uint32_t &n_tie) {
+    if (lane == 0) {
+      sm.wave_above[wave] = above;
+      sm.wave_tie[wave] = ties;
+    }
     __syncthreads();
+    n_above = n_tie = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) {
+      n_above += i < wave ? sm.wave_above[i] : 0u;
+      n_tie += i < wave ? sm.wave_tie[i] : 0u;
+    }
+  };
+  uint32_t above = 0, ties = 0, n_above, n_tie;
+  if (rank == on_border) {
+    each([&](uint32_t key, int, bool there) {
+      above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key >= found));
+    });
+    lead(above, 0, n_above, n_tie);
+    each([&](uint32_t key, int i, bool there) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(there && key >= found);
+      if (there && key >= found) out[n_above + lanes_below(m)] = i;
+      n_above += __builtin_popcountll(m);
+    });
+    return;
   }
-  // `found` is the border key; of the positions on it the first `rank` stay
-  uint32_t above = 0, ties = 0;
-  for (int i = begin + lane; i - lane < end; i += kWave) {
-    const uint32_t key = i < end ? key_at(i) : 0u;
-    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < end && key > found));
-    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < end && key == found));
-  }
-  if (lane == 0) {
-    sm.wave_above[wave] = above;
-    sm.wave_tie[wave] = ties;
-  }
-  __syncthreads();
-  uint32_t n_above = 0, n_tie = 0;
-  for (int i = 0; i < wave; ++i) {
-    n_above += sm.wave_above[i];
-    n_tie += sm.wave_tie[i];
-  }
-  for (int i = begin + lane; i - lane < end; i += kWave) {
-    const uint32_t key = i < end ? key_at(i) : 0u;
-    const uint64_t ma = __builtin_amdgcn_ballot_w64(i < end && key > found);
-    const uint64_t mt = __builtin_amdgcn_ballot_w64(i < end && key == found);
+  each([&](uint32_t key, int, bool there) {
+    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key > found));
+    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key == found));
+  });
+  lead(above, ties, n_above, n_tie);
+  each([&](uint32_t key, int i, bool there) {
+    const uint64_t ma = __builtin_amdgcn_ballot_w64(there && key > found);
+    const uint64_t mt = __builtin_amdgcn_ballot_w64(there && key == found);
     const uint32_t a = n_above + lanes_below(ma), t = n_tie + lanes_below(mt);
-    const bool stays = i < end && (key > found || (key == found && t < rank));
-    if (stays) out[a + min(t, rank)] = i;
+    if (there && (key > found || (key == found && t < rank))) out[a + min(t, rank)] = i;
     n_above += __builtin_popcountll(ma);
     n_tie += __builtin_popcountll(mt);
-  }
+  });
 }
 
-// Rows of every part of the listed positions, a workgroup per kGatherRows
-// result rows of one stream: their source positions are read once into LDS and
-// serve all parts. A row moves in units of 8 or 4 bytes.
-constexpr int kGatherRows = 256;
-
-template <typename U>
-__device__ __forceinline__ void gather_part(const GatherPart &p, const int *src, int64_t stream, int row0, int rows,
-                                            int keep, FastDiv per_row) {
-  const uint32_t n = per_row.d, total = (uint32_t)rows * n;
-  for (uint32_t i = threadIdx.x; i < total; i += 256) {
-    const uint32_t r = per_row.div(i), c = i - r * n;
-    const int t = src[r], o = row0 + (int)r;
-    U v = 0;
-    if (t >= 0) {
-      const uint8_t *from = p.src_pages ? p.src_pages[stream * p.src_max_pages + (t >> p.src_shift)] +
-                                              (int64_t)(t & ((1 << p.src_shift) - 1)) * p.row_bytes
-                                        : p.src + stream * p.src_stride + (int64_t)t * p.row_bytes;
-      v = ((const U *)from)[c];
-    }
-    uint8_t *to = p.dst_pages ? p.dst_pages[stream * p.dst_max_pages + (o >> p.dst_shift)] +
-                                    (int64_t)(o & ((1 << p.dst_shift) - 1)) * p.row_bytes
-                              : p.dst + stream * p.dst_stride + (int64_t)o * p.row_bytes;
-    if (o < keep || p.dst_pages) ((U *)to)[c] = v;
-  }
-}
+// Rows of the listed positions, a workgroup per `rows_per` result rows of one
+// stream and one array: their source positions are read once into LDS. A row
+// moves in units of 8 or 4 bytes, the units of a workgroup in the order of the
+// result, kMoves per thread in flight. Bound by the bytes, of which the source's
+// come in whole 64-byte pieces: a 72-byte row out of its neighbours costs about
+// two of them.
+constexpr int kGatherRows = 256, kMoves = 8;
 
 struct GatherKernelArgs {
   GatherArgs a;
   FastDiv per_row[kMaxGather];   // units of a row
+  int rows_per;
 };
+
+template <typename U>
+__device__ __forceinline__ void gather_part(const GatherPart &p, const int *src, int64_t stream, int row0, int rows,
+                                            FastDiv per_row) {
+  const uint32_t n = per_row.d, total = (uint32_t)rows * n;
+  for (uint32_t i0 = threadIdx.x; i0 < total; i0 += 256 * kMoves) {
+    U v[kMoves];
+#pragma unroll
+    for (int j = 0; j < kMoves; ++j) {
+      const uint32_t i = i0 + 256 * j;
+      v[j] = 0;
+      if (i >= total) continue;
+      const uint32_t r = per_row.div(i);
+      const int t = src[r];
+      if (t < 0) continue;
+      const uint8_t *from = p.src_pages ? p.src_pages[stream * p.src_max_pages + (t >> p.src_shift)] +
+                                              (int64_t)(t & ((1 << p.src_shift) - 1)) * p.row_bytes
+                                        : p.src + stream * p.src_stride + (int64_t)t * p.row_bytes;
+      v[j] = ((const U *)from)[i - r * n];
+    }
+#pragma unroll
+    for (int j = 0; j < kMoves; ++j) {
+      const uint32_t i = i0 + 256 * j;
+      if (i >= total) continue;
+      const uint32_t r = per_row.div(i);
+      const int o = row0 + (int)r;
+      uint8_t *to = p.dst_pages ? p.dst_pages[stream * p.dst_max_pages + (o >> p.dst_shift)] +
+                                      (int64_t)(o & ((1 << p.dst_shift) - 1)) * p.row_bytes
+                                : p.dst + stream * p.dst_stride + (int64_t)o * p.row_bytes;
+      ((U *)to)[i - r * n] = v[j];
+    }
+  }
+}
 
 __global__ void __launch_bounds__(256) gather_rows_kernel(const GatherKernelArgs k) {
   __shared__ int src[kGatherRows];
   const GatherArgs &a = k.a;
-  const uint32_t tiles = (uint32_t)(a.fill + kGatherRows - 1) / kGatherRows;
+  const uint32_t tiles = (uint32_t)(a.fill + k.rows_per - 1) / (uint32_t)k.rows_per;
   const int64_t stream = blockIdx.x / tiles;
-  const int row0 = (int)(blockIdx.x - (uint32_t)stream * tiles) * kGatherRows, rows = min(kGatherRows, a.fill - row0);
+  const int row0 = (int)(blockIdx.x - (uint32_t)stream * tiles) * k.rows_per;
+  const GatherPart &p = a.part[blockIdx.y];
+  // contiguous results end at keep; pages are filled up with zeros
+  const int rows = min(k.rows_per, (p.dst_pages ? a.fill : a.keep) - row0);
   if ((int)threadIdx.x < rows) {
     const int o = row0 + (int)threadIdx.x;
     const int t = o < a.keep ? a.kept[stream * a.keep + o] : -1;
     src[threadIdx.x] = t < a.S ? t : -1;   // a position outside the cache moves zeros
   }
   __syncthreads();
-  for (int i = 0; i < a.n_parts; ++i) {
-    const GatherPart &p = a.part[i];
-    if (p.unit == 8) gather_part<uint64_t>(p, src, stream, row0, rows, a.keep, k.per_row[i]);
-    else gather_part<uint32_t>(p, src, stream, row0, rows, a.keep, k.per_row[i]);
-  }
+  if (rows <= 0) return;
+  if (p.unit == 8) gather_part<uint64_t>(p, src, stream, row0, rows, k.per_row[blockIdx.y]);
+  else gather_part<uint32_t>(p, src, stream, row0, rows, k.per_row[blockIdx.y]);
 }
 
 }  // namespace
 
 hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_streams, int S, int keep, int sink,
                                int recent, int *kept, hipStream_t s) {
-  evict_select_kernel<<<(unsigned)n_streams, kSelThreads, 0, s>>>(weights, stride, S, keep, sink, recent, kept);
+  const int steps = (S + kSelThreads - 1) / kSelThreads;
+#define PQKV_SELECT(K) \
+  evict_select_kernel<K><<<(unsigned)n_streams, kSelThreads, 0, s>>>(weights, stride, S, keep, sink, recent, kept)
+  if (steps <= 2) PQKV_SELECT(2);
+  else if (steps <= 8) PQKV_SELECT(8);
+  else if (steps <= 16) PQKV_SELECT(16);
+  else if (steps <= 32) PQKV_SELECT(32);
+  else if (steps <= 64) PQKV_SELECT(64);
+  else PQKV_SELECT(0);
+#undef PQKV_SELECT
   return hipGetLastError();
 }
 
 hipError_t launch_gather_rows(const GatherArgs &a, int64_t n_streams, hipStream_t s) {
-  const int64_t grid = (int64_t)((a.fill + kGatherRows - 1) / kGatherRows) * n_streams;
+  // fewer rows per workgroup where that leaves compute units without one
+  const int rows_per = (int64_t)a.fill * n_streams < 1024 * kGatherRows ? 64 : kGatherRows;
+  const dim3 grid((unsigned)((int64_t)((a.fill + rows_per - 1) / rows_per) * n_streams), a.n_parts);
   auto units = [&](int i) { return FastDiv(i < a.n_parts ? (uint32_t)(a.part[i].row_bytes / a.part[i].unit) : 1u); };
-  const GatherKernelArgs k{a, {units(0), units(1), units(2), units(3), units(4), units(5)}};
-  gather_rows_kernel<<<(unsigned)grid, 256, 0, s>>>(k);
+  const GatherKernelArgs k{a, {units(0), units(1), units(2), units(3), units(4), units(5)}, rows_per};
+  gather_rows_kernel<<<grid, 256, 0, s>>>(k);
   return hipGetLastError();
 }
 

@@ -274,9 +274,12 @@ hipError_t launch_decode_mfma_paged(const DecodeArgs &a, int bits, hipStream_t s
 // The same kernels writing a.logits (keys and values of `bits` each, contiguous
 // or, with a.k_pages, paged).
 hipError_t launch_decode_mfma_logits(const DecodeArgs &a, int bits, hipStream_t s);
-// weights_out = weights_in + the softmax weights of a decode call, summed over
-// each kv head's query heads, from its logits and its splits' partials.
-hipError_t launch_decode_weights(const DecodeArgs &a, const DecodeWeights &w, hipStream_t s);
+// The end of such a call: out as launch_decode_merge (with R), and w.out = w.in
+// + the softmax weights summed over each kv head's query heads, from the logits
+// and the splits' partials.
+constexpr int kMaxGroupWeights = 1024;   // query heads per kv head
+hipError_t launch_decode_merge_weights(const DecodeArgs &a, const DecodeWeights &w, const float *R, void *out,
+                                       int out_dtype, hipStream_t s);
 // Mixed widths with kv heads of exactly two kinds, 4-bit K and V sharing one
 // codebook (a4) and 2-bit K and V (a2): one launch over both head lists.
 hipError_t launch_decode_mfma_pair(const DecodeArgs &a4, const DecodeArgs &a2, hipStream_t s);
@@ -387,19 +390,19 @@ struct AttnWeightsArgs {
   const float *codebook;         // [16]
   int bits, B, Hq, Hkv, G, Sq, q_start, S, S_max, d, causal;
   int row0, rows;                // this pass's rows of every stream
-  int row_tiles;                 // their 16-row records, an even count
+  int row_tiles;                 // their 16-row records, a multiple of four
   int tblocks, chunks, chunk_rows;   // token blocks; row chunks of chunk_rows (a multiple of 32)
   uint8_t *records;              // [stream][row_tiles] the rows as matrix operands
   float *row_factor;             // [stream][16 row_tiles]: undoes each row's power of two
   float2 *part;                  // [stream][tblocks][rows]: maximum and sum over the block's tokens
-  float2 *stat;                  // [stream][rows]: maximum and 1 / sum over all tokens
-  float *col;                    // [stream][chunk][tblocks * weight_tokens]: sums over a chunk's rows
+  float2 *stat;                  // [stream][16 row_tiles]: maximum and 1 / sum over all tokens
+  int tokens;                    // tokens of a workgroup: 128 (with QJL always) or 256
+  float *col;                    // [stream][chunk][tblocks * tokens]: sums over a chunk's rows
   const float *in;
   int64_t in_stride;
   float *out;
   int64_t out_stride;
 };
-constexpr int weight_tokens(bool qjl) { return qjl ? 128 : 256; }   // tokens per workgroup
 hipError_t launch_attn_weights(const AttnWeightsArgs &a, hipStream_t s);
 // out = in (or zeros) for S tokens of every stream.
 hipError_t launch_weights_copy(const float *in, int64_t in_stride, float *out, int64_t out_stride, int64_t streams,

@@ -3,6 +3,7 @@
 // tokens (attn_weights_kernel).
 #include <type_traits>
 
+#include "pqkv_decode_merge.h"
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
@@ -34,19 +35,21 @@ __device__ __forceinline__ float rows4_sum(float x) {
 // with M and L merged from the splits' partials. A workgroup takes 1024
 // tokens of one (batch, kv head): it merges the group's partials first (few,
 // and in L2), then reads one row of logits per head, four tokens per thread.
-// Bound by those rows: 4 (G + 2) bytes per token and kv head.
+// Bound by those rows: 4 (G + 2) bytes per token and kv head. The same launch
+// joins the output's splits (decode_merge_body, the workgroups after them),
+// which needs nothing of the weights: a launch less.
 constexpr int kDwTokens = 1024;
 
 template <bool VEC>
-__global__ void __launch_bounds__(256) decode_weights_kernel(const DecodeArgs a, const DecodeWeights w) {
-  extern __shared__ float2 ml[];   // per head of the group: M, 1 / L
+__device__ __forceinline__ void decode_weights_body(float2 *ml, const DecodeArgs &a, const DecodeWeights &w,
+                                                    uint32_t blk) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t tiles = (uint32_t)(a.S + kDwTokens - 1) / kDwTokens;
-  const int64_t bh = blockIdx.x / tiles;
-  const int t0 = (int)(blockIdx.x - (uint32_t)bh * tiles) * kDwTokens + 4 * tid;
+  const int64_t bh = blk / tiles;
+  const int t0 = (int)(blk - (uint32_t)bh * tiles) * kDwTokens + 4 * tid;
   const int b = (int)(bh / a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
   const int64_t row0 = (int64_t)b * a.Hq + (int64_t)h * a.gq;
-  for (int g = wave; g < a.gq; g += 4) {
+  for (int g = wave; g < a.gq; g += 4) {   // ml: per head of the group M, 1 / L
     const float *p = a.part + (row0 + g) * a.split_stride * (a.d + 2);
     float mx = -INFINITY, L = 0.0f;
     for (int sp = lane; sp < a.split_stride; sp += 64) mx = fmaxf(mx, p[(int64_t)sp * (a.d + 2)]);
@@ -87,6 +90,23 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const DecodeArgs a,
     if (t0 + j < a.S) out[j] = (in ? in[j] : 0.0f) + sum[j];
 }
 
+template <int D, typename TOUT, bool VEC>
+__global__ void __launch_bounds__(256) decode_merge_weights_kernel(const DecodeArgs a, const DecodeWeights w,
+                                                                  const float *__restrict__ R,
+                                                                  TOUT *__restrict__ out, int weight_blocks) {
+  __shared__ union {
+    MergeSmem<D> merge;
+    float2 ml[kMaxGroupWeights];
+  } sm;
+  const int blk = blockIdx.x;
+  if (blk < weight_blocks) {
+    decode_weights_body<VEC>(sm.ml, a, w, (uint32_t)blk);
+  } else {
+    const int m = blk - weight_blocks;
+    decode_merge_body<D, TOUT, true>(sm.merge, a.part, R, out, a.B * a.Hq, a.split_stride, m / (D / 32), m % (D / 32));
+  }
+}
+
 // ---- of a chunk of query tokens ----
 //
 // Row r = i G + g of a (batch, kv head) stream is query token i of the
@@ -121,6 +141,7 @@ struct WeightsKernelArgs {
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) const half8_t lds_chalf8;
 
 template <int D, bool QJL>
@@ -197,10 +218,11 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
   }
 }
 
-template <int D, bool QJL, bool STATS>
-__global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const WeightsKernelArgs k) {
+// TT: 16-token tiles per wave.
+template <int D, bool QJL, int TT, bool STATS>
+__global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights_kernel(const WeightsKernelArgs k) {
   using Rec = RowRec<D, QJL>;
-  constexpr int KS = Rec::KS, TT = weight_tokens(QJL) / (16 * kWW), RT = kStage / 16;
+  constexpr int KS = Rec::KS, TOK = 16 * TT * kWW, RT = kStage / 16;
   constexpr int SEGS = RT * Rec::BYTES / 1024;
   __shared__ __attribute__((aligned(16))) uint8_t qb[2][RT * Rec::BYTES];
   __shared__ float2 pair_tab[256];                 // 4-bit: byte -> two centroids; 2-bit: nibble
@@ -228,14 +250,14 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
   const uint32_t n_streams = (uint32_t)(a.B * a.Hkv);
   const int chunk = a.chunks - 1 - (int)(gi / n_streams), tb = (int)tbu;
   const int64_t stream = gi % n_streams;
-  const int t0 = tb * weight_tokens(QJL), tw0 = t0 + 16 * TT * wave, tw1 = tw0 + 16 * TT - 1;
+  const int t0 = tb * TOK, tw0 = t0 + 16 * TT * wave, tw1 = tw0 + 16 * TT - 1;
   int r_begin = chunk * a.chunk_rows;
   const int r_end = min(r_begin + a.chunk_rows, a.rows);
   if (a.causal) {   // the first row that sees token t0
     const int64_t first = (int64_t)(t0 - a.q_start) * a.G - a.row0;
     if (first >= r_end) {
       if (!STATS && a.chunks == 1)   // no row sees the block: what there was stays
-        for (int t = t0 + tid; t < min(t0 + weight_tokens(QJL), a.S); t += 64 * kWW)
+        for (int t = t0 + tid; t < min(t0 + TOK, a.S); t += 64 * kWW)
           a.out[stream * a.out_stride + t] = a.in ? a.in[stream * a.in_stride + t] : 0.0f;
       return;
     }
@@ -246,17 +268,17 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
   const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
       (void *)records, (short)0, (int)((int64_t)a.row_tiles * Rec::BYTES), 0x00020000);
   const float *factor = a.row_factor + stream * a.row_tiles * 16;
-  auto copy_stage = [&](int s) {
+  const float2 *stat = a.stat + stream * a.row_tiles * 16;
+  auto copy_stage = [&](int s, lds_u8 *__restrict dst) {
     const int at = __builtin_amdgcn_readfirstlane(s * RT * Rec::BYTES);
 #pragma unroll
     for (int j = 0; j < SEGS / kWW; ++j) {
       const int sg = wave + kWW * j;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (lds_void *)(qb[s & 1] + 1024 * sg), 16, 16 * lane, at + 1024 * sg,
-                                               0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (lds_void *)(dst + 1024 * sg), 16, 16 * lane, at + 1024 * sg, 0, 0);
     }
   };
   const int s0 = r_begin / kStage, s1 = (r_end + kStage - 1) / kStage;
-  copy_stage(s0);
+  copy_stage(s0, (lds_u8 *)qb[s0 & 1]);
 
   // ---- this wave's keys, 16 TT tokens: lane (col, grp) holds coordinates
   // 32 ks + 8 grp .. + 7 of token 16 tt + col ----
@@ -343,8 +365,8 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = kStage * s + 16 * rt + col;
-      o.f[rt] = factor[r] * kundo;
-      if constexpr (!STATS) o.x[rt] = r < a.rows ? a.stat[stream * a.rows + r] : make_float2(INFINITY, 0.0f);
+      o.f[rt] = factor[r];
+      if constexpr (!STATS) o.x[rt] = stat[r];
     }
     return o;
   };
@@ -354,36 +376,51 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
 #pragma unroll
     for (int i = 0; i < 4; ++i) csum[tt][i] = 0.0f;
 
-  auto compute = [&](int s, const RowInfo &info, auto masked) {
+  // Stage s out of buf; stage s + 1 (if `more`) is copied into the other buffer
+  // meanwhile. (The two are restricted pointers so that the compiler knows the
+  // copy apart from the reads: it would wait for it before the first of them.)
+  auto compute = [&](int s, const RowInfo &info, const lds_u8 *__restrict buf, lds_u8 *__restrict other, bool more,
+                     auto masked) {
     constexpr bool kMasked = decltype(masked)::value;
-    const lds_chalf8 *q = (const lds_chalf8 *)(qb[s & 1] + 16 * lane);
+    if (more) copy_stage(s + 1, other);
+    const lds_chalf8 *q = (const lds_chalf8 *)(buf + 16 * lane);
     float4_t acc[RT][TT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) acc[rt][tt] = (float4_t){0.f, 0.f, 0.f, 0.f};
+    // step n = (row tile, k-step); its operands are read one step ahead (the
+    // fence holds products and reads in place, other work may move)
+    half8_t rows[2][Rec::PARTS];
+    auto read = [&](int n) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+      for (int p = 0; p < Rec::PARTS; ++p) rows[n & 1][p] = q[(n * Rec::PARTS + p) * 64];
+    };
+    read(0);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const half8_t bh = q[((rt * KS + ks) * Rec::PARTS) * 64], bl = q[((rt * KS + ks) * Rec::PARTS + 1) * 64];
+    for (int n = 0; n < RT * KS; ++n) {
+      const int rt = n / KS, ks = n % KS;
+      if (n + 1 < RT * KS) read(n + 1);
+      __builtin_amdgcn_sched_barrier(0x0676);
+      const half8_t bh = rows[n & 1][0], bl = rows[n & 1][1];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[tt][ks], bh, acc[rt][tt], 0, 0, 0);
+        acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bl, acc[rt][tt], 0, 0, 0);
+        acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bh, acc[rt][tt], 0, 0, 0);
+      }
+      if constexpr (QJL) {
+        const half8_t ph = rows[n & 1][2], pl = rows[n & 1][3];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[tt][ks], bh, acc[rt][tt], 0, 0, 0);
-          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bl, acc[rt][tt], 0, 0, 0);
-          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[tt][ks], bh, acc[rt][tt], 0, 0, 0);
-        }
-        if constexpr (QJL) {
-          const half8_t ph = q[((rt * KS + ks) * Rec::PARTS + 2) * 64], pl = q[((rt * KS + ks) * Rec::PARTS + 3) * 64];
-#pragma unroll
-          for (int tt = 0; tt < TT; ++tt) {
-            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], pl, acc[rt][tt], 0, 0, 0);
-            acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], ph, acc[rt][tt], 0, 0, 0);
-          }
+          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], pl, acc[rt][tt], 0, 0, 0);
+          acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(sg[tt][ks], ph, acc[rt][tt], 0, 0, 0);
         }
       }
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      const float f = info.f[rt] * kundo;
       int last = a.S - 1;   // the last token the lane's row sees
       if (kMasked && a.causal)
         last = min(last, a.q_start + (int)k.group.div((uint32_t)(kStage * s + 16 * rt + col + a.row0)));
@@ -397,13 +434,13 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
             if (kMasked && 16 * tt + i > rel) acc[rt][tt][i] = -INFINITY;
             m = fmaxf(m, acc[rt][tt][i]);
           }
-        m = rows4_max(m) * info.f[rt];      // the factor is positive: the maximum stays where it is
+        m = rows4_max(m) * f;      // the factor is positive: the maximum stays where it is
         const float ref = kMasked && m == -INFINITY ? 0.0f : m;
         float l = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], info.f[rt], -ref));
+          for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], f, -ref));
         l = rows4_sum(l);
         if (grp == 0) st[s & 1][wave][16 * rt + col] = make_float2(m, l);
       } else {
@@ -411,7 +448,7 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], info.f[rt], -info.x[rt].x));
+            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], f, -info.x[rt].x));
             if (kMasked && 16 * tt + i > rel) e = 0.0f;
             csum[tt][i] = __builtin_fmaf(e, info.x[rt].y, csum[tt][i]);
           }
@@ -436,20 +473,19 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
   for (int s = s0; s < s1; ++s) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // stage s has arrived (this wave's part)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // everyone's; stage s - 1 has been read
-    RowInfo next = info;
-    if (s + 1 < s1) {
-      copy_stage(s + 1);
-      next = row_info(s + 1);
-    }
+    const bool more = s + 1 < s1;
+    const RowInfo next = row_info(more ? s + 1 : s);
     if (STATS && s > s0) write_stats(s - 1);
+    lds_u8 *buf = (lds_u8 *)qb[s & 1], *other = (lds_u8 *)qb[(s + 1) & 1];
     const int p_first = a.q_start + (int)k.group.div((uint32_t)(kStage * s + a.row0));
     const int p_last = a.q_start + (int)k.group.div((uint32_t)(kStage * s + kStage - 1 + a.row0));
-    if (tw0 >= a.S || (a.causal && p_last < tw0)) {
-      if (STATS && lane < kStage) st[s & 1][wave][lane] = make_float2(-INFINITY, 0.0f);   // none of its tokens
+    if (tw0 >= a.S || (a.causal && p_last < tw0)) {   // none of the wave's tokens
+      if (more) copy_stage(s + 1, other);
+      if (STATS && lane < kStage) st[s & 1][wave][lane] = make_float2(-INFINITY, 0.0f);
     } else if (tw1 >= a.S || (a.causal && p_first < tw1)) {
-      compute(s, info, std::true_type{});
+      compute(s, info, buf, other, more, std::true_type{});
     } else {
-      compute(s, info, std::false_type{});
+      compute(s, info, buf, other, more, std::false_type{});
     }
     info = next;
   }
@@ -468,24 +504,25 @@ __global__ void __launch_bounds__(64 * kWW, 2) attn_weights_kernel(const Weights
       for (int sft = 1; sft < 16; sft <<= 1) v += shfl_xor_f(v, sft);
       const int t = tw0 + 16 * tt + 4 * grp + i;
       if (col == 0) {
-        if (a.chunks > 1) a.col[((stream * a.chunks + chunk) * a.tblocks + tb) * weight_tokens(QJL) + t - t0] = v;
+        if (a.chunks > 1) a.col[((stream * a.chunks + chunk) * a.tblocks + tb) * TOK + t - t0] = v;
         else if (t < a.S)
           a.out[stream * a.out_stride + t] = (a.in ? a.in[stream * a.in_stride + t] : 0.0f) + v;
       }
     }
 }
 
-// Joins the token blocks' maxima and sums of 32 rows, eight threads per row.
-__global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs k, int tokens) {
+// Joins the token blocks' maxima and sums of 32 rows, eight threads per row;
+// rows past the last one get (inf, 0), whose weights are 0.
+__global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs k) {
   __shared__ float2 sub[8][32];
   const AttnWeightsArgs &a = k.a;
-  const uint32_t tiles = (uint32_t)(a.rows + 31) / 32;
+  const uint32_t tiles = (uint32_t)a.row_tiles / 2;
   const int64_t stream = blockIdx.x / tiles;
   const int rl = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int r = (int)(blockIdx.x - (uint32_t)stream * tiles) * 32 + rl;
   const int rr = min(r, a.rows - 1);
   const int last = a.causal ? min(a.q_start + (int)k.group.div((uint32_t)(rr + a.row0)), a.S - 1) : a.S - 1;
-  const int n = last / tokens + 1;
+  const int n = last / a.tokens + 1;
   const float2 *p = a.part + stream * a.tblocks * a.rows + rr;
   float m = -INFINITY, l = 0.0f;
   auto join = [&](float2 x) {
@@ -498,28 +535,28 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs
   for (int i = q; i < n; i += 8) join(p[(int64_t)i * a.rows]);
   sub[q][rl] = make_float2(m, l);
   __syncthreads();
-  if (q != 0 || r >= a.rows) return;
+  if (q != 0) return;
 #pragma unroll
   for (int i = 1; i < 8; ++i) join(sub[i][rl]);
-  a.stat[stream * a.rows + r] = make_float2(m, 1.0f / l);
+  a.stat[stream * a.row_tiles * 16 + r] = r < a.rows ? make_float2(m, 1.0f / l) : make_float2(INFINITY, 0.0f);
 }
 
 // out = in + the row chunks' sums of one token, in the chunks' order.
-__global__ void __launch_bounds__(256) weights_join_kernel(const AttnWeightsArgs a, int tokens) {
+__global__ void __launch_bounds__(256) weights_join_kernel(const AttnWeightsArgs a) {
   const uint32_t tiles = (uint32_t)(a.S + 255) / 256;
   const int64_t stream = blockIdx.x / tiles;
   const int t = (int)(blockIdx.x - (uint32_t)stream * tiles) * 256 + threadIdx.x;
   if (t >= a.S) return;
-  const int tb = t / tokens;
+  const int tb = t / a.tokens;
   int c0 = 0;
   if (a.causal) {   // chunks that end before the first row that sees the block were not computed
-    const int64_t first = (int64_t)(tb * tokens - a.q_start) * a.G - a.row0;
+    const int64_t first = (int64_t)(tb * a.tokens - a.q_start) * a.G - a.row0;
     if (first >= a.rows) c0 = a.chunks;
     else if (first > 0) c0 = (int)(first / a.chunk_rows);
   }
   float sum = 0.0f;
 #pragma unroll 4
-  for (int c = c0; c < a.chunks; ++c) sum += a.col[((stream * a.chunks + c) * a.tblocks) * (int64_t)tokens + t];
+  for (int c = c0; c < a.chunks; ++c) sum += a.col[((stream * a.chunks + c) * a.tblocks) * (int64_t)a.tokens + t];
   a.out[stream * a.out_stride + t] = (a.in ? a.in[stream * a.in_stride + t] : 0.0f) + sum;
 }
 
@@ -531,37 +568,53 @@ __global__ void __launch_bounds__(256) weights_copy_kernel(const float *in, int6
   if (t < S) out[stream * out_stride + t] = in ? in[stream * in_stride + t] : 0.0f;
 }
 
-template <int D, bool QJL>
+template <int D, bool QJL, int TT>
 void launch_passes(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
-  constexpr int tokens = weight_tokens(QJL);
   WeightsKernelArgs k{a, FastDiv((uint32_t)a.G), 0};
   const int64_t groups = streams * a.chunks;
   if (groups % 8 == 0 || groups >= 64) k.xcd_groups = (int)groups;
   const unsigned grid = (unsigned)((k.xcd_groups ? (groups + 7) / 8 * 8 : groups) * a.tblocks);
   weights_rows_kernel<D, QJL><<<(unsigned)(streams * a.row_tiles), 2 * D, 0, s>>>(k);
-  attn_weights_kernel<D, QJL, true><<<grid, 64 * kWW, 0, s>>>(k);
-  attn_stats_kernel<<<(unsigned)(streams * ((a.rows + 31) / 32)), 256, 0, s>>>(k, tokens);
-  attn_weights_kernel<D, QJL, false><<<grid, 64 * kWW, 0, s>>>(k);
+  attn_weights_kernel<D, QJL, TT, true><<<grid, 64 * kWW, 0, s>>>(k);
+  attn_stats_kernel<<<(unsigned)(streams * (a.row_tiles / 2)), 256, 0, s>>>(k);
+  attn_weights_kernel<D, QJL, TT, false><<<grid, 64 * kWW, 0, s>>>(k);
   if (a.chunks > 1)   // (one chunk: the sums are the result)
-    weights_join_kernel<<<(unsigned)(streams * ((a.S + 255) / 256)), 256, 0, s>>>(a, tokens);
+    weights_join_kernel<<<(unsigned)(streams * ((a.S + 255) / 256)), 256, 0, s>>>(a);
+}
+
+template <int D>
+void launch_head(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
+  if (a.pq != nullptr) launch_passes<D, true, 2>(a, streams, s);
+  else if (a.tokens == 128) launch_passes<D, false, 2>(a, streams, s);
+  else launch_passes<D, false, 4>(a, streams, s);
 }
 
 }  // namespace
 
-hipError_t launch_decode_weights(const DecodeArgs &a, const DecodeWeights &w, hipStream_t s) {
-  const unsigned grid = (unsigned)((int64_t)((a.S + kDwTokens - 1) / kDwTokens) * a.B * a.Hkv);
-  const size_t lds = (size_t)a.gq * sizeof(float2);
+hipError_t launch_decode_merge_weights(const DecodeArgs &a, const DecodeWeights &w, const float *R, void *out,
+                                       int out_dtype, hipStream_t s) {
+  if (a.split_stride > kMaxSplits || a.gq > kMaxGroupWeights) return hipErrorInvalidValue;
+  const int wb = (int)((int64_t)((a.S + kDwTokens - 1) / kDwTokens) * a.B * a.Hkv);
+  const int mb = (a.B * a.Hq + kMergeHeads - 1) / kMergeHeads * (a.d / 32);
   const bool vec = ((uintptr_t)w.out | (uintptr_t)w.in) % 16 == 0 && (w.out_stride | (w.in ? w.in_stride : 0)) % 4 == 0;
-  if (vec) decode_weights_kernel<true><<<grid, 256, lds, s>>>(a, w);
-  else decode_weights_kernel<false><<<grid, 256, lds, s>>>(a, w);
+#define PQKV_DMW(DD, T, V) \
+  decode_merge_weights_kernel<DD, T, V><<<(unsigned)(wb + mb), 256, 0, s>>>(a, w, R, (T *)out, wb)
+#define PQKV_DMW_V(DD, T) \
+  if (vec) PQKV_DMW(DD, T, true); \
+  else PQKV_DMW(DD, T, false)
+  if (a.d == 128 && out_dtype == PQKV_F32) { PQKV_DMW_V(128, float); }
+  else if (a.d == 128) { PQKV_DMW_V(128, half_t); }
+  else if (out_dtype == PQKV_F32) { PQKV_DMW_V(64, float); }
+  else { PQKV_DMW_V(64, half_t); }
+#undef PQKV_DMW_V
+#undef PQKV_DMW
   return hipGetLastError();
 }
 
 hipError_t launch_attn_weights(const AttnWeightsArgs &a, hipStream_t s) {
   const int64_t streams = (int64_t)a.B * a.Hkv;
-  const bool qjl = a.pq != nullptr;
-  if (a.d == 128) qjl ? launch_passes<128, true>(a, streams, s) : launch_passes<128, false>(a, streams, s);
-  else qjl ? launch_passes<64, true>(a, streams, s) : launch_passes<64, false>(a, streams, s);
+  if (a.d == 128) launch_head<128>(a, streams, s);
+  else launch_head<64>(a, streams, s);
   return hipGetLastError();
 }
 

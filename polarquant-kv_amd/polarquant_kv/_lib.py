@@ -198,9 +198,10 @@ def dtype_code(t) -> int:
 
 
 def stream_of(t) -> int:
-    """The current torch stream of the tensor's device, as a hipStream_t."""
+    """The current torch stream of the tensor's device, as a hipStream_t (the
+    raw handle: torch.cuda.current_stream builds a Stream object around it, 3 us)."""
     import torch
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def ptr(t) -> int | None:

@@ -17,6 +17,7 @@ import math
 import torch
 
 from . import _lib
+from .eviction import _check_rows, _row_stride
 from .types import PagedPQCache, PQCache, vector_bytes
 
 
@@ -152,7 +153,6 @@ def _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype
 def _weights_args(B, H, S, previous, into, device):
     """(previous, into, result) of a call that gives weights: the tensors it
     reads and writes, rows [B, H] one stride apart, and the [B, H, S] result."""
-    from .eviction import _check_rows
     for name, t in (("previous", previous), ("into", into)):
         if t is None:
             continue
@@ -179,7 +179,6 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
     (same shape; may be previous itself) receives them, positions from S on
     left as they are. keys / values: PQCache or PagedPQCache of one and the
     same width (pqkv_decode_attn_weights, _paged)."""
-    from .eviction import _row_stride
     if query.dim() != 3:
         raise ValueError(f"query must be [B, Hq, d], got {tuple(query.shape)}")
     B, Hq, d = query.shape
@@ -230,7 +229,6 @@ def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, 
     `into` where given (both as decode_attention_weights takes them). keys:
     PQCache (one width) or PagedPQCache that already holds the chunk; causal as
     prefill_attention (pqkv_attn_weights, _paged)."""
-    from .eviction import _row_stride
     if query.dim() != 4:
         raise ValueError(f"query must be [B, Hq, Sq, d], got {tuple(query.shape)}")
     B, Hq, Sq, d = query.shape

@@ -62,21 +62,19 @@ def select_positions(weights: torch.Tensor, keep: int, sink: int = 0, recent: in
 
 
 def _cache_arrays(cache):
-    """The (array, row bytes) of a cache's blocks and, with signs, of those."""
-    d = cache.head_dim
-    out = []
+    """(fields of pqkv_row_array, row bytes) of a cache's blocks and, with
+    signs, of those."""
+    vb = vector_bytes(cache.head_dim, cache.n_bits)
     if isinstance(cache, PagedPQCache):
-        out.append((_lib.RowArray(None, cache.table.data_ptr(), 0, cache.page_tokens, cache.max_pages),
-                    vector_bytes(d, cache.n_bits)))
+        out = [((None, cache.table.data_ptr(), 0, cache.page_tokens, cache.max_pages), vb)]
         if cache.sign_table is not None:
-            out.append((_lib.RowArray(None, cache.sign_table.data_ptr(), 0, cache.page_tokens, cache.max_pages),
+            out.append(((None, cache.sign_table.data_ptr(), 0, cache.page_tokens, cache.max_pages),
                         cache.jl_dim // 8))
         return out
-    vb = vector_bytes(d, cache.n_bits)
-    out.append((_lib.RowArray(cache.blocks.data_ptr(), None, cache.max_seq_len * vb, 0, 0), vb))
+    out = [((cache.blocks.data_ptr(), None, cache.max_seq_len * vb, 0, 0), vb)]
     if cache.qjl_signs is not None:
         m8 = cache.qjl_signs.shape[-1]
-        out.append((_lib.RowArray(cache.qjl_signs.data_ptr(), None, cache.max_seq_len * m8, 0, 0), m8))
+        out.append(((cache.qjl_signs.data_ptr(), None, cache.max_seq_len * m8, 0, 0), m8))
     return out
 
 
@@ -85,18 +83,15 @@ def _empty_like(cache, positions: int, room: int):
     `room` positions), its rows not yet written."""
     B, H, d = cache.batch, cache.num_heads, cache.head_dim
     if isinstance(cache, PagedPQCache):
-        new = PagedPQCache(B, H, d, cache.n_bits, cache.codebooks, cache.device, page_tokens=cache.page_tokens,
-                           jl_dim=cache.jl_dim, max_pages=max(1, -(-positions // cache.page_tokens)))
-        new.reserve(positions)
-        return new
-    vb = vector_bytes(d, cache.n_bits)
+        return PagedPQCache(B, H, d, cache.n_bits, cache.codebooks, cache.device, page_tokens=cache.page_tokens,
+                            jl_dim=cache.jl_dim, max_pages=1, reserve=positions)
     fresh = torch.empty if room == positions else torch.zeros
-    signs = None
+    device, signs = cache.blocks.device, None
     if cache.qjl_signs is not None:
-        signs = fresh(B, H, room, cache.qjl_signs.shape[-1], dtype=torch.uint8, device=cache.blocks.device)
-    return PQCache(blocks=fresh(B, H, room, vb, dtype=torch.uint8, device=cache.blocks.device), head_dim=d,
-                   n_bits=cache.n_bits, seq_len=0, max_seq_len=room, codebooks=cache.codebooks, qjl_signs=signs,
-                   jl_dim=cache.jl_dim)
+        signs = fresh(B, H, room, cache.qjl_signs.shape[-1], dtype=torch.uint8, device=device)
+    return PQCache(blocks=fresh(B, H, room, vector_bytes(d, cache.n_bits), dtype=torch.uint8, device=device),
+                   head_dim=d, n_bits=cache.n_bits, seq_len=0, max_seq_len=room, codebooks=cache.codebooks,
+                   qjl_signs=signs, jl_dim=cache.jl_dim)
 
 
 def _check_cache(cache, name: str, B: int, H: int, device) -> None:
@@ -148,11 +143,11 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
             raise ValueError(f"cache {i} holds {c.seq_len} positions, the first one {S}")
     src, dst, sizes, new_rows = [], [], [], []
     with _lib.on_device(kept):
-        fill = keep
         new = [_empty_like(c, keep, room) for c in caches]
+        capacity = {c.capacity for c in new if isinstance(c, PagedPQCache)}
+        if len(capacity) > 1:
+            raise ValueError("paged caches in one move must share page_tokens")
         for old, c in zip(caches, new):
-            if isinstance(c, PagedPQCache):
-                fill = max(fill, c.capacity)
             for (a, size), (n, _) in zip(_cache_arrays(old), _cache_arrays(c)):
                 src.append(a)
                 dst.append(n)
@@ -165,18 +160,17 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
             t = _check_rows(t, "rows")
             held.append(t)
             n = torch.empty(B, H, keep, dtype=t.dtype, device=t.device)
-            src.append(_lib.RowArray(t.data_ptr(), None, 4 * _row_stride(t), 0, 0))
-            dst.append(_lib.RowArray(n.data_ptr(), None, 4 * keep, 0, 0))
+            src.append((t.data_ptr(), None, 4 * _row_stride(t), 0, 0))
+            dst.append((n.data_ptr(), None, 4 * keep, 0, 0))
             sizes.append(4)
             new_rows.append(n)
         if len(src) > _lib.MAX_GATHER:
             raise ValueError(f"{len(src)} arrays in one move, at most {_lib.MAX_GATHER}")
-        if any(isinstance(c, PagedPQCache) for c in new) and len({c.capacity for c in new if isinstance(c, PagedPQCache)}) > 1:
-            raise ValueError("paged caches in one move must share page_tokens")
         if keep > 0:
-            _lib.check(_lib.lib().pqkv_gather_rows(
-                len(src), (_lib.RowArray * len(src))(*src), (_lib.RowArray * len(dst))(*dst), _lib.int_array(sizes),
-                kept.data_ptr(), B * H, S, keep, fill, _lib.stream_of(kept)))
+            arrays = _lib.RowArray * len(src)
+            _lib.check(_lib.lib().pqkv_gather_rows(len(src), arrays(*src), arrays(*dst), _lib.int_array(sizes),
+                                                   kept.data_ptr(), B * H, S, keep, max(capacity, default=keep),
+                                                   _lib.stream_of(kept)))
     return new, new_rows
 
 

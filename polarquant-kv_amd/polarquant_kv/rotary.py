@@ -121,25 +121,24 @@ def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved, amplitude):
+    def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse):
         ctx.save_for_backward(positions, freqs)
-        ctx.how = (interleaved, amplitude)
+        ctx.how = (interleaved, amplitude, not inverse)
         ctx.set_materialize_grads(False)
-        return _turn(q, k, positions, freqs, interleaved, amplitude, False)
+        return _turn(q, k, positions, freqs, interleaved, amplitude, inverse)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         # y = M x with M a scaled rotation of each pair, so the gradient is the
         # same turn back: linear in g, and nothing of x is kept for it
-        positions, freqs = ctx.saved_tensors
         if gq is None and gk is None:
-            return (None,) * 6
+            return (None,) * 7
+        turn = _Rotary.apply if torch.is_grad_enabled() else _turn      # (create_graph: differentiable again)
         if gq is None:
-            out = (None, _turn(gk, None, positions, freqs, *ctx.how, True)[0])
+            out = (None, turn(gk, None, *ctx.saved_tensors, *ctx.how)[0])
         else:
-            out = _turn(gq, gk, positions, freqs, *ctx.how, True)
-        return *out, None, None, None, None
+            out = turn(gq, gk, *ctx.saved_tensors, *ctx.how)
+        return *out, None, None, None, None, None
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,
@@ -171,8 +170,11 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"positions must be integers, got {positions.dtype}")
     if tuple(positions.shape) not in ((T,), (B, T)):
         raise ValueError(f"positions must be [{T}] or [{B}, {T}], got {tuple(positions.shape)}")
-    positions = positions.to(torch.int64).contiguous()
-    return _Rotary.apply(query, key, positions, frequencies.contiguous(), bool(interleaved), float(amplitude))
+    args = (query, key, positions.to(torch.int64).contiguous(), frequencies.contiguous(), bool(interleaved),
+            float(amplitude))
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        return _Rotary.apply(*args, False)
+    return _turn(*args, False)
 
 
 class RotaryEmbedding:

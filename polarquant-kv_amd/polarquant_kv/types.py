@@ -85,7 +85,7 @@ class PagedPQCache:
     QJL sign pages beside their block pages (same page index)."""
 
     def __init__(self, batch: int, num_heads: int, head_dim: int, n_bits: int, codebooks, device,
-                 page_tokens: int = 256, jl_dim: int = 0, max_pages: int = 16):
+                 page_tokens: int = 256, jl_dim: int = 0, max_pages: int = 16, reserve: int = 0):
         import torch
         if page_tokens < 64 or page_tokens > 65536 or page_tokens & (page_tokens - 1):
             raise ValueError(f"page_tokens must be a power of two in 64..65536, got {page_tokens}")
@@ -96,11 +96,14 @@ class PagedPQCache:
         self.seq_len = 0
         self.groups: list = []        # page group p: uint8 [B, H, page_tokens, vector_bytes]
         self.sign_groups: list = []   # with jl_dim: uint8 [B, H, page_tokens, jl_dim / 8]
+        self._adopted = None          # (capacity, storage) of caller-managed pages
+        if reserve > 0:
+            self.reserve(reserve)
+            return
         self.max_pages = max(1, int(max_pages))
         n = batch * num_heads
         self.table = torch.zeros(n, self.max_pages, dtype=torch.int64, device=self.device)
         self.sign_table = torch.zeros_like(self.table) if jl_dim else None
-        self._adopted = None          # (capacity, storage) of caller-managed pages
 
     def adopt(self, table, capacity: int, storage, sign_table=None) -> None:
         """Use caller-managed pages instead of page groups: table (and, for a
@@ -193,20 +196,22 @@ class PagedPQCache:
         n = -(-int(positions) // self.page_tokens)
         if n == 0:
             return
-        self._widen(n)
+        self.sign_table = None
         B, H, P = self.batch, self.num_heads, self.page_tokens
 
-        def pages(row_bytes, table):
-            g = torch.empty(n, B, H, P, row_bytes, dtype=torch.uint8, device=self.device)
+        def pages(row_bytes):
+            # page p of stream s is number s * n + p, so that the table is one
+            # ascending row of addresses
             size = P * row_bytes
-            # page p of stream s: page number p * B * H + s
-            at = torch.arange(g.data_ptr(), g.data_ptr() + n * B * H * size, size, device=self.device)
-            table[:, :n] = at.view(n, B * H).t()
-            return list(g.unbind(0))
+            g = torch.empty(B, H, n, P, row_bytes, dtype=torch.uint8, device=self.device)
+            at = torch.arange(g.data_ptr(), g.data_ptr() + B * H * n * size, size, dtype=torch.int64,
+                              device=self.device)
+            return list(g.unbind(2)), at.view(B * H, n)
 
-        self.groups = pages(self.vector_bytes, self.table)
-        if self.sign_table is not None:
-            self.sign_groups = pages(self.jl_dim // 8, self.sign_table)
+        self.groups, self.table = pages(self.vector_bytes)
+        if self.jl_dim:
+            self.sign_groups, self.sign_table = pages(self.jl_dim // 8)
+        self.max_pages = n
 
     def memory_bytes(self) -> int:
         """Device bytes of the allocated pages (and the page tables)."""

@@ -237,3 +237,15 @@ def test_turning_by_a_sum_of_positions():
 
     size = (q.abs().double().view(2, -1).sum(0) * k.abs().double().view(2, -1).sum(0)).sum().item()
     assert math.isclose(score(5, 2), score(500005, 500002), abs_tol=4 * 2.0 ** -20 * size)
+
+
+def test_gradient_of_the_gradient():
+    """f is linear in x, so d/dx of <grad f, u> is 0 and d/dg of it is f(u)."""
+    q, _, pos, freqs, _ = make(CASES[3])
+    q = q.requires_grad_(True)
+    out = rotary.apply_rotary(q, None, pos, freqs, interleaved=True, amplitude=1.5)[0]
+    g = torch.randn_like(out).requires_grad_(True)
+    dq, = torch.autograd.grad(out, q, g, create_graph=True)
+    u = torch.randn_like(dq)
+    dg, = torch.autograd.grad(dq, g, u)
+    check(dg.contiguous(), u, pos, freqs, True, 1.5)
