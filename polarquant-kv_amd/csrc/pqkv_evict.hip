@@ -10,7 +10,8 @@
 // the rank. Counts and indices are whole numbers, so no order of the atomic
 // additions changes the result. One workgroup per stream, its keys in registers
 // up to 65536 positions (KPT per thread), so that the weights are read once and
-// all their loads are in flight together; longer streams are read again in each
+// all their loads are in flight together (the thread counts below differ so that
+// at most half of the steps are empty); longer streams are read again in each
 // pass, from L2. Weights crowd into few exponents, so the first digit's
 // additions meet in few bins: there each bin has eight counters, a lane's by its
 // number. Bound by the instructions of one compute unit per stream.
@@ -62,37 +63,40 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float *
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float *w = weights + blockIdx.x * stride;
   int *out = kept + (int64_t)blockIdx.x * keep;
-  // each wave takes one contiguous run of whole 64-position steps
-  const int steps = (S + kSelThreads - 1) / kSelThreads;
-  const int begin = wave * steps * kWave, end = min(S, begin + steps * kWave);
-  auto key_of = [&](int i, float x) { return i < sink || i >= S - recent ? 0xFFFFFFFFu : weight_key(x); };
+  // Each wave takes one contiguous run of whole 64-position steps. Positions
+  // past the last one have the lowest key, and the highest numbers, so they are
+  // never among the first `keep` and need no test of their own.
+  const int steps = KPT > 0 ? KPT : (S + kSelThreads - 1) / kSelThreads;
+  const int begin = wave * steps * kWave;
+  auto key_of = [&](int i, float x) {
+    const uint32_t key = i < sink || i >= S - recent ? 0xFFFFFFFFu : weight_key(x);
+    return i < S ? key : 0u;
+  };
   uint32_t keys[KPT > 0 ? KPT : 1];
   if constexpr (KPT > 0) {
 #pragma unroll
-    for (int j = 0; j < KPT; ++j) {
-      const int i = begin + j * kWave + lane;
-      keys[j] = __builtin_bit_cast(uint32_t, j < steps && i < end ? w[i] : 0.0f);
-    }
+    for (int j = 0; j < KPT; ++j)
+      keys[j] = __builtin_bit_cast(uint32_t, w[min(begin + j * kWave + lane, S - 1)]);
 #pragma unroll
     for (int j = 0; j < KPT; ++j) keys[j] = key_of(begin + j * kWave + lane, __builtin_bit_cast(float, keys[j]));
   }
-  // f(key, position, whether there is one) for the wave's positions, step by step
+  // f(key, position) for the wave's positions, step by step
   auto each = [&](auto f) {
     if constexpr (KPT > 0) {
 #pragma unroll
-      for (int j = 0; j < KPT; ++j) {
-        if (j >= steps) break;
-        const int i = begin + j * kWave + lane;
-        f(keys[j], i, i < end);
-      }
+      for (int j = 0; j < KPT; ++j) f(keys[j], begin + j * kWave + lane);
     } else {
       constexpr int U = 16;   // loads in flight
-      for (int i0 = begin + lane; i0 - lane < end; i0 += U * kWave) {
+      for (int j0 = 0; j0 < steps; j0 += U) {
+        const int i0 = begin + j0 * kWave + lane;
         float x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = i0 + u * kWave < end ? w[i0 + u * kWave] : 0.0f;
+        for (int u = 0; u < U; ++u) x[u] = w[min(i0 + u * kWave, S - 1)];
 #pragma unroll
-        for (int u = 0; u < U; ++u) f(key_of(i0 + u * kWave, x[u]), i0 + u * kWave, i0 + u * kWave < end);
+        for (int u = 0; u < U; ++u) {
+          if (j0 + u >= steps) break;
+          f(key_of(i0 + u * kWave, x[u]), i0 + u * kWave);
+        }
       }
     }
   };
@@ -106,8 +110,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float *
     const uint32_t low = (1u << bits) - 1;
     for (int i = tid; i < kBins * copies / 4; i += kSelThreads) ((u32x4 *)sm.hist)[i] = (u32x4){0u, 0u, 0u, 0u};
     __syncthreads();
-    each([&](uint32_t key, int, bool there) {
-      if (there && (key & mask) == found)
+    each([&](uint32_t key, int) {
+      if ((key & mask) == found)
         atomicAdd(&sm.hist[((key >> shift) & low) * copies + (lane & (copies - 1))], 1u);
     });
     __syncthreads();
@@ -159,27 +163,24 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float *
   };
   uint32_t above = 0, ties = 0, n_above, n_tie;
   if (rank == on_border) {
-    each([&](uint32_t key, int, bool there) {
-      above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key >= found));
-    });
+    each([&](uint32_t key, int) { above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= found)); });
     lead(above, 0, n_above, n_tie);
-    each([&](uint32_t key, int i, bool there) {
-      const uint64_t m = __builtin_amdgcn_ballot_w64(there && key >= found);
-      if (there && key >= found) out[n_above + lanes_below(m)] = i;
+    each([&](uint32_t key, int i) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(key >= found);
+      if (key >= found) out[n_above + lanes_below(m)] = i;
       n_above += __builtin_popcountll(m);
     });
     return;
   }
-  each([&](uint32_t key, int, bool there) {
-    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key > found));
-    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && key == found));
+  each([&](uint32_t key, int) {
+    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > found));
+    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == found));
   });
   lead(above, ties, n_above, n_tie);
-  each([&](uint32_t key, int i, bool there) {
-    const uint64_t ma = __builtin_amdgcn_ballot_w64(there && key > found);
-    const uint64_t mt = __builtin_amdgcn_ballot_w64(there && key == found);
+  each([&](uint32_t key, int i) {
+    const uint64_t ma = __builtin_amdgcn_ballot_w64(key > found), mt = __builtin_amdgcn_ballot_w64(key == found);
     const uint32_t a = n_above + lanes_below(ma), t = n_tie + lanes_below(mt);
-    if (there && (key > found || (key == found && t < rank))) out[a + min(t, rank)] = i;
+    if (key > found || (key == found && t < rank)) out[a + min(t, rank)] = i;
     n_above += __builtin_popcountll(ma);
     n_tie += __builtin_popcountll(mt);
   });
@@ -260,9 +261,13 @@ hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_s
 #define PQKV_SELECT(K) \
   evict_select_kernel<K><<<(unsigned)n_streams, kSelThreads, 0, s>>>(weights, stride, S, keep, sink, recent, kept)
   if (steps <= 2) PQKV_SELECT(2);
+  else if (steps <= 4) PQKV_SELECT(4);
   else if (steps <= 8) PQKV_SELECT(8);
-  else if (steps <= 16) PQKV_SELECT(16);
+  else if (steps <= 12) PQKV_SELECT(12);
+  else if (steps <= 18) PQKV_SELECT(18);
+  else if (steps <= 24) PQKV_SELECT(24);
   else if (steps <= 32) PQKV_SELECT(32);
+  else if (steps <= 48) PQKV_SELECT(48);
   else if (steps <= 64) PQKV_SELECT(64);
   else PQKV_SELECT(0);
 #undef PQKV_SELECT
