@@ -95,10 +95,11 @@ WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl)
                           (int64_t)(512 << 20) / (streams * rec_row));
   rows = std::max<int64_t>(rows / 64 * 64, 64);
   p.rows = (int)std::min(rows, total);
-  // rows of a workgroup: about 2048 workgroups (four rounds of two per compute
-  // unit); at least 128 rows, under which decoding the keys is most of the work,
-  // at most 2048, whose records (1 MB at d = 128) a group of workgroups shares in L2
-  const int64_t want = p.rows * streams * p.tblocks / 2048;
+  // rows of a workgroup: about 1024 workgroups; at least 128 rows, under which
+  // decoding the keys is most of the work, at most 1024, whose records (0.5 MB at
+  // d = 128) a group of workgroups shares in L2 and which leave the last round
+  // of a long chunk short (2048 rows: 1.48 ms for 32764 rows on 8191 tokens, 1.45)
+  const int64_t want = p.rows * streams * p.tblocks / 1024;
   p.chunk_rows = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, 128), 1024);
   p.q = align256((size_t)B * Hq * Sq * d * 4);
   p.pq = qjl ? p.q : 0;
@@ -167,15 +168,24 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
   float *q32 = (float *)take(p.q), *pq32 = (float *)take(p.pq);
   const int64_t nvec = (int64_t)B * Hq * Sq;
   const float qs = scale * 1.4426950408889634f;
-  int tok = pqkv::prof_begin("weights_rotate", st);
-  hipError_t e = has_qjl ? pqkv::launch_rotate2(q, q_dtype, R, p_rot, q32, pq32, nvec, d, qs, 1.0f / (float)m, st)
-                         : pqkv::launch_rotate(q, q_dtype, R, q32, PQKV_F32, nvec, d, 0, qs, st);
-  pqkv::prof_end(tok, st);
-  if (e != hipSuccess) return report_hip_error(e, "attn_weights query rotation");
+  // the queries are rotated on their way into the rows' records where they can
+  // be read 16 bytes at a time and no projection needs them rotated, else before
+  const bool direct = !has_qjl && (uintptr_t)q % 16 == 0;
+  if (!direct) {
+    const int t = pqkv::prof_begin("weights_rotate", st);
+    const hipError_t r = has_qjl ? pqkv::launch_rotate2(q, q_dtype, R, p_rot, q32, pq32, nvec, d, qs, 1.0f / (float)m, st)
+                                 : pqkv::launch_rotate(q, q_dtype, R, q32, PQKV_F32, nvec, d, 0, qs, st);
+    pqkv::prof_end(t, st);
+    if (r != hipSuccess) return report_hip_error(r, "attn_weights query rotation");
+  }
   pqkv::AttnWeightsArgs a;
   memset(&a, 0, sizeof(a));
-  a.q = q32;
+  a.q = direct ? nullptr : q32;
   a.pq = has_qjl ? pq32 : nullptr;
+  a.x = direct ? q : nullptr;
+  a.x_dtype = q_dtype;
+  a.R = R;
+  a.q_scale = qs;
   a.k_cache = k_cache;
   a.qjl = qjl;
   if (pg) {
@@ -214,8 +224,8 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
     a.chunks = p.chunks(a.rows);
     a.in = row0 ? out : in;
     a.in_stride = row0 ? out_stride : in_stride;
-    tok = pqkv::prof_begin("attn_weights", st);
-    e = pqkv::launch_attn_weights(a, st);
+    const int tok = pqkv::prof_begin("attn_weights", st);
+    const hipError_t e = pqkv::launch_attn_weights(a, st);
     pqkv::prof_end(tok, st);
     if (e != hipSuccess) return report_hip_error(e, "attn_weights launch");
   }

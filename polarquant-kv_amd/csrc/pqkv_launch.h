@@ -383,6 +383,10 @@ hipError_t launch_prefill_merge(const PrefillArgs &a, int stream0, int ns, int r
 // (b, kv head) is query token i of the group's head g.
 struct AttnWeightsArgs {
   const float *q, *pq;           // [B][Hq][Sq][d] fp32, rotated, times scale*log2(e); projections (QJL) or null
+  const void *x;                 // or (q null) the queries as they are, on a 16-byte boundary, in x_dtype,
+  int x_dtype;                   // to be rotated by R and scaled by q_scale
+  const float *R;
+  float q_scale;
   const uint8_t *k_cache;        // [B][Hkv][S_max] vectors, or pages as in DecodeArgs
   const uint8_t *qjl;
   const uint8_t *const *k_pages, *const *s_pages;

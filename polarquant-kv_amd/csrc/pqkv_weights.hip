@@ -168,6 +168,36 @@ __device__ __forceinline__ int scale_exponent(float most, int largest) {
   return ex == 0 || ex == 255 ? 0 : min(135 - ex, largest);
 }
 
+// The address of row r of a pass in a [B][Hq][Sq] arrangement of vectors.
+__device__ __forceinline__ int64_t row_vector(const WeightsKernelArgs &k, int64_t stream, int r) {
+  const AttnWeightsArgs &a = k.a;
+  const int b = (int)(stream / a.Hkv), h = (int)(stream - (int64_t)b * a.Hkv);
+  const uint32_t rr = (uint32_t)(min(r, a.rows - 1) + a.row0), tok = k.group.div(rr);
+  return ((int64_t)b * a.Hq + h * a.G + (int)(rr - tok * a.G)) * a.Sq + tok;
+}
+
+// Eight values of each of a row's parts (queries, projections) -> its share of
+// the record: hi and lo, times 2^sh.
+template <int D, bool QJL>
+__device__ __forceinline__ void put_row(uint8_t *rec, int j, int rl, const float (&x)[QJL ? 2 : 1][8], int sh) {
+  using Rec = RowRec<D, QJL>;
+  const float sc = __builtin_ldexpf(1.0f, sh);
+#pragma unroll
+  for (int p = 0; p < (QJL ? 2 : 1); ++p) {
+    half8_t hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      half_t u, v;
+      split_parts(x[p][i] * sc, &u, &v);
+      hi[i] = u;
+      lo[i] = v;
+    }
+    uint8_t *seg = rec + ((j >> 2) * Rec::PARTS + 2 * p) * 1024 + ((j & 3) * 16 + rl) * 16;
+    *(half8_t *)seg = hi;
+    *(half8_t *)(seg + 1024) = lo;
+  }
+}
+
 // Rotated queries (and projections) -> records of 16 rows, and each row's
 // factor. Rows past the pass's last one are zeros.
 template <int D, bool QJL>
@@ -179,11 +209,9 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
   const uint32_t tiles = (uint32_t)a.row_tiles;
   const int64_t stream = blockIdx.x / tiles;
   const int tile = (int)(blockIdx.x - (uint32_t)stream * tiles), r = tile * 16 + rl;
-  const int b = (int)(stream / a.Hkv), h = (int)(stream - (int64_t)b * a.Hkv);
   float x[QJL ? 2 : 1][8];
   float mx = 0.0f;
-  const uint32_t tok = k.group.div((uint32_t)(min(r, a.rows - 1) + a.row0));
-  const int64_t row = ((int64_t)b * a.Hq + h * a.G + (min(r, a.rows - 1) + a.row0 - (int)tok * a.G)) * a.Sq + tok;
+  const int64_t row = row_vector(k, stream, r);
 #pragma unroll
   for (int p = 0; p < (QJL ? 2 : 1); ++p) {
     const float *src = (p ? a.pq : a.q) + row * D + 8 * j;
@@ -200,21 +228,138 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
   for (int i = 0; i < D / 8; ++i) mx = fmaxf(mx, most[i][rl]);
   const int sh = scale_exponent(mx, 100);
   if (j == 0) a.row_factor[stream * tiles * 16 + r] = __builtin_ldexpf(1.0f, -sh);
-  uint8_t *rec = a.records + (stream * tiles + tile) * Rec::BYTES;
-  const float sc = __builtin_ldexpf(1.0f, sh);
+  put_row<D, QJL>(a.records + (stream * tiles + tile) * Rec::BYTES, j, rl, x, sh);
+}
+
+// The same from the queries themselves (a.x, rows on 16-byte boundaries, no
+// QJL): y = R x on the matrix cores, so that the rotated queries are never
+// written. A = R, split hi / lo once per workgroup into registers (a wave's D /
+// 4 outputs), B = 16 queries as they lie in memory: fp16 queries are their own
+// high part (two products), fp32 ones are scaled and split (three).
+// 32764 x 8 rows (d = 128): 58 us (200 MB, 3.5 TB/s) where rotating first (75)
+// and weights_rows_kernel (48) took 123.
+template <int D, typename T>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_rows_kernel(const WeightsKernelArgs k, uint32_t n_tiles) {
+  using Rec = RowRec<D, false>;
+  constexpr int KS = D / 32, OT = D / 64;          // outputs of a wave: OT tiles of 16
+  constexpr bool F32 = sizeof(T) == 4;
+  __shared__ __align__(16) float ys[2][16][D + 4];
+  __shared__ float most[2][4][16];
+  const AttnWeightsArgs &a = k.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+
+  // the wave's rows of R, scaled by a power of two of its own
+  float4 rv[OT][KS][2];
+  float rm = 0.0f;
 #pragma unroll
-  for (int p = 0; p < (QJL ? 2 : 1); ++p) {
-    half8_t hi, lo;
+  for (int o = 0; o < OT; ++o)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      half_t u, v;
-      split_parts(x[p][i] * sc, &u, &v);
-      hi[i] = u;
-      lo[i] = v;
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        rv[o][ks][p] = *(const float4 *)(a.R + (16 * (OT * wave + o) + col) * D + 32 * ks + 8 * grp + 4 * p);
+        const float4 u = rv[o][ks][p];
+        rm = fmaxf(fmaxf(fmaxf(rm, fabsf(u.x)), fmaxf(fabsf(u.y), fabsf(u.z))), fabsf(u.w));
+      }
+  const int rsh = scale_exponent(wave_max(rm), 100);
+  const float rscale = __builtin_ldexpf(1.0f, rsh), undo = a.q_scale * __builtin_ldexpf(1.0f, -rsh);
+  half8_t rh[OT][KS], rl[OT][KS];
+#pragma unroll
+  for (int o = 0; o < OT; ++o)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const float4 u = rv[o][ks][0], v = rv[o][ks][1];
+      const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        half_t p, q;
+        split_parts(e[i] * rscale, &p, &q);
+        rh[o][ks][i] = p;
+        rl[o][ks][i] = q;
+      }
     }
-    uint8_t *seg = rec + ((j >> 2) * Rec::PARTS + 2 * p) * 1024 + ((j & 3) * 16 + rl) * 16;
-    *(half8_t *)seg = hi;
-    *(half8_t *)(seg + 1024) = lo;
+
+  struct Operand {
+    half8_t h[KS], l[F32 ? KS : 1];
+    float undo;
+  };
+  const uint32_t tiles = (uint32_t)a.row_tiles;
+  auto load = [&](uint32_t n) {
+    Operand o;
+    const int64_t stream = n / tiles;
+    const int r = (int)(n - (uint32_t)stream * tiles) * 16 + col;
+    const T *src = (const T *)a.x + row_vector(k, stream, r) * D + 8 * grp;
+    o.undo = r < a.rows ? undo : 0.0f;             // rows past the last one: zeros
+    if constexpr (F32) {
+      float4 u[KS][2];
+      float mx = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          u[ks][p] = *(const float4 *)(src + 32 * ks + 4 * p);
+          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(u[ks][p].x)), fmaxf(fabsf(u[ks][p].y), fabsf(u[ks][p].z))), fabsf(u[ks][p].w));
+        }
+      const int sh = scale_exponent(rows4_max(mx), 100);
+      const float sc = __builtin_ldexpf(1.0f, sh);
+      o.undo *= __builtin_ldexpf(1.0f, -sh);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float e[8] = {u[ks][0].x, u[ks][0].y, u[ks][0].z, u[ks][0].w, u[ks][1].x, u[ks][1].y, u[ks][1].z, u[ks][1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          half_t p, q;
+          split_parts(e[i] * sc, &p, &q);
+          o.h[ks][i] = p;
+          o.l[ks][i] = q;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) o.h[ks] = *(const half8_t *)(src + 32 * ks);
+    }
+    return o;
+  };
+  uint32_t n = blockIdx.x;
+  int buf = 0;
+  Operand x = load(n);
+  for (; n < n_tiles; n += gridDim.x, buf ^= 1) {
+    const Operand now = x;
+    if (n + gridDim.x < n_tiles) x = load(n + gridDim.x);
+    float4_t acc[OT];
+#pragma unroll
+    for (int o = 0; o < OT; ++o) acc[o] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl[o][ks], now.h[ks], acc[o], 0, 0, 0);
+        if constexpr (F32) acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[o][ks], now.l[ks], acc[o], 0, 0, 0);
+        acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh[o][ks], now.h[ks], acc[o], 0, 0, 0);
+      }
+    // through LDS into the record's order (two buffers: one barrier a tile),
+    // the row's largest value beside it
+    float mx = 0.0f;
+#pragma unroll
+    for (int o = 0; o < OT; ++o) {
+      const float4_t y = now.undo == 0.0f ? (float4_t){0.f, 0.f, 0.f, 0.f} : acc[o] * now.undo;
+      *(float4_t *)&ys[buf][col][16 * (OT * wave + o) + 4 * grp] = y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fabsf(y[i]));
+    }
+    mx = rows4_max(mx);
+    if (grp == 0) most[buf][wave][col] = mx;
+    __syncthreads();
+    const int rr = tid & 15, j = tid >> 4;
+    if (j < D / 8) {
+      float y[1][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[0][i] = ys[buf][rr][8 * j + i];
+      mx = fmaxf(fmaxf(most[buf][0][rr], most[buf][1][rr]), fmaxf(most[buf][2][rr], most[buf][3][rr]));
+      const int sh = scale_exponent(mx, 100);
+      if (j == 0) a.row_factor[(int64_t)n * 16 + rr] = __builtin_ldexpf(1.0f, -sh);
+      put_row<D, false>(a.records + (int64_t)n * Rec::BYTES, j, rr, y, sh);
+    }
   }
 }
 
@@ -574,7 +719,14 @@ void launch_passes(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
   const int64_t groups = streams * a.chunks;
   if (groups % 8 == 0 || groups >= 64) k.xcd_groups = (int)groups;
   const unsigned grid = (unsigned)((k.xcd_groups ? (groups + 7) / 8 * 8 : groups) * a.tblocks);
-  weights_rows_kernel<D, QJL><<<(unsigned)(streams * a.row_tiles), 2 * D, 0, s>>>(k);
+  const uint32_t tiles = (uint32_t)(streams * a.row_tiles);
+  if (!QJL && a.x != nullptr) {
+    const unsigned blocks = tiles < 1024 ? tiles : 1024;   // (each reads R once)
+    if (a.x_dtype == PQKV_F16) weights_rotate_rows_kernel<D, half_t><<<blocks, 256, 0, s>>>(k, tiles);
+    else weights_rotate_rows_kernel<D, float><<<blocks, 256, 0, s>>>(k, tiles);
+  } else {
+    weights_rows_kernel<D, QJL><<<tiles, 2 * D, 0, s>>>(k);
+  }
   attn_weights_kernel<D, QJL, TT, true><<<grid, 64 * kWW, 0, s>>>(k);
   attn_stats_kernel<<<(unsigned)(streams * (a.row_tiles / 2)), 256, 0, s>>>(k);
   attn_weights_kernel<D, QJL, TT, false><<<grid, 64 * kWW, 0, s>>>(k);

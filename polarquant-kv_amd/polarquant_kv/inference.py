@@ -28,7 +28,12 @@ Differences, all on purpose:
     <= p0 + i): the compressed cache, the uncompressed cache and no cache.
     The reference calls non-causal SDPA / compressed attention on all three
     (inference/attention.py:63-92), so a chunk's queries see its later
-    tokens; causal=False reproduces that.
+    tokens; causal=False reproduces that;
+  - a manager can keep how much attention weight each cached position has
+    got (track_weights) and cut its caches to the heaviest ones (evict), so a
+    sequence may grow past max_seq_len cached positions;
+  - the attention layer can turn its queries and keys by their positions
+    (rotary), which the manager counts apart from the slots of its caches.
 All GPU work goes through libpqkv_hip.so.
 """
 
@@ -56,16 +61,20 @@ class KVCacheManager:
     """Compressed KV cache of one attention layer: up to max_seq_len
     positions per (batch, head), kept in pages of page_tokens positions
     (a power of two, >= 64), filled by prefill (several tokens) and decode
-    (one token) appends."""
+    (one token) appends. With track_weights, attend() also adds up the
+    softmax weight that each cached position gets, for evict()."""
 
     def __init__(self, config: PolarQuantConfig, max_seq_len: int, batch: int, num_heads: int, head_dim: int,
-                 device: str = "cuda", rotation_seed: int = 42, page_tokens: int = 256):
+                 device: str = "cuda", rotation_seed: int = 42, page_tokens: int = 256, track_weights: bool = False):
         from .rotation import generate_rotation_matrix
         if config.enable_compression:
             quantizer._validate_params(config.n_bits, config.group_size, head_dim)
             if config.n_bits not in (2, 4):
                 raise ValueError(f"the codebook format stores 2- or 4-bit codes, got n_bits={config.n_bits}")
+        elif track_weights:
+            raise ValueError("weights are kept for compressed caches")
         self.config = config
+        self.track_weights = track_weights
         self.page_tokens = int(page_tokens)
         self.max_seq_len = int(max_seq_len)
         self.batch = batch
@@ -86,6 +95,10 @@ class KVCacheManager:
         self._key_cache: torch.Tensor | None = None
         self._value_cache: torch.Tensor | None = None
         self._seq_len = 0
+        self._next_position = 0
+        # with track_weights: [batch, num_heads, room] of every slot, room >= seq_len
+        self._weights: torch.Tensor | None = None
+        self._positions: torch.Tensor | None = None
 
     # ---- allocation ----
     def _allocate(self):
@@ -104,6 +117,24 @@ class KVCacheManager:
         return self._seq_len
 
     @property
+    def next_position(self) -> int:
+        """Position of the next appended token: how many were appended since
+        the last reset, those evicted since among them."""
+        return self._next_position
+
+    @property
+    def weights(self) -> torch.Tensor | None:
+        """[batch, num_heads, seq_len] float32: the attention weight each cached
+        position has got (track_weights)."""
+        return None if self._weights is None else self._weights[:, :, :self._seq_len]
+
+    @property
+    def positions(self) -> torch.Tensor | None:
+        """[batch, num_heads, seq_len] int32: where the token of each slot
+        stood in its sequence (track_weights)."""
+        return None if self._positions is None else self._positions[:, :, :self._seq_len]
+
+    @property
     def memory_bytes(self) -> int:
         """Bytes of the cached positions (K + V, and the QJL signs)."""
         if self._seq_len == 0:
@@ -119,10 +150,13 @@ class KVCacheManager:
 
     @property
     def allocated_bytes(self) -> int:
-        """Device bytes held: the pages allocated so far (and their tables);
-        uncompressed, the max_seq_len-position arrays."""
+        """Device bytes held: the pages allocated so far (and their tables,
+        weights and positions); uncompressed, the max_seq_len-position arrays."""
         if self.config.enable_compression:
-            return 0 if self._keys is None else self._keys.memory_bytes() + self._values.memory_bytes()
+            if self._keys is None:
+                return 0
+            tracked = 0 if self._weights is None else 8 * self._weights.numel()
+            return self._keys.memory_bytes() + self._values.memory_bytes() + tracked
         return 0 if self._key_cache is None else 2 * self._key_cache.numel() * 2
 
     @property
@@ -153,7 +187,27 @@ class KVCacheManager:
         else:
             self._key_cache[:, :, self._seq_len:self._seq_len + T] = key.to(torch.float16)
             self._value_cache[:, :, self._seq_len:self._seq_len + T] = value.to(torch.float16)
+        if self.track_weights:
+            self._track(T)
         self._seq_len += T
+        self._next_position += T
+
+    def _track(self, T: int) -> None:
+        """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions."""
+        S, need = self._seq_len, self._seq_len + T
+        room = 0 if self._weights is None else self._weights.shape[2]
+        if need > room:
+            room = min(max(need, 2 * room, self.page_tokens), self.max_seq_len)
+            shape = (self.batch, self.num_heads, room)
+            w = torch.zeros(shape, dtype=torch.float32, device=self.device)
+            p = torch.zeros(shape, dtype=torch.int32, device=self.device)
+            if S:
+                w[:, :, :S], p[:, :, :S] = self._weights[:, :, :S], self._positions[:, :, :S]
+            self._weights, self._positions = w, p
+        else:
+            self._weights[:, :, S:need] = 0.0
+        self._positions[:, :, S:need] = torch.arange(self._next_position, self._next_position + T, dtype=torch.int32,
+                                                     device=self.device)
 
     def get_kv(self):
         """Compressed: the two PagedPQCache objects (seq_len positions valid);
@@ -167,16 +221,36 @@ class KVCacheManager:
     def reset(self) -> None:
         """Forget the cached positions (the pages are kept for reuse)."""
         self._seq_len = 0
+        self._next_position = 0
         for c in (self._keys, self._values):
             if c is not None:
                 c.seq_len = 0
+
+    def evict(self, keep: int, sink: int = 4, recent: int = 64):
+        """Cut the caches to `keep` positions per (batch, head): the first
+        `sink`, the last `recent` and those with the most attention weight so
+        far, in their order (eviction.evict; needs track_weights). Nothing is
+        done when no more than that are cached. Returns the Eviction, or None."""
+        if not self.track_weights:
+            raise ValueError("evict() needs track_weights")
+        if keep < 1 or keep < sink + recent:
+            raise ValueError(f"keep={keep} must be at least 1 and sink + recent = {sink + recent}")
+        if self._seq_len <= keep:
+            return None
+        from . import eviction
+        r = eviction.evict(self._keys, self._values, self._weights, keep, sink=sink, recent=recent,
+                           positions=self._positions)
+        self._keys, self._values, self._weights, self._positions = r.keys, r.values, r.weights, r.positions
+        self._seq_len = keep
+        return r
 
     # ---- reads ----
     def attend(self, query: torch.Tensor, causal: bool = True) -> torch.Tensor:
         """query [batch, q_heads, Sq, head_dim] for the last Sq cached
         positions -> [batch, q_heads, Sq, head_dim] fp16: compressed
         attention (decode for Sq = 1, causal prefill otherwise) with the QJL
-        term when the manager keeps signs."""
+        term when the manager keeps signs. With track_weights the queries'
+        weights are added to those of the cached positions."""
         if self._seq_len == 0:
             return torch.zeros_like(query, dtype=torch.float16)
         if not self.config.enable_compression:
@@ -192,24 +266,41 @@ class KVCacheManager:
                 s = s.masked_fill(pos[None, :] > qpos[:, None], float("-inf"))
             return torch.matmul(torch.softmax(s, -1), v).half()
         Sq = query.shape[2]
+        start = self._seq_len - Sq
+        if self.track_weights:
+            w = self._weights
+            if Sq == 1:
+                out, _ = attention.decode_attention_weights(query[:, :, 0], self._keys, self._values, self.R,
+                                                            jl_rot=self.jl_rot, out_dtype=torch.float16, previous=w,
+                                                            into=w)
+                return out.unsqueeze(2)
+            attention.attention_weights(query, self._keys, self.R, start, causal=causal, jl_rot=self.jl_rot,
+                                        previous=w, into=w)
+            return attention.prefill_attention(query, self._keys, self._values, self.R, start, causal=causal,
+                                               out_dtype=torch.float16, jl_rot=self.jl_rot)
         jl = self.jl_matrix if self.jl_rot is not None else None
         return attention.compressed_attention_gpu(query, self._keys, self._values, self.R, jl_matrix=jl,
-                                                  causal=causal, q_start=self._seq_len - Sq)
+                                                  causal=causal, q_start=start)
 
 
 class CompressedMultiHeadAttention(torch.nn.Module):
     """Multi-head (GQA) attention whose KV cache is the compressed one
-    (src/polarquant_kv_cuda/inference/attention.py:12-95)."""
+    (src/polarquant_kv_cuda/inference/attention.py:12-95). rotary
+    (rotary.RotaryEmbedding of the head's size): queries and keys turned by
+    their positions before the keys are cached."""
 
     def __init__(self, config: PolarQuantConfig, embed_dim: int, num_heads: int, num_kv_heads: int | None = None,
-                 causal: bool = True):
+                 causal: bool = True, rotary=None):
         super().__init__()
         self.config = config
+        self.rotary = rotary
         self.causal = causal
         self.embed_dim = embed_dim
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads or num_heads
         self.head_dim = embed_dim // num_heads
+        if rotary is not None and rotary.head_dim != self.head_dim:
+            raise ValueError(f"rotary head_dim {rotary.head_dim}, the layer's {self.head_dim}")
         self.q_proj = torch.nn.Linear(embed_dim, num_heads * self.head_dim, bias=False)
         self.k_proj = torch.nn.Linear(embed_dim, self.num_kv_heads * self.head_dim, bias=False)
         self.v_proj = torch.nn.Linear(embed_dim, self.num_kv_heads * self.head_dim, bias=False)
@@ -223,6 +314,9 @@ class CompressedMultiHeadAttention(torch.nn.Module):
         q = self.q_proj(x).reshape(B, T, self.num_heads, self.head_dim).transpose(1, 2).half()
         k = self.k_proj(x).reshape(B, T, self.num_kv_heads, self.head_dim).transpose(1, 2).half()
         v = self.v_proj(x).reshape(B, T, self.num_kv_heads, self.head_dim).transpose(1, 2).half()
+        if self.rotary is not None:
+            start = 0 if cache_manager is None else cache_manager.next_position
+            q, k = self.rotary(q, k, torch.arange(start, start + T, device=x.device))
         if cache_manager is not None:
             cache_manager.append(k.contiguous(), v.contiguous())
             out = cache_manager.attend(q.contiguous(), causal=self.causal)
