@@ -434,14 +434,17 @@ int pqkv_evict_select(const float *weights, int64_t weights_stride, int64_t n_st
  * A row is row_bytes[a] bytes (a multiple of 4). An array is contiguous (rows
  * of stream s from base + s * stride bytes on) or, with `pages`, paged as the
  * caches above (row t in the page pages[s * max_pages + t / page_tokens];
- * base and stride unused). Paged results also get zeros in rows keep ..
- * fill - 1 (fill >= keep; contiguous results end at keep). A kept position
- * outside 0 .. S - 1 gives a row of zeros. Bases, strides and pages are 4-byte
- * aligned (pages 16-byte, as everywhere). dst must not overlap src. */
+ * base and stride unused). A paged result whose base is set lies in one piece,
+ * page p of stream s at base + s * stride + p * page_tokens * row_bytes, and its
+ * table (entries 0 .. ceil(fill / page_tokens) - 1 of every stream) is written by
+ * the call. Paged results also get zeros in rows keep .. fill - 1 (fill >= keep;
+ * contiguous results end at keep). A kept position outside 0 .. S - 1 gives a row
+ * of zeros. Bases, strides and pages are 4-byte aligned (pages 16-byte, as
+ * everywhere). dst must not overlap src. */
 #define PQKV_MAX_GATHER 6
 typedef struct pqkv_row_array {
     const void *base;
-    const uint8_t *const *pages;
+    const uint8_t *const *pages;   /* written where a paged result has a base */
     int64_t stride;
     int page_tokens, max_pages;
 } pqkv_row_array;

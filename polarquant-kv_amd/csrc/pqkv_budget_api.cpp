@@ -343,21 +343,27 @@ int pqkv_gather_rows(int n_arrays, const pqkv_row_array *src, const pqkv_row_arr
         if (shift < 0) return shift;
         (is_src ? p.src_shift : p.dst_shift) = shift;
         (is_src ? p.src_max_pages : p.dst_max_pages) = r->max_pages;
-      } else {
-        if (!r->base && rows > 0) return fail_status(PQKV_ERR_INVALID, "gather_rows: null array %d", i);
-        if (((uintptr_t)r->base | (uintptr_t)r->stride) % 4)
-          return fail_status(PQKV_ERR_INVALID, "gather_rows: array %d is not 4-byte aligned", i);
-        if (r->stride < (is_src ? S : (int64_t)keep) * rb)
-          return fail_status(PQKV_ERR_INVALID, "gather_rows: array %d: stride %lld below its rows", i,
-                             (long long)r->stride);
-        align |= (uintptr_t)r->base | (uintptr_t)r->stride;
+        if (is_src || !r->base) continue;
+        if ((uintptr_t)r->base % 16 || r->stride % 16 || ((int64_t)r->page_tokens * rb) % 16)
+          return fail_status(PQKV_ERR_INVALID, "gather_rows: pages of array %d are not 16-byte aligned", i);
+      } else if (!r->base && rows > 0) {
+        return fail_status(PQKV_ERR_INVALID, "gather_rows: null array %d", i);
       }
+      if (((uintptr_t)r->base | (uintptr_t)r->stride) % 4)
+        return fail_status(PQKV_ERR_INVALID, "gather_rows: array %d is not 4-byte aligned", i);
+      const int64_t held = is_src ? S : r->pages ? (rows + r->page_tokens - 1) / r->page_tokens * r->page_tokens : keep;
+      if (r->stride < held * rb)
+        return fail_status(PQKV_ERR_INVALID, "gather_rows: array %d: stride %lld below its rows", i,
+                           (long long)r->stride);
+      align |= (uintptr_t)r->base | (uintptr_t)r->stride;
     }
+    const bool table = dst[i].pages && dst[i].base;
     p.src = (const uint8_t *)src[i].base;
     p.src_pages = src[i].pages;
     p.src_stride = src[i].stride;
     p.dst = (uint8_t *)const_cast<void *>(dst[i].base);
-    p.dst_pages = (uint8_t *const *)dst[i].pages;
+    p.dst_pages = table ? nullptr : (uint8_t *const *)dst[i].pages;
+    p.dst_table = table ? (uint8_t **)dst[i].pages : nullptr;
     p.dst_stride = dst[i].stride;
     p.row_bytes = rb;
     p.unit = align % 8 == 0 ? 8 : 4;

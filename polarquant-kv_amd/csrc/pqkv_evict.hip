@@ -241,7 +241,13 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const GatherKernelArgs
   const int row0 = (int)(blockIdx.x - (uint32_t)stream * tiles) * k.rows_per;
   const GatherPart &p = a.part[blockIdx.y];
   // contiguous results end at keep; pages are filled up with zeros
-  const int rows = min(k.rows_per, (p.dst_pages ? a.fill : a.keep) - row0);
+  const int rows = min(k.rows_per, (p.dst_pages || p.dst_table ? a.fill : a.keep) - row0);
+  if (p.dst_table) {   // the pages that start in these rows
+    const int page = 1 << p.dst_shift, first = (row0 + page - 1) >> p.dst_shift;
+    const int pg = first + (int)threadIdx.x;
+    if ((pg << p.dst_shift) < row0 + rows)
+      p.dst_table[stream * p.dst_max_pages + pg] = p.dst + stream * p.dst_stride + (int64_t)pg * page * p.row_bytes;
+  }
   if ((int)threadIdx.x < rows) {
     const int o = row0 + (int)threadIdx.x;
     const int t = o < a.keep ? a.kept[stream * a.keep + o] : -1;

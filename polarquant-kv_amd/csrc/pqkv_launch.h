@@ -433,7 +433,8 @@ struct GatherPart {
   const uint8_t *src;
   const uint8_t *const *src_pages;   // or null: contiguous
   uint8_t *dst;
-  uint8_t *const *dst_pages;
+  uint8_t *const *dst_pages;         // pages to follow, or null: rows lie from dst on
+  uint8_t **dst_table;               // or null: the table of those rows' pages, to be written
   int64_t src_stride, dst_stride;    // bytes between streams
   int src_shift, src_max_pages, dst_shift, dst_max_pages;
   int row_bytes, unit;

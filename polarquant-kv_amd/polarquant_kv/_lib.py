@@ -214,6 +214,14 @@ def require_device(*tensors) -> None:
             raise ValueError("GPU entry points take device tensors (the hot path has no CPU fallback)")
 
 
+def dense_f32(t):
+    """t (or None) as contiguous float32: itself where it is that already."""
+    import torch
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 def require_one_device(*tensors) -> None:
     """The tensors a call reads and writes are on one device."""
     where = [t.device for t in tensors if t is not None]

@@ -48,7 +48,10 @@ def check_shapes(B: int, Hq: int, d: int, keys: PQCache, values: PQCache, rotati
     if rotation_matrix is not None and tuple(rotation_matrix.shape) != (d, d):
         raise ValueError(f"rotation matrix must be ({d}, {d}), got {tuple(rotation_matrix.shape)}")
     for name, c in (("keys", keys), ("values", values)):
-        per_batch = (sum(c.max_seq_len * vector_bytes(d, b) for b in c.head_bits()))
+        if c.mixed:
+            per_batch = sum(c.max_seq_len * vector_bytes(d, b) for b in c.head_bits())
+        else:
+            per_batch = Hkv * c.max_seq_len * vector_bytes(d, c.n_bits)
         if c.blocks.numel() < B * per_batch:
             raise ValueError(f"{name}: {c.blocks.numel()} cache bytes, the shape needs {B * per_batch}")
     if keys.qjl_signs is not None and keys.qjl_signs.numel() < B * Hkv * keys.max_seq_len * (d // 8):
@@ -194,9 +197,8 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
     out_dtype = query.dtype if out_dtype is None else out_dtype
     S = keys.seq_len
     previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
-    q = query.contiguous()
-    R = rotation_matrix.to(torch.float32).contiguous()
-    P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    q = query if query.is_contiguous() else query.contiguous()
+    R, P = _lib.dense_f32(rotation_matrix), _lib.dense_f32(jl_rot)
     out = torch.empty(B, Hq, d, dtype=out_dtype, device=q.device)
     lib = _lib.lib()
     ws = torch.empty(lib.pqkv_decode_attn_weights_workspace_bytes(B, Hq, Hkv, max(S, 1), d), dtype=torch.uint8,
@@ -243,9 +245,8 @@ def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, 
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     S = keys.seq_len
     previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
-    q = query.contiguous()
-    R = rotation_matrix.to(torch.float32).contiguous()
-    P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    q = query if query.is_contiguous() else query.contiguous()
+    R, P = _lib.dense_f32(rotation_matrix), _lib.dense_f32(jl_rot)
     lib = _lib.lib()
     ws = torch.empty(max(1, lib.pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d, int(P is not None))), dtype=torch.uint8,
                      device=q.device)

@@ -29,6 +29,8 @@ def _check_budget(S: int, keep: int, sink: int, recent: int) -> None:
 
 def _check_rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """t with rows [B, H] one stride apart and dense."""
+    if t.is_contiguous():
+        return t
     B, H, S = t.shape
     dense = t.stride(2) == 1 or S <= 1
     if not dense or (B > 1 and H > 1 and t.stride(0) != H * t.stride(1)) or _row_stride(t) < S:
@@ -39,9 +41,9 @@ def _check_rows(t: torch.Tensor, name: str) -> torch.Tensor:
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between consecutive (batch, head) rows of a [B, H, S] tensor."""
     B, H, S = t.shape
-    if H > 1:
-        return t.stride(1)
-    return t.stride(0) if B > 1 else max(S, 1)
+    if t.is_contiguous() or B * H <= 1:
+        return max(S, 1)
+    return t.stride(1) if H > 1 else t.stride(0)
 
 
 def select_positions(weights: torch.Tensor, keep: int, sink: int = 0, recent: int = 0) -> torch.Tensor:
@@ -80,18 +82,26 @@ def _cache_arrays(cache):
 
 def _empty_like(cache, positions: int, room: int):
     """A cache of the same kind for `positions` positions (a contiguous one of
-    `room` positions), its rows not yet written."""
+    `room` positions) whose rows (and, paged, tables) are not yet written, and
+    its arrays as _cache_arrays gives them."""
     B, H, d = cache.batch, cache.num_heads, cache.head_dim
     if isinstance(cache, PagedPQCache):
-        return PagedPQCache(B, H, d, cache.n_bits, cache.codebooks, cache.device, page_tokens=cache.page_tokens,
-                            jl_dim=cache.jl_dim, max_pages=1, reserve=positions)
+        if positions == 0:
+            return PagedPQCache(B, H, d, cache.n_bits, cache.codebooks, cache.device, cache.page_tokens,
+                                cache.jl_dim, 1), ()
+        new = PagedPQCache(B, H, d, cache.n_bits, cache.codebooks, cache.device, cache.page_tokens, cache.jl_dim,
+                           tables=False)
+        P, n = cache.page_tokens, -(-positions // cache.page_tokens)
+        return new, [((pool.data_ptr(), table.data_ptr(), n * P * pool.shape[-1], P, n), pool.shape[-1])
+                     for pool, table in zip(new.reserve(positions), (new.table, new.sign_table))]
     fresh = torch.empty if room == positions else torch.zeros
     device, signs = cache.blocks.device, None
     if cache.qjl_signs is not None:
         signs = fresh(B, H, room, cache.qjl_signs.shape[-1], dtype=torch.uint8, device=device)
-    return PQCache(blocks=fresh(B, H, room, vector_bytes(d, cache.n_bits), dtype=torch.uint8, device=device),
-                   head_dim=d, n_bits=cache.n_bits, seq_len=0, max_seq_len=room, codebooks=cache.codebooks,
-                   qjl_signs=signs, jl_dim=cache.jl_dim)
+    new = PQCache(blocks=fresh(B, H, room, vector_bytes(d, cache.n_bits), dtype=torch.uint8, device=device),
+                  head_dim=d, n_bits=cache.n_bits, seq_len=0, max_seq_len=room, codebooks=cache.codebooks,
+                  qjl_signs=signs, jl_dim=cache.jl_dim)
+    return new, _cache_arrays(new)
 
 
 def _check_cache(cache, name: str, B: int, H: int, device) -> None:
@@ -129,7 +139,7 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
         raise ValueError(f"kept must be [B, H, keep] int32, got {tuple(kept.shape)} {kept.dtype}")
     _lib.require_device(kept, *rows)
     _lib.require_one_device(kept, *rows)
-    kept = kept.contiguous()
+    kept = kept if kept.is_contiguous() else kept.contiguous()
     B, H, keep = kept.shape
     room = keep if room is None else int(room)
     if room < keep:
@@ -143,16 +153,19 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
             raise ValueError(f"cache {i} holds {c.seq_len} positions, the first one {S}")
     src, dst, sizes, new_rows = [], [], [], []
     with _lib.on_device(kept):
-        new = [_empty_like(c, keep, room) for c in caches]
-        capacity = {c.capacity for c in new if isinstance(c, PagedPQCache)}
-        if len(capacity) > 1:
-            raise ValueError("paged caches in one move must share page_tokens")
-        for old, c in zip(caches, new):
-            for (a, size), (n, _) in zip(_cache_arrays(old), _cache_arrays(c)):
+        new, fill = [], keep
+        for old in caches:
+            c, arrays = _empty_like(old, keep, room)
+            if isinstance(c, PagedPQCache):
+                if fill not in (keep, c.capacity):
+                    raise ValueError("paged caches in one move must share page_tokens")
+                fill = c.capacity
+            for (a, size), (n, _) in zip(_cache_arrays(old), arrays):
                 src.append(a)
                 dst.append(n)
                 sizes.append(size)
             c.seq_len = keep
+            new.append(c)
         held = []                      # copies that the launch reads
         for t in rows:
             if t.dim() != 3 or t.element_size() != 4 or t.shape[:2] != (B, H) or t.shape[2] < S:
@@ -169,7 +182,7 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
         if keep > 0:
             arrays = _lib.RowArray * len(src)
             _lib.check(_lib.lib().pqkv_gather_rows(len(src), arrays(*src), arrays(*dst), _lib.int_array(sizes),
-                                                   kept.data_ptr(), B * H, S, keep, max(capacity, default=keep),
+                                                   kept.data_ptr(), B * H, S, keep, fill,
                                                    _lib.stream_of(kept)))
     return new, new_rows
 

@@ -14,6 +14,7 @@ differ.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -96,8 +97,13 @@ def _code(t: torch.Tensor) -> int:
     return _lib.dtype_code(t.dtype)
 
 
+@functools.lru_cache(maxsize=256)
+def _int64_3(a: int, b: int, c: int):
+    return (_lib.c_int64 * 3)(a, b, c)
+
+
 def _strides(x: torch.Tensor):
-    return (_lib.c_int64 * 3)(x.stride(0), x.stride(1), x.stride(2))
+    return _int64_3(*x.stride()[:3])       # (read-only to the call)
 
 
 def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):

@@ -85,7 +85,7 @@ class PagedPQCache:
     QJL sign pages beside their block pages (same page index)."""
 
     def __init__(self, batch: int, num_heads: int, head_dim: int, n_bits: int, codebooks, device,
-                 page_tokens: int = 256, jl_dim: int = 0, max_pages: int = 16, reserve: int = 0):
+                 page_tokens: int = 256, jl_dim: int = 0, max_pages: int = 16, tables: bool = True):
         import torch
         if page_tokens < 64 or page_tokens > 65536 or page_tokens & (page_tokens - 1):
             raise ValueError(f"page_tokens must be a power of two in 64..65536, got {page_tokens}")
@@ -97,10 +97,9 @@ class PagedPQCache:
         self.groups: list = []        # page group p: uint8 [B, H, page_tokens, vector_bytes]
         self.sign_groups: list = []   # with jl_dim: uint8 [B, H, page_tokens, jl_dim / 8]
         self._adopted = None          # (capacity, storage) of caller-managed pages
-        if reserve > 0:
-            self.reserve(reserve)
-            return
         self.max_pages = max(1, int(max_pages))
+        if not tables:                # reserve() follows and makes them
+            return
         n = batch * num_heads
         self.table = torch.zeros(n, self.max_pages, dtype=torch.int64, device=self.device)
         self.sign_table = torch.zeros_like(self.table) if jl_dim else None
@@ -186,32 +185,31 @@ class PagedPQCache:
                 self.sign_groups.append(sg)
                 self.sign_table[:, p] = sg.data_ptr() + streams * (P * (self.jl_dim // 8))
 
-    def reserve(self, positions: int) -> None:
+    def reserve(self, positions: int) -> list:
         """The pages of a cache that has none yet, for `positions` positions, in
-        one allocation whose bytes are not set: for a writer that fills every
-        page to its end."""
+        one allocation per table. Neither their bytes nor the tables are set:
+        for a writer that fills every page to its end and the tables
+        (pqkv_gather_rows). Page p of stream s is number s * n + p of its
+        allocation. Returns the allocations [B, H, n, page_tokens, row bytes]:
+        of the blocks and, with jl_dim, of the signs."""
         import torch
         if self._adopted is not None or self.groups:
             raise ValueError("reserve() is for a cache without pages")
         n = -(-int(positions) // self.page_tokens)
         if n == 0:
-            return
-        self.sign_table = None
-        B, H, P = self.batch, self.num_heads, self.page_tokens
-
-        def pages(row_bytes):
-            # page p of stream s is number s * n + p, so that the table is one
-            # ascending row of addresses
-            size = P * row_bytes
-            g = torch.empty(B, H, n, P, row_bytes, dtype=torch.uint8, device=self.device)
-            at = torch.arange(g.data_ptr(), g.data_ptr() + B * H * n * size, size, dtype=torch.int64,
-                              device=self.device)
-            return list(g.unbind(2)), at.view(B * H, n)
-
-        self.groups, self.table = pages(self.vector_bytes)
-        if self.jl_dim:
-            self.sign_groups, self.sign_table = pages(self.jl_dim // 8)
-        self.max_pages = n
+            return []
+        B, H = self.batch, self.num_heads
+        tables = torch.empty(2 if self.jl_dim else 1, B * H, n, dtype=torch.int64, device=self.device)
+        self.table, self.max_pages = tables[0], n
+        blocks = torch.empty(B, H, n, self.page_tokens, self.vector_bytes, dtype=torch.uint8, device=self.device)
+        self.groups = list(blocks.unbind(2))
+        if not self.jl_dim:
+            self.sign_table = None
+            return [blocks]
+        self.sign_table = tables[1]
+        signs = torch.empty(B, H, n, self.page_tokens, self.jl_dim // 8, dtype=torch.uint8, device=self.device)
+        self.sign_groups = list(signs.unbind(2))
+        return [blocks, signs]
 
     def memory_bytes(self) -> int:
         """Device bytes of the allocated pages (and the page tables)."""

@@ -114,7 +114,9 @@ def test_gather_refusals():
                        (dict(src=R(FAKE, None, 7196, 0, 0)), INV), (dict(dst=R(FAKE, None, 3596, 0, 0)), INV),
                        (dict(src=R(FAKE + 2, None, 7200, 0, 0)), INV), (dict(src=R(None, None, 7200, 0, 0)), INV),
                        (dict(src=R(None, FAKE, 0, 64, 1)), INV),     # 100 positions, one page of 64
-                       (dict(dst=R(None, FAKE, 0, 64, 1), fill=65), INV), (dict(n=7), INV), (dict(n=-1), INV),
+                       (dict(dst=R(None, FAKE, 0, 64, 1), fill=65), INV),
+                       (dict(dst=R(FAKE, FAKE, 4604, 64, 1)), INV), (dict(dst=R(FAKE + 8, FAKE, 4608, 64, 1)), INV),
+                       (dict(dst=R(FAKE, FAKE, 4608 - 16, 64, 1)), INV), (dict(n=7), INV), (dict(n=-1), INV),
                        (dict(streams=-1), INV), (dict(S=-1), INV), (dict(streams=1 << 40), UNS)):
         _status(call(**kw), expect)
     assert call(n=0) == 0 and call(streams=0) == 0 and call(keep=0, fill=0) == 0
@@ -192,19 +194,21 @@ def test_row_strides():
 
 
 def test_reserved_pages():
-    c = PagedPQCache(2, 3, 64, 2, torch.zeros(16), "cpu", page_tokens=64, jl_dim=64, max_pages=1)
-    c.reserve(200)
+    c = PagedPQCache(2, 3, 64, 2, torch.zeros(16), "cpu", page_tokens=64, jl_dim=64, tables=False)
+    pools = c.reserve(200)
     assert len(c.groups) == len(c.sign_groups) == 4 and c.capacity == 256 and c.max_pages == 4
-    for groups, table in ((c.groups, c.table), (c.sign_groups, c.sign_table)):
-        for p, g in enumerate(groups):
-            assert [g[b, h].data_ptr() for b in range(2) for h in range(3)] == table[:, p].tolist()
+    for pool, groups, table, n in zip(pools, (c.groups, c.sign_groups), (c.table, c.sign_table), (20, 8)):
+        assert pool.shape == (2, 3, 4, 64, n) and table.shape == (6, 4) and table.is_contiguous()
+        assert all(g.data_ptr() == pool[0, 0, p].data_ptr() and g.shape == (2, 3, 64, n) for p, g in enumerate(groups))
+        # as the writer of the pages writes it
+        table.copy_(torch.arange(24).view(6, 4) * (64 * n) + pool.data_ptr())
     with pytest.raises(ValueError):
         c.reserve(10)
+    before = c.table.clone(), c.sign_table.clone()
     c.ensure(257)                                             # grows on by page groups
-    assert len(c.groups) == 5
+    assert len(c.groups) == 5 and torch.equal(c.table[:, :4], before[0]) and torch.equal(c.sign_table[:, :4], before[1])
     e = PagedPQCache(1, 1, 64, 4, torch.zeros(16), "cpu", page_tokens=64)
-    e.reserve(0)
-    assert e.capacity == 0
+    assert e.reserve(0) == [] and e.capacity == 0
 
 
 def test_frequencies_plain_and_linear():
