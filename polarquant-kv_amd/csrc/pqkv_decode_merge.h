@@ -15,17 +15,18 @@ namespace pqkv {
 // outputs from the matching 32 columns of R, staged as [32][D + 4] (16-byte
 // reads; each 16-lane phase of them covers all 64 banks).
 // ROT = false (R == nullptr): the normalised o_rot itself is the output.
-template <int D>
+// MS: the most splits.
+template <int D, int MS = kMaxSplits>
 struct MergeSmem {
   static constexpr int NC = 32;    // output columns per workgroup
   static constexpr int RP = D + 4;
   __align__(16) float rs[NC * RP];    // rs[jj][k] = R[k][c0 + jj]
   __align__(16) float os[kMergeHeads * D];
-  float wts[kMergeHeads][kMaxSplits];
+  float wts[kMergeHeads][MS];
 };
 
-template <int D, typename TOUT, bool ROT = true>
-__device__ __forceinline__ void decode_merge_body(MergeSmem<D> &sm, const float *__restrict__ part,
+template <int D, typename TOUT, bool ROT = true, int MS = kMaxSplits>
+__device__ __forceinline__ void decode_merge_body(MergeSmem<D, MS> &sm, const float *__restrict__ part,
                                                   const float *__restrict__ R, TOUT *__restrict__ out, int BHq,
                                                   int splits, int hg, int cg) {
   constexpr int NH = kMergeHeads;

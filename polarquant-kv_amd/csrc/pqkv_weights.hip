@@ -29,6 +29,15 @@ __device__ __forceinline__ float rows4_sum(float x) {
   return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
 }
 
+// The sum over each 16-lane row, in all of its lanes (row rotations).
+template <int N>
+__device__ __forceinline__ float row_ror_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float row16_sum(float x) {
+  return row_ror_add<1>(row_ror_add<2>(row_ror_add<4>(row_ror_add<8>(x))));
+}
+
 // ---- after a decode call ----
 //
 // weights[t] = in[t] + sum over the kv head's query heads of exp2(s_t - M) / L,
@@ -49,6 +58,17 @@ __device__ __forceinline__ void decode_weights_body(float2 *ml, const DecodeArgs
   const int t0 = (int)(blk - (uint32_t)bh * tiles) * kDwTokens + 4 * tid;
   const int b = (int)(bh / a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
   const int64_t row0 = (int64_t)b * a.Hq + (int64_t)h * a.gq;
+  // the first heads' logits (and what there was) are on their way while the
+  // partials are merged
+  constexpr int AHEAD = 4;
+  const bool there = t0 < a.S;
+  const float *lrow = w.logits + row0 * w.logit_stride + (there ? t0 : 0);
+  const float *in = w.in ? w.in + bh * w.in_stride + t0 : nullptr;
+  const bool vec = VEC && t0 + 4 <= a.S;
+  float4 s[AHEAD], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int g = 0; g < AHEAD; ++g) s[g] = *(const float4 *)(lrow + (int64_t)min(g, a.gq - 1) * w.logit_stride);
+  if (vec && in) o = *(const float4 *)in;
   for (int g = wave; g < a.gq; g += 4) {   // ml: per head of the group M, 1 / L
     const float *p = a.part + (row0 + g) * a.split_stride * (a.d + 2);
     float mx = -INFINITY, L = 0.0f;
@@ -62,27 +82,22 @@ __device__ __forceinline__ void decode_weights_body(float2 *ml, const DecodeArgs
     if (lane == 0) ml[g] = make_float2(mx, L > 0.0f ? 1.0f / L : 0.0f);
   }
   __syncthreads();
-  if (t0 >= a.S) return;
+  if (!there) return;
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const float *lrow = w.logits + row0 * w.logit_stride + t0;
+  auto add = [&](float4 v, float2 x) {
+    sum[0] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - x.x), x.y, sum[0]);
+    sum[1] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.y - x.x), x.y, sum[1]);
+    sum[2] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.z - x.x), x.y, sum[2]);
+    sum[3] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.w - x.x), x.y, sum[3]);
+  };
+#pragma unroll
+  for (int g = 0; g < AHEAD; ++g)
+    if (g < a.gq) add(s[g], ml[g]);
 #pragma unroll 4
-  for (int g = 0; g < a.gq; ++g) {
-    const float4 s = *(const float4 *)(lrow + (int64_t)g * w.logit_stride);
-    const float2 x = ml[g];
-    sum[0] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.x - x.x), x.y, sum[0]);
-    sum[1] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.y - x.x), x.y, sum[1]);
-    sum[2] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.z - x.x), x.y, sum[2]);
-    sum[3] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.w - x.x), x.y, sum[3]);
-  }
-  const float *in = w.in ? w.in + bh * w.in_stride + t0 : nullptr;
+  for (int g = AHEAD; g < a.gq; ++g) add(*(const float4 *)(lrow + (int64_t)g * w.logit_stride), ml[g]);
   float *out = w.out + bh * w.out_stride + t0;
-  if (VEC && t0 + 4 <= a.S) {
-    float4 o = in ? *(const float4 *)in : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    o.x += sum[0];
-    o.y += sum[1];
-    o.z += sum[2];
-    o.w += sum[3];
-    *(float4 *)out = o;
+  if (vec) {
+    *(float4 *)out = make_float4(o.x + sum[0], o.y + sum[1], o.z + sum[2], o.w + sum[3]);
     return;
   }
 #pragma unroll
@@ -90,12 +105,14 @@ __device__ __forceinline__ void decode_weights_body(float2 *ml, const DecodeArgs
     if (t0 + j < a.S) out[j] = (in ? in[j] : 0.0f) + sum[j];
 }
 
-template <int D, typename TOUT, bool VEC>
+// MS: the most splits the join's table of their weights holds (1024 of them
+// leave room for half as many workgroups).
+template <int D, typename TOUT, bool VEC, int MS>
 __global__ void __launch_bounds__(256) decode_merge_weights_kernel(const DecodeArgs a, const DecodeWeights w,
                                                                   const float *__restrict__ R,
                                                                   TOUT *__restrict__ out, int weight_blocks) {
   __shared__ union {
-    MergeSmem<D> merge;
+    MergeSmem<D, MS> merge;
     float2 ml[kMaxGroupWeights];
   } sm;
   const int blk = blockIdx.x;
@@ -103,7 +120,7 @@ __global__ void __launch_bounds__(256) decode_merge_weights_kernel(const DecodeA
     decode_weights_body<VEC>(sm.ml, a, w, (uint32_t)blk);
   } else {
     const int m = blk - weight_blocks;
-    decode_merge_body<D, TOUT, true>(sm.merge, a.part, R, out, a.B * a.Hq, a.split_stride, m / (D / 32), m % (D / 32));
+    decode_merge_body<D, TOUT, true, MS>(sm.merge, a.part, R, out, a.B * a.Hq, a.split_stride, m / (D / 32), m % (D / 32));
   }
 }
 
@@ -151,15 +168,24 @@ struct RowRec {                                    // 16 rows as B operands
   static constexpr int BYTES = KS * PARTS * 1024;  // segment (ks, part): 64 lanes x 16 bytes
 };
 
-// (x in a register of its own: where it is a product, the conversion may
+// Eight values as high and low parts, two at a time (one conversion a pair).
+// (x in registers of its own: where it is a product, the conversion may
 // otherwise be fused with it and round the unrounded product, while the
 // remainder is taken from the rounded one: a step of the high part lost on
 // values next to a tie)
-__device__ __forceinline__ void split_parts(float x, half_t *hi, half_t *lo) {
-  asm("" : "+v"(x));
-  const half_t h = (half_t)x;
-  *hi = h;
-  *lo = (half_t)(x - (float)h);
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split_parts(const float (&x)[8], half8_t *hi, half8_t *lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float u = x[i], v = x[i + 1];
+    asm("" : "+v"(u), "+v"(v));
+    const half2_t h = __builtin_convertvector((float2_t){u, v}, half2_t);
+    const half2_t l = __builtin_convertvector((float2_t){u - (float)h.x, v - (float)h.y}, half2_t);
+    (*hi)[i] = h.x;
+    (*hi)[i + 1] = h.y;
+    (*lo)[i] = l.x;
+    (*lo)[i + 1] = l.y;
+  }
 }
 
 // The power of two that brings `most` to [2^8, 2^9); 0 if it is zero, subnormal or not finite.
@@ -185,13 +211,10 @@ __device__ __forceinline__ void put_row(uint8_t *rec, int j, int rl, const float
 #pragma unroll
   for (int p = 0; p < (QJL ? 2 : 1); ++p) {
     half8_t hi, lo;
+    float e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      half_t u, v;
-      split_parts(x[p][i] * sc, &u, &v);
-      hi[i] = u;
-      lo[i] = v;
-    }
+    for (int i = 0; i < 8; ++i) e[i] = x[p][i] * sc;
+    split_parts(e, &hi, &lo);
     uint8_t *seg = rec + ((j >> 2) * Rec::PARTS + 2 * p) * 1024 + ((j & 3) * 16 + rl) * 16;
     *(half8_t *)seg = hi;
     *(half8_t *)(seg + 1024) = lo;
@@ -269,14 +292,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_ro
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const float4 u = rv[o][ks][0], v = rv[o][ks][1];
-      const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        half_t p, q;
-        split_parts(e[i] * rscale, &p, &q);
-        rh[o][ks][i] = p;
-        rl[o][ks][i] = q;
-      }
+      const float e[8] = {u.x * rscale, u.y * rscale, u.z * rscale, u.w * rscale,
+                          v.x * rscale, v.y * rscale, v.z * rscale, v.w * rscale};
+      split_parts(e, &rh[o][ks], &rl[o][ks]);
     }
 
   struct Operand {
@@ -305,14 +323,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_ro
       o.undo *= __builtin_ldexpf(1.0f, -sh);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const float e[8] = {u[ks][0].x, u[ks][0].y, u[ks][0].z, u[ks][0].w, u[ks][1].x, u[ks][1].y, u[ks][1].z, u[ks][1].w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          half_t p, q;
-          split_parts(e[i] * sc, &p, &q);
-          o.h[ks][i] = p;
-          o.l[ks][i] = q;
-        }
+        const float e[8] = {u[ks][0].x * sc, u[ks][0].y * sc, u[ks][0].z * sc, u[ks][0].w * sc,
+                            u[ks][1].x * sc, u[ks][1].y * sc, u[ks][1].z * sc, u[ks][1].w * sc};
+        split_parts(e, &o.h[ks], &o.l[ks]);
       }
     } else {
 #pragma unroll
@@ -472,18 +485,16 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
   for (int tt = 0; tt < TT; ++tt) {
     const float rs = radius[tt] * kscale;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < KS; ++ks) {
+      float e[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 c = pair_tab[a.bits == 4 ? (code[tt][ks] >> (8 * i)) & 255 : (code[tt][ks] >> (4 * i)) & 15];
-        half_t u, v;
-        split_parts(c.x * rs, &u, &v);
-        kh[tt][ks][2 * i] = u;
-        kl[tt][ks][2 * i] = v;
-        split_parts(c.y * rs, &u, &v);
-        kh[tt][ks][2 * i + 1] = u;
-        kl[tt][ks][2 * i + 1] = v;
+        e[2 * i] = c.x * rs;
+        e[2 * i + 1] = c.y * rs;
       }
+      split_parts(e, &kh[tt][ks], &kl[tt][ks]);
+    }
     if constexpr (QJL) {
       uint32_t w[D / 32];
       bool ones = true;
@@ -644,9 +655,7 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
   for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v = csum[tt][i];
-#pragma unroll
-      for (int sft = 1; sft < 16; sft <<= 1) v += shfl_xor_f(v, sft);
+      const float v = row16_sum(csum[tt][i]);
       const int t = tw0 + 16 * tt + 4 * grp + i;
       if (col == 0) {
         if (a.chunks > 1) a.col[((stream * a.chunks + chunk) * a.tblocks + tb) * TOK + t - t0] = v;
@@ -656,15 +665,17 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
     }
 }
 
-// Joins the token blocks' maxima and sums of 32 rows, eight threads per row;
+// Joins the token blocks' maxima and sums of RW rows, 256 / RW threads per row;
 // rows past the last one get (inf, 0), whose weights are 0.
+template <int RW>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs k) {
-  __shared__ float2 sub[8][32];
+  constexpr int SUB = 256 / RW;
+  __shared__ float2 sub[SUB][RW];
   const AttnWeightsArgs &a = k.a;
-  const uint32_t tiles = (uint32_t)a.row_tiles / 2;
+  const uint32_t tiles = (uint32_t)a.row_tiles * 16 / RW;
   const int64_t stream = blockIdx.x / tiles;
-  const int rl = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int r = (int)(blockIdx.x - (uint32_t)stream * tiles) * 32 + rl;
+  const int rl = threadIdx.x % RW, q = threadIdx.x / RW;
+  const int r = (int)(blockIdx.x - (uint32_t)stream * tiles) * RW + rl;
   const int rr = min(r, a.rows - 1);
   const int last = a.causal ? min(a.q_start + (int)k.group.div((uint32_t)(rr + a.row0)), a.S - 1) : a.S - 1;
   const int n = last / a.tokens + 1;
@@ -677,12 +688,12 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs
     m = mn;
   };
 #pragma unroll 8
-  for (int i = q; i < n; i += 8) join(p[(int64_t)i * a.rows]);
+  for (int i = q; i < n; i += SUB) join(p[(int64_t)i * a.rows]);
   sub[q][rl] = make_float2(m, l);
   __syncthreads();
   if (q != 0) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) join(sub[i][rl]);
+  for (int i = 1; i < SUB; ++i) join(sub[i][rl]);
   a.stat[stream * a.row_tiles * 16 + r] = r < a.rows ? make_float2(m, 1.0f / l) : make_float2(INFINITY, 0.0f);
 }
 
@@ -728,7 +739,9 @@ void launch_passes(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
     weights_rows_kernel<D, QJL><<<tiles, 2 * D, 0, s>>>(k);
   }
   attn_weights_kernel<D, QJL, TT, true><<<grid, 64 * kWW, 0, s>>>(k);
-  attn_stats_kernel<<<(unsigned)(streams * (a.row_tiles / 2)), 256, 0, s>>>(k);
+  // few rows of many blocks: more threads per row (128 rows x 8 streams of 1024 blocks 11 us -> 6)
+  if (tiles <= 1024 && a.tblocks > 64) attn_stats_kernel<8><<<2 * tiles, 256, 0, s>>>(k);
+  else attn_stats_kernel<32><<<tiles / 2, 256, 0, s>>>(k);
   attn_weights_kernel<D, QJL, TT, false><<<grid, 64 * kWW, 0, s>>>(k);
   if (a.chunks > 1)   // (one chunk: the sums are the result)
     weights_join_kernel<<<(unsigned)(streams * ((a.S + 255) / 256)), 256, 0, s>>>(a);
@@ -749,11 +762,14 @@ hipError_t launch_decode_merge_weights(const DecodeArgs &a, const DecodeWeights 
   const int wb = (int)((int64_t)((a.S + kDwTokens - 1) / kDwTokens) * a.B * a.Hkv);
   const int mb = (a.B * a.Hq + kMergeHeads - 1) / kMergeHeads * (a.d / 32);
   const bool vec = ((uintptr_t)w.out | (uintptr_t)w.in) % 16 == 0 && (w.out_stride | (w.in ? w.in_stride : 0)) % 4 == 0;
-#define PQKV_DMW(DD, T, V) \
-  decode_merge_weights_kernel<DD, T, V><<<(unsigned)(wb + mb), 256, 0, s>>>(a, w, R, (T *)out, wb)
+#define PQKV_DMW(DD, T, V, M) \
+  decode_merge_weights_kernel<DD, T, V, M><<<(unsigned)(wb + mb), 256, 0, s>>>(a, w, R, (T *)out, wb)
 #define PQKV_DMW_V(DD, T) \
-  if (vec) PQKV_DMW(DD, T, true); \
-  else PQKV_DMW(DD, T, false)
+  if (a.split_stride > 64) { \
+    if (vec) PQKV_DMW(DD, T, true, kMaxSplits); \
+    else PQKV_DMW(DD, T, false, kMaxSplits); \
+  } else if (vec) PQKV_DMW(DD, T, true, 64); \
+  else PQKV_DMW(DD, T, false, 64)
   if (a.d == 128 && out_dtype == PQKV_F32) { PQKV_DMW_V(128, float); }
   else if (a.d == 128) { PQKV_DMW_V(128, half_t); }
   else if (out_dtype == PQKV_F32) { PQKV_DMW_V(64, float); }
