@@ -374,8 +374,9 @@ int pqkv_prefill_attn(const void *q, int q_dtype, const float *R,
  * weights_*_stride floats in (a stride of at least S); weights_out may be
  * weights_in with the same stride, and may not overlap it otherwise. Keys and
  * values of one width n_bits (2 or 4), no per-head widths; S = 0 writes zeros
- * to out and no weights. S < 2^24, groups Hq / Hkv of up to 1024. The output equals pqkv_decode_attn's bit
- * for bit. */
+ * to out and no weights. S < 2^24, groups Hq / Hkv of up to 1024. The output
+ * equals pqkv_decode_attn's (its default kernel's) bit for bit. The workspace
+ * is 16-byte aligned and needs no initialisation. */
 size_t pqkv_decode_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int d);
 int pqkv_decode_attn_weights(const void *q, int q_dtype, const float *R,
                              const uint8_t *k_cache, const uint8_t *v_cache,
@@ -405,7 +406,8 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * (keys only: no values are read). Sq = 0 copies weights_in (or writes zeros);
  * S = 0 writes nothing. Groups Hq / Hkv of up to 1024, S < 2^24. The workspace
  * (qjl: with signs) needs no initialisation; past the rotated queries it stays
- * below 1 GB (long chunks run in passes). */
+ * below 1 GB up to a thousand (batch, kv-head) streams (long chunks run in
+ * passes). Queries on a 16-byte boundary are rotated on the way. */
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
                       int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,

@@ -137,6 +137,10 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, gq, gk):
         # y = M x with M a scaled rotation of each pair, so the gradient is the
         # same turn back: linear in g, and nothing of x is kept for it
+        if not ctx.needs_input_grad[0]:
+            gq = None
+        if not ctx.needs_input_grad[1]:
+            gk = None
         if gq is None and gk is None:
             return (None,) * 7
         turn = _Rotary.apply if torch.is_grad_enabled() else _turn      # (create_graph: differentiable again)

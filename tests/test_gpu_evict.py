@@ -203,6 +203,27 @@ def test_rows_that_are_views():
         assert torch.equal(m, torch.gather(v, 2, kept.long())) and m.dtype == v.dtype
 
 
+def test_rows_into_pages_of_a_table():
+    """pqkv_gather_rows into pages that lie anywhere (a result with a table and
+    no base): rows keep .. fill - 1 are zeros, the last page's rest is left alone."""
+    from polarquant_kv import _lib
+    B, H, S, keep, P, fill = 1, 3, 500, 150, 64, 170
+    c = random_cache(B, H, S, 64, 4, False, 8)
+    n, size = -(-fill // P), P * 36
+    pool = torch.full((H * n + 2, P, 36), 0xA5, dtype=torch.uint8, device=DEV)
+    slot = torch.randperm(H * n).view(H, n) + 1
+    table = (pool.data_ptr() + slot * size).to(DEV)
+    kept = torch.stack([torch.randperm(S)[:keep].sort().values for _ in range(H)]).int().to(DEV)
+    src = _lib.RowArray(c.blocks.data_ptr(), None, S * 36, 0, 0)
+    dst = _lib.RowArray(None, table.data_ptr(), 0, P, n)
+    _lib.check(_lib.lib().pqkv_gather_rows(1, (_lib.RowArray * 1)(src), (_lib.RowArray * 1)(dst), _lib.int_array([36]),
+                                           kept.data_ptr(), H, S, keep, fill, _lib.stream_of(kept)))
+    rows = pool[slot.flatten().to(DEV)].view(H, n * P, 36)
+    want = torch.gather(c.blocks[0], 1, kept.long()[..., None].expand(H, keep, 36))
+    assert torch.equal(rows[:, :keep], want) and not rows[:, keep:fill].any() and bool((rows[:, fill:] == 0xA5).all())
+    assert bool((pool[[0, -1]] == 0xA5).all())
+
+
 def test_caches_past_four_gigabytes():
     """Byte offsets of one stream past 2^32: 4-bit rows of 72 bytes, 61 million
     positions (the page-free cache is 4.4 GB)."""

@@ -120,6 +120,9 @@ def test_queries_alone_keys_alone_and_unused_outputs():
     g = torch.randn_like(qo)
     dq, = torch.autograd.grad(qo, q1, g)
     check(dq.contiguous(), g, pos, freqs, False, 1.0, inverse=True)
+    qo, ko = rotary.apply_rotary(q, k1, pos, freqs)                  # a query that needs no gradient
+    dk, = torch.autograd.grad((qo.float().sum() + ko.float().sum()), k1)
+    check(dk.contiguous(), torch.ones_like(k), pos, freqs, False, 1.0, inverse=True)
 
 
 def test_positions_of_each_sequence_and_integer_types():
