@@ -339,7 +339,9 @@ struct DecodeSmem {
 // through a buffer over its own page.
 // WS (decode with weights): every token's logit (exp2 domain) also goes to
 // a.logits, from the registers in which the softmax holds it: a lane holds
-// four consecutive tokens of one head, one 16-byte store.
+// four consecutive tokens of one head, one 16-byte store (8 sequences of 32768
+// tokens, 32 / 8 heads, 4 bits: 72 us where the kernel without takes 68; the
+// stores are 34 MB beside 302 read).
 // FREE: the steady-state iteration has no scheduling fences between its
 // table reads, softmax weights and products (the mixed-width pair kernel and
 // the ggml layout, 3.5 % and 2.4 % faster that way; the other kernels are as
