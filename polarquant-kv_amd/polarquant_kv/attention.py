@@ -190,7 +190,8 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
     if keys.mixed or values.mixed or keys.n_bits != values.n_bits:
         raise ValueError("weights take keys and values of one and the same width")
     _lib.require_device(query, rotation_matrix, jl_rot)
-    _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks)
+    _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks,
+                            values.codebooks, values.table if paged else values.blocks)
     if jl_rot is not None and keys.qjl_signs is None:
         raise ValueError("QJL correction requested but the key cache has no signs")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)

@@ -230,7 +230,9 @@ class KVCacheManager:
         """Cut the caches to `keep` positions per (batch, head): the first
         `sink`, the last `recent` and those with the most attention weight so
         far, in their order (eviction.evict; needs track_weights). Nothing is
-        done when no more than that are cached. Returns the Eviction, or None."""
+        done when no more than that are cached. Returns the Eviction, whose
+        caches, weights and positions are the manager's own from then on, or
+        None."""
         if not self.track_weights:
             raise ValueError("evict() needs track_weights")
         if keep < 1 or keep < sink + recent:

@@ -145,12 +145,10 @@ class PagedPQCache:
     def head_bits(self) -> list:
         return [self.n_bits] * self.num_heads
 
-    def _widen(self, pages: int) -> None:
+    def _widen(self, width: int) -> None:
+        """Tables of `width` pages where they are narrower."""
         import torch
-        width = self.max_pages
-        while width < pages:
-            width *= 2
-        if width == self.max_pages:
+        if width <= self.max_pages:
             return
         n = self.batch * self.num_heads
         t = torch.zeros(n, width, dtype=torch.int64, device=self.device)
@@ -172,7 +170,10 @@ class PagedPQCache:
         need = -(-int(positions) // self.page_tokens)
         if need <= len(self.groups):
             return
-        self._widen(need)
+        width = self.max_pages
+        while width < need:
+            width *= 2
+        self._widen(width)
         B, H, P = self.batch, self.num_heads, self.page_tokens
         streams = torch.arange(B * H, dtype=torch.int64, device=self.device)
         while len(self.groups) < need:

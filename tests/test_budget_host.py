@@ -211,6 +211,22 @@ def test_reserved_pages():
     assert e.reserve(0) == [] and e.capacity == 0
 
 
+@pytest.mark.parametrize("pages", [(3, 16), (16, 3), (1, 3), (5, 7)])
+def test_tables_of_two_caches_get_one_width(pages):
+    """The kernels walk both tables with one row stride, whatever the caches'
+    tables were made for (an evicted cache's have as many pages as it needs)."""
+    cb = torch.zeros(16)
+    keys, values = (PagedPQCache(2, 2, 64, 4, cb, "cpu", 64, 0, n) for n in pages)
+    for c in (keys, values):
+        c.ensure(c.max_pages * 64)
+        c.seq_len = 40
+    rows = [c.table.clone() for c in (keys, values)]
+    attention.check_paged(2, 4, 64, keys, values)
+    assert keys.max_pages == values.max_pages == max(pages)
+    for c, old in zip((keys, values), rows):
+        assert c.table.shape == (4, max(pages)) and torch.equal(c.table[:, :old.shape[1]], old)
+
+
 def test_frequencies_plain_and_linear():
     f, m = rotary.rotary_frequencies(8, 10000.0)
     assert f.dtype == torch.float64 and m == 1.0
