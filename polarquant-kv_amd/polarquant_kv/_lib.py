@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PQKV_LIBRARY selects another build of the library (same ABI), e.g. one
@@ -34,6 +35,13 @@ class RowArray(ctypes.Structure):
 
 
 MAX_GATHER = 6                          # PQKV_MAX_GATHER
+
+
+def row_arrays(fields) -> bytes:
+    """pqkv_row_array[] of the arrays' five fields each, one after the other
+    (0 for no pointer)."""
+    return struct.pack("PPqii" * (len(fields) // 5), *fields)
+
 
 # name -> (restype, argtypes); the full exported surface of include/pqkv.h
 SIGNATURES = {
@@ -120,8 +128,8 @@ SIGNATURES = {
                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "pqkv_evict_select": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "pqkv_gather_rows": (c_int, [c_int, ctypes.POINTER(RowArray), ctypes.POINTER(RowArray), c_int_p, c_void_p, c_int64,
-                                 c_int, c_int, c_int, c_void_p]),
+    "pqkv_gather_rows": (c_int, [c_int, c_void_p, c_void_p, c_int_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                 c_void_p]),
     "pqkv_rotary": (c_int, [c_void_p, c_int64_p, c_void_p, c_int, c_void_p, c_int64_p, c_void_p, c_int, c_int,
                             c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                             c_void_p]),

@@ -200,7 +200,7 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
     previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
     q = query if query.is_contiguous() else query.contiguous()
     R, P = _lib.dense_f32(rotation_matrix), _lib.dense_f32(jl_rot)
-    out = torch.empty(B, Hq, d, dtype=out_dtype, device=q.device)
+    out = torch.empty_like(q, dtype=out_dtype)
     lib = _lib.lib()
     ws = torch.empty(lib.pqkv_decode_attn_weights_workspace_bytes(B, Hq, Hkv, max(S, 1), d), dtype=torch.uint8,
                      device=q.device)

@@ -68,15 +68,15 @@ def _cache_arrays(cache):
     signs, of those."""
     vb = vector_bytes(cache.head_dim, cache.n_bits)
     if isinstance(cache, PagedPQCache):
-        out = [((None, cache.table.data_ptr(), 0, cache.page_tokens, cache.max_pages), vb)]
+        out = [((0, cache.table.data_ptr(), 0, cache.page_tokens, cache.max_pages), vb)]
         if cache.sign_table is not None:
-            out.append(((None, cache.sign_table.data_ptr(), 0, cache.page_tokens, cache.max_pages),
+            out.append(((0, cache.sign_table.data_ptr(), 0, cache.page_tokens, cache.max_pages),
                         cache.jl_dim // 8))
         return out
-    out = [((cache.blocks.data_ptr(), None, cache.max_seq_len * vb, 0, 0), vb)]
+    out = [((cache.blocks.data_ptr(), 0, cache.max_seq_len * vb, 0, 0), vb)]
     if cache.qjl_signs is not None:
         m8 = cache.qjl_signs.shape[-1]
-        out.append(((cache.qjl_signs.data_ptr(), None, cache.max_seq_len * m8, 0, 0), m8))
+        out.append(((cache.qjl_signs.data_ptr(), 0, cache.max_seq_len * m8, 0, 0), m8))
     return out
 
 
@@ -94,11 +94,10 @@ def _empty_like(cache, positions: int, room: int):
         P, n = cache.page_tokens, -(-positions // cache.page_tokens)
         return new, [((pool.data_ptr(), table.data_ptr(), n * P * pool.shape[-1], P, n), pool.shape[-1])
                      for pool, table in zip(new.reserve(positions), (new.table, new.sign_table))]
-    fresh = torch.empty if room == positions else torch.zeros
-    device, signs = cache.blocks.device, None
+    fresh, signs = cache.blocks.new_empty if room == positions else cache.blocks.new_zeros, None
     if cache.qjl_signs is not None:
-        signs = fresh(B, H, room, cache.qjl_signs.shape[-1], dtype=torch.uint8, device=device)
-    new = PQCache(blocks=fresh(B, H, room, vector_bytes(d, cache.n_bits), dtype=torch.uint8, device=device),
+        signs = fresh((B, H, room, cache.qjl_signs.shape[-1]))
+    new = PQCache(blocks=fresh((B, H, room, vector_bytes(d, cache.n_bits))),
                   head_dim=d, n_bits=cache.n_bits, seq_len=0, max_seq_len=room, codebooks=cache.codebooks,
                   qjl_signs=signs, jl_dim=cache.jl_dim)
     return new, _cache_arrays(new)
@@ -161,8 +160,8 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
                     raise ValueError("paged caches in one move must share page_tokens")
                 fill = c.capacity
             for (a, size), (n, _) in zip(_cache_arrays(old), arrays):
-                src.append(a)
-                dst.append(n)
+                src += a
+                dst += n
                 sizes.append(size)
             c.seq_len = keep
             new.append(c)
@@ -172,17 +171,16 @@ def gather_positions(caches, kept: torch.Tensor, rows=(), room: int | None = Non
                 raise ValueError(f"rows must be 4-byte [{B}, {H}, >= {S}] tensors, got {tuple(t.shape)} {t.dtype}")
             t = _check_rows(t, "rows")
             held.append(t)
-            n = torch.empty(B, H, keep, dtype=t.dtype, device=t.device)
-            src.append((t.data_ptr(), None, 4 * _row_stride(t), 0, 0))
-            dst.append((n.data_ptr(), None, 4 * keep, 0, 0))
+            n = torch.empty_like(kept, dtype=t.dtype)
+            src.extend((t.data_ptr(), 0, 4 * _row_stride(t), 0, 0))
+            dst.extend((n.data_ptr(), 0, 4 * keep, 0, 0))
             sizes.append(4)
             new_rows.append(n)
-        if len(src) > _lib.MAX_GATHER:
-            raise ValueError(f"{len(src)} arrays in one move, at most {_lib.MAX_GATHER}")
+        if len(sizes) > _lib.MAX_GATHER:
+            raise ValueError(f"{len(sizes)} arrays in one move, at most {_lib.MAX_GATHER}")
         if keep > 0:
-            arrays = _lib.RowArray * len(src)
-            _lib.check(_lib.lib().pqkv_gather_rows(len(src), arrays(*src), arrays(*dst), _lib.int_array(sizes),
-                                                   kept.data_ptr(), B * H, S, keep, fill,
+            _lib.check(_lib.lib().pqkv_gather_rows(len(sizes), _lib.row_arrays(src), _lib.row_arrays(dst),
+                                                   _lib.int_array(sizes), kept.data_ptr(), B * H, S, keep, fill,
                                                    _lib.stream_of(kept)))
     return new, new_rows
 
