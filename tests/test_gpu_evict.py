@@ -192,6 +192,41 @@ def test_positions_outside_the_cache_give_zeros_and_may_repeat():
     assert not n.blocks[:, :, [0, 4, 5]].any()
 
 
+@pytest.mark.parametrize("keep,pages", [(130, 16), (190, 4), (64, 1)])
+def test_attention_on_tables_of_different_widths(keep, pages):
+    """An evicted cache's table has as many pages as it needs; beside values
+    whose table was made for more (or for as many as a power of two), both are
+    read with one row stride."""
+    from polarquant_kv import attention
+    g = torch.Generator(device=DEV).manual_seed(9)
+    B, Hq, H, d, P = 2, 8, 4, 64, 64
+    cb = torch.linspace(-1, 1, 16, device=DEV)
+    R = torch.linalg.qr(torch.randn(d, d, generator=g, device=DEV))[0].contiguous()
+
+    def cache(S):
+        rows = torch.randint(0, 256, (B, H, S, d // 32, 18), generator=g, device=DEV, dtype=torch.uint8)
+        rows[..., :2] = (0.5 + torch.rand(B, H, S, d // 32, generator=g, device=DEV)).half().view(torch.uint8).view(
+            B, H, S, d // 32, 2)                                       # a finite radius
+        return PQCache(blocks=rows.flatten(3), head_dim=d, n_bits=4, seq_len=S, max_seq_len=S, codebooks=cb)
+
+    old, values = cache(300), cache(keep)
+    kept = torch.randint(0, 300, (B, H, keep), generator=g, device=DEV, dtype=torch.int32)
+    (paged,), _ = eviction.gather_positions([paged_copy(old, P)], kept)
+    (flat,), _ = eviction.gather_positions([old], kept)
+    assert paged.max_pages == -(-keep // P)
+    wide = PagedPQCache(B, H, d, 4, cb, DEV, page_tokens=P, max_pages=pages)
+    wide.ensure(keep)
+    for p, group in enumerate(wide.groups):
+        group[:, :, :min(P, keep - p * P)] = values.blocks[:, :, p * P:(p + 1) * P]
+    wide.seq_len = keep
+    q = torch.randn(B, Hq, d, generator=g, device=DEV).half()
+    out, w = attention.decode_attention_weights(q, paged, wide, R)
+    want, w_flat = attention.decode_attention_weights(q, flat, values, R)
+    assert torch.equal(out, want) and torch.equal(w, w_flat)
+    assert torch.equal(attention.decode_attention(q, paged, wide, R), want)
+    assert paged.max_pages == wide.max_pages
+
+
 def test_rows_that_are_views():
     c = random_cache(2, 2, 60, 64, 4, False, 6)
     kept = torch.arange(0, 60, 3, device=DEV, dtype=torch.int32).expand(2, 2, 20)

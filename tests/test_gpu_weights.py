@@ -280,6 +280,29 @@ def test_on_another_stream_and_captured():
         assert torch.equal(w, attention.attention_weights(qc, kc, R, 880))
 
 
+def test_calls_on_two_streams_at_once():
+    """Each call has its own workspace: calls that overlap give what they give alone."""
+    work = [make(2, 16, 4, 3000 + 500 * i, 128, 4, bool(i), seed=5 + i) for i in range(2)]
+    chunk = [torch.randn(2, 16, 70, 128, device=DEV).half() for _ in work]
+
+    def step(i):
+        q, kc, vc, R, jl = work[i]
+        out, w = attention.decode_attention_weights(q, kc, vc, R, jl_rot=jl)
+        return out, w, attention.attention_weights(chunk[i], kc, R, kc.seq_len - 70, jl_rot=jl, previous=w)
+
+    alone = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(5):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(step(i))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_unequal_widths_and_missing_signs_are_refused():
     q, kc, vc, R, _ = make(1, 4, 2, 50, 64, 4, False)
     _, k2, _, _, _ = make(1, 4, 2, 50, 64, 2, False)
