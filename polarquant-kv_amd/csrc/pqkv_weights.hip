@@ -1,5 +1,5 @@
 // The attention weight that each cached position gets: after a decode call,
-// from the logits it wrote (decode_weights_kernel), and for a chunk of query
+// from the logits it wrote (decode_merge_weights_kernel), and for a chunk of query
 // tokens (attn_weights_kernel).
 #include <type_traits>
 
