@@ -18,6 +18,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -125,13 +126,30 @@ def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):
     return qo, ko
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether any of them carries a forward-mode derivative."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse):
         ctx.save_for_backward(positions, freqs)
+        ctx.save_for_forward(positions, freqs)
         ctx.how = (interleaved, amplitude, not inverse)
+        ctx.shapes, ctx.dtype = (q.shape, None if k is None else k.shape), q.dtype
         ctx.set_materialize_grads(False)
         return _turn(q, k, positions, freqs, interleaved, amplitude, inverse)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # y = M x: the tangent is M times x's (which may be of another type)
+        interleaved, amplitude, back = ctx.how
+        turn = _Rotary.apply if torch.is_grad_enabled() else _turn
+        moving = [t.to(ctx.dtype) for t in (tq, tk) if t is not None]
+        out = list(turn(*(moving + [None])[:2], *ctx.saved_tensors, interleaved, amplitude, not back))
+        return tuple(None if shape is None else moving[0].new_zeros(shape) if t is None else out.pop(0)
+                     for t, shape in zip((tq, tk), ctx.shapes))
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -143,7 +161,8 @@ class _Rotary(torch.autograd.Function):
             gk = None
         if gq is None and gk is None:
             return (None,) * 7
-        turn = _Rotary.apply if torch.is_grad_enabled() else _turn      # (create_graph: differentiable again)
+        # (create_graph, or gradients with tangents: differentiable again)
+        turn = _Rotary.apply if torch.is_grad_enabled() or _has_tangent(gq, gk) else _turn
         if gq is None:
             out = (None, turn(gk, None, *ctx.saved_tensors, *ctx.how)[0])
         else:
@@ -159,7 +178,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     or fp32; one for both). positions: integers [T] or [B, T]; frequencies:
     radians per position, float64 (rotary_frequencies, on the device). Pairs
     are (i, i + rot_dim / 2), or neighbours with interleaved. The inputs may
-    have any strides and may be expanded; gradients flow to both."""
+    have any strides and may be expanded; gradients flow to both, and
+    forward-mode tangents (torch.autograd.forward_ad) through them."""
     for name, x in (("query", query), ("key", key)):
         if x is not None and x.dim() != 4:
             raise ValueError(f"{name} must be [B, H, T, d], got {tuple(x.shape)}")
@@ -182,7 +202,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"positions must be [{T}] or [{B}, {T}], got {tuple(positions.shape)}")
     args = (query, key, positions.to(torch.int64).contiguous(), frequencies.contiguous(), bool(interleaved),
             float(amplitude))
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+    if (torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))) or \
+            _has_tangent(query, key):
         return _Rotary.apply(*args, False)
     return _turn(*args, False)
 
