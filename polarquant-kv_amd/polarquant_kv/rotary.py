@@ -211,7 +211,9 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
 class RotaryEmbedding:
     """apply_rotary with the frequencies of one head shape: rot_dim (default:
     the whole head) of head_dim coordinates, base, scaling and pairing as
-    rotary_frequencies and apply_rotary take them."""
+    rotary_frequencies and apply_rotary take them. The first call on a device
+    copies the frequencies to it, which a graph capture does not allow: such a
+    call is refused there."""
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, base: float = 10000.0, scaling: dict | None = None,
                  interleaved: bool = False):
@@ -220,13 +222,18 @@ class RotaryEmbedding:
         if self.rot_dim > head_dim:
             raise ValueError(f"rot_dim {rot_dim} exceeds head_dim {head_dim}")
         self.interleaved = interleaved
-        self.frequencies, self.amplitude = rotary_frequencies(self.rot_dim, base, scaling)
+        with torch.inference_mode(False):
+            self.frequencies, self.amplitude = rotary_frequencies(self.rot_dim, base, scaling)
         self._on: dict = {}            # the frequencies on each device used
 
     def __call__(self, query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor):
         freqs = self._on.get(query.device)
         if freqs is None:
-            freqs = self._on[query.device] = self.frequencies.to(query.device)
+            if query.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"call the embedding on {query.device} once before a capture")
+            # they serve later calls, which may be differentiated whatever mode this one runs in
+            with torch.inference_mode(False):
+                freqs = self._on[query.device] = self.frequencies.to(query.device)
         return apply_rotary(query, key, positions, freqs, interleaved=self.interleaved, amplitude=self.amplitude)
 
 

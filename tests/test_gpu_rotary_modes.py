@@ -26,3 +26,27 @@ def test_forward_mode_tangents(dtype):
         one = [forward_ad.unpack_dual(x) for x in rotary.apply_rotary(q, dk, pos, f, **how)]
         assert one[0].tangent is None or not one[0].tangent.any()
         assert torch.equal(one[1].tangent, t[1])
+
+
+def test_embedding_used_in_inference_mode_first():
+    emb = rotary.RotaryEmbedding(64)
+    q, pos = torch.randn(1, 2, 9, 64, device=DEV), torch.arange(9, device=DEV)
+    with torch.inference_mode():
+        y = emb(q, None, pos)[0].clone()
+    q1 = q.clone().requires_grad_(True)
+    out = emb(q1, None, pos)[0]
+    assert torch.equal(out, y)
+    g, = torch.autograd.grad(out, q1, y)
+    assert torch.allclose(g, q, atol=1e-5)                      # turned and turned back
+
+
+def test_first_call_in_a_capture_is_refused(monkeypatch):
+    emb = rotary.RotaryEmbedding(64)
+    q, pos = torch.randn(1, 2, 9, 64, device=DEV), torch.arange(9, device=DEV)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before a capture"):
+        emb(q, None, pos)
+    monkeypatch.undo()
+    emb(q, None, pos)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    emb(q, None, pos)

@@ -101,3 +101,16 @@ def test_tangents_of_gradients_and_gradients_of_tangents(launches, doubles):
     assert torch.equal(g, back(tk.expand_as(tq)))
     assert torch.autograd.gradcheck(lambda a, b: rotary.apply_rotary(a, b, pos, f, amplitude=1.25),
                                     (q1, k.clone().requires_grad_(True)), check_forward_ad=True)
+
+
+def test_embedding_used_in_inference_mode_first(launches):
+    """What the embedding keeps from a call outlives its mode."""
+    q, k, _, _, pos, _ = inputs(torch.float32)
+    with torch.inference_mode():
+        emb = rotary.RotaryEmbedding(8)
+        emb(q.clone(), k.clone(), pos)
+    assert not emb.frequencies.is_inference()
+    q1 = q.clone().requires_grad_(True)
+    y, _ = emb(q1, k, pos)
+    g, = torch.autograd.grad(y, q1, torch.ones_like(y))
+    assert torch.equal(g, formula(torch.ones_like(q), pos, emb.frequencies, False, 1.0, True))
