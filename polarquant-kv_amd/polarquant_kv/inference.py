@@ -276,10 +276,12 @@ class KVCacheManager:
                                                             jl_rot=self.jl_rot, out_dtype=torch.float16, previous=w,
                                                             into=w)
                 return out.unsqueeze(2)
+            # the weights last: a call that fails has added none of them
+            out = attention.prefill_attention(query, self._keys, self._values, self.R, start, causal=causal,
+                                              out_dtype=torch.float16, jl_rot=self.jl_rot)
             attention.attention_weights(query, self._keys, self.R, start, causal=causal, jl_rot=self.jl_rot,
                                         previous=w, into=w)
-            return attention.prefill_attention(query, self._keys, self._values, self.R, start, causal=causal,
-                                               out_dtype=torch.float16, jl_rot=self.jl_rot)
+            return out
         jl = self.jl_matrix if self.jl_rot is not None else None
         return attention.compressed_attention_gpu(query, self._keys, self._values, self.R, jl_matrix=jl,
                                                   causal=causal, q_start=start)
