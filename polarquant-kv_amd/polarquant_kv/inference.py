@@ -109,8 +109,9 @@ class KVCacheManager:
             self._values = quantizer.allocate_paged_cache(B, H, d, bits, self.device, page_tokens=self.page_tokens)
         else:
             shape = (self.batch, self.num_heads, self.max_seq_len, self.head_dim)
-            self._key_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
-            self._value_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
+            with torch.inference_mode(False):   # written by later calls in whatever mode
+                self._key_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
+                self._value_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
 
     @property
     def seq_len(self) -> int:
@@ -181,26 +182,28 @@ class KVCacheManager:
             raise RuntimeError(f"KV cache full: {self._seq_len} + {T} > {self.max_seq_len}")
         if self._keys is None and self._key_cache is None:
             self._allocate()
+        if self.track_weights:                 # (first: if it fails, nothing is in the caches)
+            self._track(T)
         if self.config.enable_compression:
             quantizer.compress_pq(key, self.R, cache=self._keys, start=self._seq_len, jl_rot=self.jl_rot)
             quantizer.compress_pq(value, self.R, cache=self._values, start=self._seq_len)
         else:
             self._key_cache[:, :, self._seq_len:self._seq_len + T] = key.to(torch.float16)
             self._value_cache[:, :, self._seq_len:self._seq_len + T] = value.to(torch.float16)
-        if self.track_weights:
-            self._track(T)
         self._seq_len += T
         self._next_position += T
 
     def _track(self, T: int) -> None:
-        """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions."""
+        """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions.
+        (Not inference tensors: later calls write them in whatever mode.)"""
         S, need = self._seq_len, self._seq_len + T
         room = 0 if self._weights is None else self._weights.shape[2]
         if need > room:
             room = min(max(need, 2 * room, self.page_tokens), self.max_seq_len)
             shape = (self.batch, self.num_heads, room)
-            w = torch.zeros(shape, dtype=torch.float32, device=self.device)
-            p = torch.zeros(shape, dtype=torch.int32, device=self.device)
+            with torch.inference_mode(False):
+                w = torch.zeros(shape, dtype=torch.float32, device=self.device)
+                p = torch.zeros(shape, dtype=torch.int32, device=self.device)
             if S:
                 w[:, :, :S], p[:, :, :S] = self._weights[:, :, :S], self._positions[:, :, :S]
             self._weights, self._positions = w, p
@@ -240,8 +243,9 @@ class KVCacheManager:
         if self._seq_len <= keep:
             return None
         from . import eviction
-        r = eviction.evict(self._keys, self._values, self._weights, keep, sink=sink, recent=recent,
-                           positions=self._positions)
+        with torch.inference_mode(False):
+            r = eviction.evict(self._keys, self._values, self._weights, keep, sink=sink, recent=recent,
+                               positions=self._positions)
         self._keys, self._values, self._weights, self._positions = r.keys, r.values, r.weights, r.positions
         self._seq_len = keep
         return r

@@ -100,9 +100,16 @@ class PagedPQCache:
         self.max_pages = max(1, int(max_pages))
         if not tables:                # reserve() follows and makes them
             return
-        n = batch * num_heads
-        self.table = torch.zeros(n, self.max_pages, dtype=torch.int64, device=self.device)
-        self.sign_table = torch.zeros_like(self.table) if jl_dim else None
+        self.table, self.sign_table = self._new_tables(self.max_pages)
+
+    def _new_tables(self, width: int):
+        """Zeroed page tables of `width` pages (the second None without signs).
+        Written again by later calls in whatever mode those run, so never
+        inference tensors."""
+        import torch
+        with torch.inference_mode(False):
+            t = torch.zeros(self.batch * self.num_heads, width, dtype=torch.int64, device=self.device)
+            return t, torch.zeros_like(t) if self.jl_dim else None
 
     def adopt(self, table, capacity: int, storage, sign_table=None) -> None:
         """Use caller-managed pages instead of page groups: table (and, for a
@@ -147,17 +154,13 @@ class PagedPQCache:
 
     def _widen(self, width: int) -> None:
         """Tables of `width` pages where they are narrower."""
-        import torch
         if width <= self.max_pages:
             return
-        n = self.batch * self.num_heads
-        t = torch.zeros(n, width, dtype=torch.int64, device=self.device)
-        t[:, :self.max_pages] = self.table
-        self.table = t
-        if self.sign_table is not None:
-            t = torch.zeros_like(self.table)
-            t[:, :self.max_pages] = self.sign_table
-            self.sign_table = t
+        table, signs = self._new_tables(width)
+        table[:, :self.max_pages] = self.table
+        if signs is not None:
+            signs[:, :self.max_pages] = self.sign_table
+        self.table, self.sign_table = table, signs
         self.max_pages = width
 
     def ensure(self, positions: int) -> None:
@@ -200,7 +203,8 @@ class PagedPQCache:
         if n == 0:
             return []
         B, H = self.batch, self.num_heads
-        tables = torch.empty(2 if self.jl_dim else 1, B * H, n, dtype=torch.int64, device=self.device)
+        with torch.inference_mode(False):      # (as _new_tables)
+            tables = torch.empty(2 if self.jl_dim else 1, B * H, n, dtype=torch.int64, device=self.device)
         self.table, self.max_pages = tables[0], n
         blocks = torch.empty(B, H, n, self.page_tokens, self.vector_bytes, dtype=torch.uint8, device=self.device)
         self.groups = list(blocks.unbind(2))
@@ -248,8 +252,7 @@ class PagedPQCache:
         self.sign_groups = [g.index_select(0, index) for g in self.sign_groups]
         self.batch = int(index.numel())
         n = self.batch * self.num_heads
-        self.table = torch.zeros(n, self.max_pages, dtype=torch.int64, device=self.device)
-        self.sign_table = torch.zeros_like(self.table) if self.jl_dim else None
+        self.table, self.sign_table = self._new_tables(self.max_pages)
         streams = torch.arange(n, dtype=torch.int64, device=self.device)
         P = self.page_tokens
         for p, g in enumerate(self.groups):
