@@ -89,6 +89,19 @@ def check_paged(B: int, Hq: int, d: int, keys: PagedPQCache, values: PagedPQCach
     return Hkv
 
 
+def check_signs(jl_rot, keys, d: int) -> None:
+    """The projections of a QJL correction and the keys' signs, as the kernels
+    read them: d projections of d coordinates, d / 8 bytes of signs per key."""
+    if jl_rot is None:
+        return
+    if keys.qjl_signs is None:
+        raise ValueError("QJL correction requested but the key cache has no signs")
+    if tuple(jl_rot.shape) != (d, d):
+        raise ValueError(f"jl_rot must be ({d}, {d}), got {tuple(jl_rot.shape)}")
+    if keys.jl_dim not in (0, d):
+        raise ValueError(f"the keys' signs are of {keys.jl_dim} projections, jl_rot of {d}")
+
+
 def decode_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotation_matrix: torch.Tensor,
                      scale: float | None = None, jl_rot: torch.Tensor | None = None,
                      out_dtype: torch.dtype | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -100,6 +113,7 @@ def decode_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotati
     if isinstance(keys, PagedPQCache) or isinstance(values, PagedPQCache):
         return _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype, workspace)
     Hkv = check_shapes(B, Hq, d, keys, values, rotation_matrix)
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out_dtype = query.dtype if out_dtype is None else out_dtype
@@ -116,8 +130,6 @@ def decode_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotati
     vbits = _lib.int_array(values.head_bits()) if mixed else None
     kcb, vcb = _codebook_tables(keys, values, mixed, Hkv)
     qjl = keys.qjl_signs if jl_rot is not None else None
-    if jl_rot is not None and qjl is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
     _lib.check(lib.pqkv_decode_attn(
         q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.blocks.data_ptr(), values.blocks.data_ptr(),
@@ -130,6 +142,7 @@ def decode_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotati
 def _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype, workspace):
     B, Hq, d = query.shape
     Hkv = check_paged(B, Hq, d, keys, values, rotation_matrix)
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out_dtype = query.dtype if out_dtype is None else out_dtype
@@ -141,8 +154,6 @@ def _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype
     need = lib.pqkv_decode_workspace_bytes(B, Hq, Hkv, max(S, 1), d)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    if jl_rot is not None and keys.sign_table is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
     _lib.check(lib.pqkv_decode_attn_paged(
         q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),
@@ -189,11 +200,10 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
     Hkv = (check_paged if paged else check_shapes)(B, Hq, d, keys, values, rotation_matrix)
     if keys.mixed or values.mixed or keys.n_bits != values.n_bits:
         raise ValueError("weights take keys and values of one and the same width")
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks,
                             values.codebooks, values.table if paged else values.blocks)
-    if jl_rot is not None and keys.qjl_signs is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out_dtype = query.dtype if out_dtype is None else out_dtype
     S = keys.seq_len
@@ -239,10 +249,9 @@ def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, 
     Hkv = (check_paged if paged else check_shapes)(B, Hq, d, keys, keys, rotation_matrix)
     if keys.mixed:
         raise ValueError("weights take keys of one width")
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks)
-    if jl_rot is not None and keys.qjl_signs is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     S = keys.seq_len
     previous, into, result = _weights_args(B, Hkv, S, previous, into, query.device)
@@ -323,6 +332,7 @@ def prefill_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotat
     if isinstance(keys, PagedPQCache) or isinstance(values, PagedPQCache):
         return _prefill_paged(query, keys, values, rotation_matrix, q_start, causal, scale, out_dtype, jl_rot)
     Hkv = check_shapes(B, Hq, d, keys, values, rotation_matrix)
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out_dtype = query.dtype if out_dtype is None else out_dtype
@@ -339,8 +349,6 @@ def prefill_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotat
     vbits = _lib.int_array(values.head_bits()) if mixed else None
     kcb, vcb = _codebook_tables(keys, values, mixed, Hkv)
     qjl = keys.qjl_signs if jl_rot is not None else None
-    if jl_rot is not None and qjl is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
     _lib.check(lib.pqkv_prefill_attn(
         q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.blocks.data_ptr(), values.blocks.data_ptr(),
@@ -354,6 +362,7 @@ def prefill_attention(query: torch.Tensor, keys: PQCache, values: PQCache, rotat
 def _prefill_paged(query, keys, values, rotation_matrix, q_start, causal, scale, out_dtype, jl_rot):
     B, Hq, Sq, d = query.shape
     Hkv = check_paged(B, Hq, d, keys, values, rotation_matrix)
+    check_signs(jl_rot, keys, d)
     _lib.require_device(query, rotation_matrix, jl_rot)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out_dtype = query.dtype if out_dtype is None else out_dtype
@@ -365,8 +374,6 @@ def _prefill_paged(query, keys, values, rotation_matrix, q_start, causal, scale,
     shape = (B, Hq, Hkv, Sq, max(S, 1), d)
     ws = _lib.workspace(lib.pqkv_prefill_workspace_preferred_bytes(*shape, int(jl_rot is not None)),
                         lambda: lib.pqkv_prefill_workspace_bytes(*shape), q.device)
-    if jl_rot is not None and keys.sign_table is None:
-        raise ValueError("QJL correction requested but the key cache has no signs")
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
     _lib.check(lib.pqkv_prefill_attn_paged(
         q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),

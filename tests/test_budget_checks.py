@@ -1,0 +1,51 @@
+"""Arguments that the kernels would read past, refused before any launch; no GPU."""
+
+import pytest
+import torch
+
+from polarquant_kv import attention
+from polarquant_kv.types import PagedPQCache, PQCache
+
+D = 64
+
+
+def caches(paged, jl_dim=D):
+    out = []
+    for signs in (jl_dim, 0):
+        if paged:
+            c = PagedPQCache(1, 2, D, 4, torch.zeros(16), "cpu", 64, jl_dim=signs)
+            c.ensure(8)
+            c.seq_len = 8
+        else:
+            c = PQCache(blocks=torch.zeros(1, 2, 8, 36, dtype=torch.uint8), head_dim=D, n_bits=4, seq_len=8, max_seq_len=8,
+                        codebooks=torch.zeros(16), jl_dim=signs,
+                        qjl_signs=torch.zeros(1, 2, 8, max(signs, 64) // 8, dtype=torch.uint8) if signs else None)
+        out.append(c)
+    return out
+
+
+def calls(kc, vc, jl_rot):
+    q, R = torch.zeros(1, 4, D), torch.eye(D)
+    yield lambda: attention.decode_attention_weights(q, kc, vc, R, jl_rot=jl_rot)
+    yield lambda: attention.attention_weights(q.unsqueeze(2), kc, R, 7, jl_rot=jl_rot)
+    yield lambda: attention.decode_attention(q, kc, vc, R, jl_rot=jl_rot)
+    yield lambda: attention.prefill_attention(q.unsqueeze(2), kc, vc, R, 7, jl_rot=jl_rot)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_projections_of_another_size(paged):
+    kc, vc = caches(paged)
+    for shape in ((32, D), (D, 32), (128, D), (D,)):
+        for call in calls(kc, vc, torch.zeros(shape)):
+            with pytest.raises(ValueError, match="jl_rot must be"):
+                call()
+    for call in calls(kc, vc, torch.zeros(D, D)):               # as they should be: on to the next check
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
+    for call in calls(vc, vc, torch.zeros(D, D)):
+        with pytest.raises(ValueError, match="no signs"):
+            call()
+    kc, vc = caches(paged, 128)
+    for call in calls(kc, vc, torch.zeros(D, D)):
+        with pytest.raises(ValueError, match="projections"):
+            call()
