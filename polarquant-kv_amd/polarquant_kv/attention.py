@@ -78,15 +78,29 @@ def check_paged(B: int, Hq: int, d: int, keys: PagedPQCache, values: PagedPQCach
     for c in (keys, values):
         if c.capacity < c.seq_len:
             raise ValueError("paged cache holds fewer pages than its seq_len needs")
-    # one table width for both (the kernels take one row stride)
+    # one table width for both (the kernels take one row stride): the caches'
+    # own tables are widened once, where nothing else refers to them
     width = max(keys.max_pages, values.max_pages)
-    keys._widen(width)
-    values._widen(width)
+    for c in (keys, values):
+        if c.max_pages < width and not c.shared_tables():
+            c._widen(width)
     if Hq % Hkv:
         raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
     if rotation_matrix is not None and tuple(rotation_matrix.shape) != (d, d):
         raise ValueError(f"rotation matrix must be ({d}, {d}), got {tuple(rotation_matrix.shape)}")
     return Hkv
+
+
+def page_tables(keys: PagedPQCache, values: PagedPQCache):
+    """(keys' table, values' table, keys' sign table or None, pages per row) of a
+    checked pair, for one call: rows of one width. Where a narrower table is not
+    the cache's to replace (shared_tables), the call has a copy of its own."""
+    width = max(keys.max_pages, values.max_pages)
+
+    def wide(t):
+        return t if t is None or t.shape[1] == width else torch.nn.functional.pad(t, (0, width - t.shape[1]))
+
+    return wide(keys.table), wide(values.table), wide(keys.sign_table), width
 
 
 def check_signs(jl_rot, keys, d: int) -> None:
@@ -155,10 +169,11 @@ def _decode_paged(query, keys, values, rotation_matrix, scale, jl_rot, out_dtype
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    ktab, vtab, stab, max_pages = page_tables(keys, values)
     _lib.check(lib.pqkv_decode_attn_paged(
-        q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),
-        keys.page_tokens, keys.max_pages, keys.codebooks.data_ptr(),
-        values.codebooks.data_ptr(), keys.n_bits, keys.sign_table.data_ptr() if P is not None else None,
+        q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), ktab.data_ptr(), vtab.data_ptr(),
+        keys.page_tokens, max_pages, keys.codebooks.data_ptr(),
+        values.codebooks.data_ptr(), keys.n_bits, stab.data_ptr() if P is not None else None,
         _lib.ptr(P), d if P is not None else 0, B, Hq, Hkv, S, d, scale, out.data_ptr(), _lib.dtype_code(out_dtype),
         workspace.data_ptr(), workspace.numel(), _lib.stream_of(q)))
     return out
@@ -219,10 +234,11 @@ def decode_attention_weights(query: torch.Tensor, keys, values, rotation_matrix:
             ws.data_ptr(), ws.numel(), _lib.stream_of(q))
     with _lib.on_device(q):
         if paged:
+            ktab, vtab, stab, max_pages = page_tables(keys, values)
             _lib.check(lib.pqkv_decode_attn_weights_paged(
-                q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),
-                keys.page_tokens, keys.max_pages, kcb.data_ptr(), vcb.data_ptr(), keys.n_bits,
-                keys.sign_table.data_ptr() if P is not None else None, _lib.ptr(P), d if P is not None else 0, B, Hq,
+                q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), ktab.data_ptr(), vtab.data_ptr(),
+                keys.page_tokens, max_pages, kcb.data_ptr(), vcb.data_ptr(), keys.n_bits,
+                stab.data_ptr() if P is not None else None, _lib.ptr(P), d if P is not None else 0, B, Hq,
                 Hkv, S, d, scale, out.data_ptr(), _lib.dtype_code(out_dtype), *tail))
         else:
             _lib.check(lib.pqkv_decode_attn_weights(
@@ -375,10 +391,11 @@ def _prefill_paged(query, keys, values, rotation_matrix, q_start, causal, scale,
     ws = _lib.workspace(lib.pqkv_prefill_workspace_preferred_bytes(*shape, int(jl_rot is not None)),
                         lambda: lib.pqkv_prefill_workspace_bytes(*shape), q.device)
     P = None if jl_rot is None else jl_rot.to(torch.float32).contiguous()
+    ktab, vtab, stab, max_pages = page_tables(keys, values)
     _lib.check(lib.pqkv_prefill_attn_paged(
-        q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), keys.table.data_ptr(), values.table.data_ptr(),
-        keys.page_tokens, keys.max_pages, keys.codebooks.data_ptr(),
-        values.codebooks.data_ptr(), keys.n_bits, keys.sign_table.data_ptr() if P is not None else None,
+        q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr(), ktab.data_ptr(), vtab.data_ptr(),
+        keys.page_tokens, max_pages, keys.codebooks.data_ptr(),
+        values.codebooks.data_ptr(), keys.n_bits, stab.data_ptr() if P is not None else None,
         _lib.ptr(P), d if P is not None else 0, B, Hq, Hkv, Sq, q_start, S, d, scale, int(causal), out.data_ptr(),
         _lib.dtype_code(out_dtype), ws.data_ptr(), ws.numel(), _lib.stream_of(q)))
     return out

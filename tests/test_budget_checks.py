@@ -49,3 +49,39 @@ def test_projections_of_another_size(paged):
     for call in calls(kc, vc, torch.zeros(D, D)):
         with pytest.raises(ValueError, match="projections"):
             call()
+
+
+def adopted(width, pages):
+    c = PagedPQCache(1, 2, D, 4, torch.zeros(16), "cpu", 64, jl_dim=D)
+    table, signs = (torch.arange(2 * width).view(2, width) + o for o in (1000, 2000))
+    c.adopt(table, pages * 64, [], signs)
+    c.seq_len = 40
+    return c, table, signs
+
+
+@pytest.mark.parametrize("widths", [(2, 5), (5, 2)])
+def test_tables_of_the_caller_stay_the_callers(widths):
+    """What their owner writes into them later is what later calls read."""
+    (keys, kt, ks), (values, vt, _) = (adopted(w, 1) for w in widths)
+    attention.check_paged(1, 4, D, keys, values)
+    assert keys.table is kt and values.table is vt and keys.sign_table is ks
+    for _ in range(2):
+        k, v, s, n = attention.page_tables(keys, values)
+        assert n == 5 and all(t.shape == (2, 5) and t.is_contiguous() for t in (k, v, s))
+        assert torch.equal(k[:, :kt.shape[1]], kt) and torch.equal(v[:, :vt.shape[1]], vt)
+        assert torch.equal(s[:, :ks.shape[1]], ks)
+        kt[1, 1], vt[1, 1], ks[1, 1] = 77, 78, 79               # the owner's next page
+
+
+def test_tables_are_not_replaced_within_a_capture(monkeypatch):
+    keys, values = (PagedPQCache(1, 2, D, 4, torch.zeros(16), "cpu", 64, max_pages=n) for n in (3, 7))
+    for c in (keys, values):
+        c.ensure(100)
+        c.seq_len = 70
+    monkeypatch.setattr(PagedPQCache, "shared_tables", lambda self: True)
+    before = keys.table
+    attention.check_paged(1, 4, D, keys, values)
+    assert keys.table is before and attention.page_tables(keys, values)[0].shape == (2, 7)
+    monkeypatch.undo()
+    attention.check_paged(1, 4, D, keys, values)
+    assert keys.table.shape == (2, 7) and attention.page_tables(keys, values)[0] is keys.table
