@@ -405,9 +405,9 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * softmax(s)_t, arguments as pqkv_prefill_attn and pqkv_decode_attn_weights
  * (keys only: no values are read). Sq = 0 copies weights_in (or writes zeros);
  * S = 0 writes nothing. Groups Hq / Hkv of up to 1024, S < 2^24. The workspace
- * (qjl: with signs) needs no initialisation; past the rotated queries it stays
- * below 1 GB up to a thousand (batch, kv-head) streams (long chunks run in
- * passes). Queries on a 16-byte boundary are rotated on the way. */
+ * (qjl: with signs) needs no initialisation; past the rotated queries and their
+ * projections, which only signs need, it stays below 1 GB up to a thousand
+ * (batch, kv-head) streams (long chunks run in passes). */
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
                       int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,

@@ -68,8 +68,8 @@ int decode_weights_run(const void *q, int q_dtype, const float *R, const uint8_t
 }
 
 // One pass of a chunk's weights over `rows` rows of every stream, and its
-// workspace: rotated queries (and projections), the rows' records and factors,
-// the token blocks' partials, the rows' statistics, the row chunks' sums.
+// workspace: with QJL the rotated queries and their projections, the rows'
+// records and factors, the token blocks' partials, the rows' statistics, the row chunks' sums.
 struct WeightsPlan {
   int tokens, tblocks, rows, chunk_rows;
   size_t q, pq, records, factor, part, stat, col;
@@ -101,8 +101,8 @@ WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl)
   // of a long chunk short (with 2048 rows 32764 rows on 8191 tokens take 2 % more)
   const int64_t want = p.rows * streams * p.tblocks / 1024;
   p.chunk_rows = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, 128), 1024);
-  p.q = align256((size_t)B * Hq * Sq * d * 4);
-  p.pq = qjl ? p.q : 0;
+  p.q = qjl ? align256((size_t)B * Hq * Sq * d * 4) : 0;
+  p.pq = p.q;
   p.records = align256((size_t)streams * row_tiles(p.rows) * 16 * rec_row);
   p.factor = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float));
   p.part = align256((size_t)streams * p.tblocks * p.rows * sizeof(float2));
@@ -168,21 +168,19 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
   float *q32 = (float *)take(p.q), *pq32 = (float *)take(p.pq);
   const int64_t nvec = (int64_t)B * Hq * Sq;
   const float qs = scale * 1.4426950408889634f;
-  // the queries are rotated on their way into the rows' records where they can
-  // be read 16 bytes at a time and no projection needs them rotated, else before
-  const bool direct = !has_qjl && (uintptr_t)q % 16 == 0;
-  if (!direct) {
+  // the queries are rotated on their way into the rows' records, or before
+  // where projections need them rotated too
+  if (has_qjl) {
     const int t = pqkv::prof_begin("weights_rotate", st);
-    const hipError_t r = has_qjl ? pqkv::launch_rotate2(q, q_dtype, R, p_rot, q32, pq32, nvec, d, qs, 1.0f / (float)m, st)
-                                 : pqkv::launch_rotate(q, q_dtype, R, q32, PQKV_F32, nvec, d, 0, qs, st);
+    const hipError_t r = pqkv::launch_rotate2(q, q_dtype, R, p_rot, q32, pq32, nvec, d, qs, 1.0f / (float)m, st);
     pqkv::prof_end(t, st);
     if (r != hipSuccess) return report_hip_error(r, "attn_weights query rotation");
   }
   pqkv::AttnWeightsArgs a;
   memset(&a, 0, sizeof(a));
-  a.q = direct ? nullptr : q32;
+  a.q = has_qjl ? q32 : nullptr;
   a.pq = has_qjl ? pq32 : nullptr;
-  a.x = direct ? q : nullptr;
+  a.x = q;
   a.x_dtype = q_dtype;
   a.R = R;
   a.q_scale = qs;

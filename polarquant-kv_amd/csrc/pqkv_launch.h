@@ -382,9 +382,9 @@ hipError_t launch_prefill_merge(const PrefillArgs &a, int stream0, int ns, int r
 // Weights of a chunk's rows (pqkv_attn_weights): row i * G + g of stream
 // (b, kv head) is query token i of the group's head g.
 struct AttnWeightsArgs {
-  const float *q, *pq;           // [B][Hq][Sq][d] fp32, rotated, times scale*log2(e); projections (QJL) or null
-  const void *x;                 // or (q null) the queries as they are, on a 16-byte boundary, in x_dtype,
-  int x_dtype;                   // to be rotated by R and scaled by q_scale
+  const float *q, *pq;           // with QJL: [B][Hq][Sq][d] fp32, rotated, times scale*log2(e); projections
+  const void *x;                 // without: the queries as they are, in x_dtype, to be rotated by R and
+  int x_dtype;                   // scaled by q_scale
   const float *R;
   float q_scale;
   const uint8_t *k_cache;        // [B][Hkv][S_max] vectors, or pages as in DecodeArgs

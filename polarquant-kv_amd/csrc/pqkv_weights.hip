@@ -228,10 +228,11 @@ __device__ __forceinline__ void put_row(uint8_t *rec, int j, int rl, const float
   }
 }
 
-// Rotated queries (and projections) -> records of 16 rows, and each row's
-// factor. Rows past the pass's last one are zeros.
-template <int D, bool QJL>
+// With QJL: rotated queries and projections -> records of 16 rows, and each
+// row's factor. Rows past the pass's last one are zeros.
+template <int D>
 __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernelArgs k) {
+  constexpr bool QJL = true;
   using Rec = RowRec<D, QJL>;
   __shared__ float most[D / 8][16];
   const AttnWeightsArgs &a = k.a;
@@ -239,11 +240,11 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
   const uint32_t tiles = (uint32_t)a.row_tiles;
   const int64_t stream = blockIdx.x / tiles;
   const int tile = (int)(blockIdx.x - (uint32_t)stream * tiles), r = tile * 16 + rl;
-  float x[QJL ? 2 : 1][8];
+  float x[2][8];
   float mx = 0.0f;
   const int64_t row = row_vector(k, stream, r);
 #pragma unroll
-  for (int p = 0; p < (QJL ? 2 : 1); ++p) {
+  for (int p = 0; p < 2; ++p) {
     const float *src = (p ? a.pq : a.q) + row * D + 8 * j;
     const float4 u = *(const float4 *)src, v = *(const float4 *)(src + 4);
     const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
@@ -261,14 +262,15 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
   put_row<D, QJL>(a.records + (stream * tiles + tile) * Rec::BYTES, j, rl, x, sh);
 }
 
-// The same from the queries themselves (a.x, rows on 16-byte boundaries, no
-// QJL): y = R x on the matrix cores, so that the rotated queries are never
+// Without QJL, from the queries themselves (a.x): y = R x on the matrix cores, so that the rotated queries are never
 // written. A = R, split hi / lo once per workgroup into registers (a wave's D /
 // 4 outputs), B = 16 queries as they lie in memory: fp16 queries are their own
-// high part (two products), fp32 ones are scaled and split (three).
+// high part (two products), fp32 ones are scaled and split (three). Queries off a
+// 16-byte boundary (ALIGNED false) are read in the pieces that their type's
+// alignment allows.
 // 32764 x 8 rows (d = 128): 58 us (200 MB, 3.5 TB/s) where rotating first (75)
-// and weights_rows_kernel (48) took 123.
-template <int D, typename T>
+// and making records of the result (48) took 123.
+template <int D, typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_rows_kernel(const WeightsKernelArgs k, uint32_t n_tiles) {
   using Rec = RowRec<D, false>;
   constexpr int KS = D / 32, OT = D / 64;          // outputs of a wave: OT tiles of 16
@@ -309,6 +311,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_ro
     float undo;
   };
   const uint32_t tiles = (uint32_t)a.row_tiles;
+  auto read = [&](const T *src, auto &to) {   // 16 bytes
+    if constexpr (ALIGNED) to = *(const std::remove_reference_t<decltype(to)> *)src;
+    else __builtin_memcpy(&to, src, 16);
+  };
   auto load = [&](uint32_t n) {
     Operand o;
     const int64_t stream = n / tiles;
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_ro
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          u[ks][p] = *(const float4 *)(src + 32 * ks + 4 * p);
+          read(src + 32 * ks + 4 * p, u[ks][p]);
           mx = fmaxf(fmaxf(fmaxf(mx, fabsf(u[ks][p].x)), fmaxf(fabsf(u[ks][p].y), fabsf(u[ks][p].z))), fabsf(u[ks][p].w));
         }
       const int sh = scale_exponent(rows4_max(mx), 100);
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) weights_rotate_ro
       }
     } else {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) o.h[ks] = *(const half8_t *)(src + 32 * ks);
+      for (int ks = 0; ks < KS; ++ks) read(src + 32 * ks, o.h[ks]);
     }
     return o;
   };
@@ -738,12 +744,19 @@ void launch_passes(const AttnWeightsArgs &a, int64_t streams, hipStream_t s) {
   if (groups % 8 == 0 || groups >= 64) k.xcd_groups = (int)groups;
   const unsigned grid = (unsigned)((k.xcd_groups ? (groups + 7) / 8 * 8 : groups) * a.tblocks);
   const uint32_t tiles = (uint32_t)(streams * a.row_tiles);
-  if (!QJL && a.x != nullptr) {
-    const unsigned blocks = tiles < 1024 ? tiles : 1024;   // (each reads R once)
-    if (a.x_dtype == PQKV_F16) weights_rotate_rows_kernel<D, half_t><<<blocks, 256, 0, s>>>(k, tiles);
-    else weights_rotate_rows_kernel<D, float><<<blocks, 256, 0, s>>>(k, tiles);
+  if constexpr (QJL) {
+    weights_rows_kernel<D><<<tiles, 2 * D, 0, s>>>(k);
   } else {
-    weights_rows_kernel<D, QJL><<<tiles, 2 * D, 0, s>>>(k);
+    const unsigned blocks = tiles < 1024 ? tiles : 1024;   // (each reads R once)
+    auto rotate = [&](auto t, auto aligned) {
+      weights_rotate_rows_kernel<D, decltype(t), decltype(aligned)::value><<<blocks, 256, 0, s>>>(k, tiles);
+    };
+    auto typed = [&](auto t) {
+      if ((uintptr_t)a.x % 16 == 0) rotate(t, std::true_type{});
+      else rotate(t, std::false_type{});
+    };
+    if (a.x_dtype == PQKV_F16) typed(half_t{});
+    else typed(float{});
   }
   attn_weights_kernel<D, QJL, TT, true><<<grid, 64 * kWW, 0, s>>>(k);
   // few rows of many blocks: more threads per row (128 rows x 8 streams of 1024 blocks 11 us -> 6)

@@ -1,0 +1,22 @@
+"""How large the workspaces of a cache under a budget are; no GPU."""
+
+import pytest
+
+from polarquant_kv import _lib
+
+
+def weights(B, Hq, Hkv, Sq, S, d, qjl):
+    return _lib.lib().pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d, qjl)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,S,d", [(1, 32, 8, 8191, 8191, 128), (8, 32, 8, 8192, 131072, 128),
+                                             (1, 64, 8, 32768, 32768, 128), (64, 14, 2, 4096, 4096, 64)])
+def test_rotated_queries_have_room_only_with_signs(B, Hq, Hkv, Sq, S, d):
+    """Without signs the queries are rotated on their way into the rows'
+    records, whose room (two halves of 2 bytes a coordinate, in passes of at most
+    512 MB) grows no further with the chunk."""
+    rotated = B * Hq * Sq * d * 4
+    plain, signed = weights(B, Hq, Hkv, Sq, S, d, 0), weights(B, Hq, Hkv, Sq, S, d, 1)
+    assert plain < min(1 << 30, 2 * rotated + (256 << 20))
+    assert 2 * rotated < signed < 2 * rotated + (1 << 30)
+    assert weights(4 * B, Hq, Hkv, 4 * Sq, S, d, 0) < 1 << 30
