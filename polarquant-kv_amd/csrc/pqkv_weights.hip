@@ -76,11 +76,12 @@ __device__ __forceinline__ void decode_weights_body(float2 *ml, const DecodeArgs
     for (int sp = lane; sp < a.split_stride; sp += 64) mx = fmaxf(mx, p[(int64_t)sp * (a.d + 2)]);
     mx = wave_max(mx);
     for (int sp = lane; sp < a.split_stride; sp += 64) {
-      const float m = p[(int64_t)sp * (a.d + 2)];
-      if (m != -INFINITY) L = __builtin_fmaf(__builtin_amdgcn_exp2f(m - mx), p[(int64_t)sp * (a.d + 2) + 1], L);
+      // (a split without a number to its maximum has the sum NaN, which stays)
+      const float m = p[(int64_t)sp * (a.d + 2)], e = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+      L = __builtin_fmaf(e, p[(int64_t)sp * (a.d + 2) + 1], L);
     }
     L = wave_sum(L);
-    if (lane == 0) ml[g] = make_float2(mx, L > 0.0f ? 1.0f / L : 0.0f);
+    if (lane == 0) ml[g] = make_float2(mx, L == 0.0f ? 0.0f : 1.0f / L);
   }
   __syncthreads();
   if (!there) return;

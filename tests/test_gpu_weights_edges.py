@@ -28,3 +28,65 @@ def test_queries_off_a_16_byte_boundary(dtype, d, qjl):
         moved.copy_(q)
         assert moved.data_ptr() % 16 != 0 and moved.is_contiguous()
         assert torch.equal(attention.attention_weights(moved, kc, R, 230, jl_rot=jl), at_home)
+
+
+def spoil(cache, b, h, t, value):
+    cache.blocks[b, h, t].view(-1, 18)[:, :2] = torch.tensor([value], device=DEV).half().view(torch.uint8)
+
+
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("S,at", [(65, 64), (65, 3), (1000, 999), (1000, 500), (4097, 4096), (1, 0)])
+@pytest.mark.parametrize("paged", [False, True])
+def test_decode_weights_with_a_key_that_is_not_a_number(S, at, paged):
+    """One NaN logit makes all weights of its rows NaN, wherever it stands among
+    the splits, and no others."""
+    q, kc, vc, R, _ = make(2, 14, 2, S, 128, 4, False)
+    _, clean = attention.decode_attention_weights(q, kc, vc, R)
+    spoil(kc, 1, 0, at, NAN)
+    k, v = (paged_copy(c, 64) if paged else c for c in (kc, vc))
+    out, w = attention.decode_attention_weights(q, k, v, R)
+    assert bool(torch.isnan(w[1, 0]).all()) and bool(torch.isnan(out[1, :7]).all())
+    keep = torch.ones(2, 2, dtype=torch.bool, device=DEV)
+    keep[1, 0] = False
+    assert torch.equal(w[keep], clean[keep]) and bool(torch.isfinite(out[0]).all() and torch.isfinite(out[1, 7:]).all())
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_decode_weights_with_a_query_that_is_not_a_number(value):
+    q, kc, vc, R, _ = make(2, 8, 2, 900, 64, 4, False)
+    _, clean = attention.decode_attention_weights(q, kc, vc, R)
+    q[0, 5, 17] = value
+    _, w = attention.decode_attention_weights(q, kc, vc, R)
+    assert bool(torch.isnan(w[0, 1]).all())
+    assert torch.equal(w[0, 0], clean[0, 0]) and torch.equal(w[1], clean[1])
+
+
+@pytest.mark.parametrize("heads", [9, 11, 13, 17])
+def test_groups_that_divide_into_uneven_launches(heads):
+    q, kc, vc, R, _ = make(1, 2 * heads, 2, 700, 128, 4, False)
+    want, tol, _ = exact(q.unsqueeze(2), kc, R)
+    out, w = attention.decode_attention_weights(q, kc, vc, R)
+    close(w, want, tol)
+    assert torch.equal(out, attention.decode_attention(q, kc, vc, R))
+
+
+def test_callers_page_tables_of_different_widths():
+    """The caller's tables are read as they are at each call."""
+    q, kc, vc, R, _ = make(1, 4, 2, 150, 64, 4, False)
+    want, w = attention.decode_attention_weights(q, kc, vc, R)
+    kp, vp = paged_copy(kc, 64), paged_copy(vc, 64)
+    wide = torch.nn.functional.pad(vp.table, (0, 5))
+    vp.adopt(wide, vp.capacity, vp._adopted[1])
+    vp.seq_len = 150
+    narrow = kp.table
+    for i in range(2):
+        out, got = attention.decode_attention_weights(q, kp, vp, R)
+        assert torch.equal(out, want) and torch.equal(got, w) and kp.table is narrow and vp.table is wide
+        assert torch.equal(attention.decode_attention(q, kp, vp, R), want)
+        a, b = (attention.prefill_attention(q.unsqueeze(2), k, v, R, 149) for k, v in ((kp, vp), (kc, vc)))
+        assert torch.equal(a, b)
+        moved = torch.cat([g.reshape(-1) for g in kp._adopted[1]])         # the owner moves its pages
+        narrow += moved.data_ptr() - kp._adopted[1][0].data_ptr()
+        kp._adopted = (kp._adopted[0], [moved.view_as(kp._adopted[1][0])])
