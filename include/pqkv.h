@@ -404,7 +404,10 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * weights_in[b][h][t] + sum over kv head h's query heads and the Sq tokens of
  * softmax(s)_t, arguments as pqkv_prefill_attn and pqkv_decode_attn_weights
  * (keys only: no values are read). Sq = 0 copies weights_in (or writes zeros);
- * S = 0 writes nothing. Groups Hq / Hkv of up to 1024, S < 2^24. The workspace
+ * S = 0 writes nothing. A row with a logit that is not a number gives NaN to
+ * every position that it sees and nothing to the others; what stands at
+ * positions that no row sees is of no effect. Groups Hq / Hkv of up to 1024,
+ * S < 2^24. The workspace
  * (qjl: with signs) needs no initialisation; past the rotated queries and their
  * projections, which only signs need, it stays below 1 GB up to a thousand
  * (batch, kv-head) streams (long chunks run in passes). */

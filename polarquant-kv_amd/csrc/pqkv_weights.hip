@@ -591,9 +591,12 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float f = info.f[rt] * kundo;
-      int last = a.S - 1;   // the last token the lane's row sees
-      if (kMasked && a.causal)
-        last = min(last, a.q_start + (int)k.group.div((uint32_t)(kStage * s + 16 * rt + col + a.row0)));
+      int last = a.S - 1;   // the last token the lane's row sees; none where the pass has no such row
+      if (kMasked) {
+        const int r = kStage * s + 16 * rt + col;
+        if (a.causal) last = min(last, a.q_start + (int)k.group.div((uint32_t)(r + a.row0)));
+        if (r >= a.rows) last = -1;
+      }
       const int rel = last - tw0 - 4 * grp;
       if constexpr (STATS) {
         float m = -INFINITY;
@@ -618,14 +621,16 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], f, -info.x[rt].x));
-            if (kMasked && 16 * tt + i > rel) e = 0.0f;
-            csum[tt][i] = __builtin_fmaf(e, info.x[rt].y, csum[tt][i]);
+            // (the whole term is dropped: a row that is not a number has 1 / L = NaN)
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][tt][i], f, -info.x[rt].x));
+            const float with = __builtin_fmaf(e, info.x[rt].y, csum[tt][i]);
+            csum[tt][i] = kMasked && 16 * tt + i > rel ? csum[tt][i] : with;
           }
       }
     }
   };
-  // STATS: the four waves' statistics of stage s, joined and written
+  // STATS: the four waves' statistics of stage s, joined and written (a maximum
+  // of -inf has the sum 0, or NaN where all its logits are that, which stays)
   auto write_stats = [&](int s) {
     const int r = kStage * s + lane;
     if (wave != (s & (kWW - 1)) || lane >= kStage || r < r_begin || r >= r_end) return;
@@ -635,7 +640,7 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
 #pragma unroll
     for (int w = 0; w < kWW; ++w) {
       const float2 x = st[s & 1][w][lane];
-      if (x.x != -INFINITY) l = __builtin_fmaf(x.y, __builtin_amdgcn_exp2f(x.x - m), l);
+      l = __builtin_fmaf(x.y, x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - m), l);
     }
     a.part[(stream * a.tblocks + tb) * a.rows + r] = make_float2(m, l);
   };
@@ -696,9 +701,8 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const WeightsKernelArgs
   const float2 *p = a.part + stream * a.tblocks * a.rows + rr;
   float m = -INFINITY, l = 0.0f;
   auto join = [&](float2 x) {
-    const float mn = fmaxf(m, x.x);
-    if (mn == -INFINITY) return;
-    l = l * __builtin_amdgcn_exp2f(m - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
+    const float mn = fmaxf(m, x.x), ref = mn == -INFINITY ? 0.0f : mn;   // (no maximum: sums of 0, or NaN)
+    l = l * __builtin_amdgcn_exp2f(m - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
     m = mn;
   };
 #pragma unroll 8

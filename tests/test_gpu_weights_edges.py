@@ -30,6 +30,26 @@ def test_queries_off_a_16_byte_boundary(dtype, d, qjl):
         assert torch.equal(attention.attention_weights(moved, kc, R, 230, jl_rot=jl), at_home)
 
 
+def visible64(q, kc, R, q_start, causal=True):
+    """[B, Hkv, S] float64: each row's softmax over the positions that it sees, and
+    nothing from it for the others, whatever it holds."""
+    B, Hq, Sq, d = q.shape
+    H, S = kc.num_heads, kc.seq_len
+    x = (q.double() @ R.double().t() * d ** -0.5) @ decoded(kc).repeat_interleave(Hq // H, 1).transpose(2, 3)
+    seen = torch.ones(Sq, S, dtype=torch.bool, device=DEV)
+    if causal:
+        seen = torch.arange(S, device=DEV) <= torch.arange(q_start, q_start + Sq, device=DEV)[:, None]
+    w = torch.softmax(x.masked_fill(~seen, float("-inf")), -1).masked_fill(~seen, 0.0)
+    return w.view(B, H, -1, S).sum(2)
+
+
+def same(got, want, rel):
+    """NaN in the same places; near elsewhere."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), (torch.isnan(got).sum(), torch.isnan(want).sum())
+    a, b = torch.nan_to_num(got.double()), torch.nan_to_num(want)
+    assert bool(((a - b).abs() <= rel * b + 1e-37).all()), ((a - b).abs() - rel * b).max().item()
+
+
 def spoil(cache, b, h, t, value):
     cache.blocks[b, h, t].view(-1, 18)[:, :2] = torch.tensor([value], device=DEV).half().view(torch.uint8)
 
@@ -90,3 +110,48 @@ def test_callers_page_tables_of_different_widths():
         moved = torch.cat([g.reshape(-1) for g in kp._adopted[1]])         # the owner moves its pages
         narrow += moved.data_ptr() - kp._adopted[1][0].data_ptr()
         kp._adopted = (kp._adopted[0], [moved.view_as(kp._adopted[1][0])])
+
+
+CHUNKS = [
+    # Hq, Hkv, Sq, q_start, S, d
+    (4, 2, 33, 0, 33, 64), (14, 2, 65, 190, 255, 128), (8, 8, 16, 113, 129, 64), (12, 4, 40, 100, 600, 128),
+    (2, 1, 1100, 100, 1200, 64), (32, 8, 300, 700, 1000, 128),
+]
+
+
+@pytest.mark.parametrize("case", CHUNKS, ids=["Hq{}_Hkv{}_Sq{}_at{}_S{}_d{}".format(*c) for c in CHUNKS])
+def test_chunk_weights_with_a_key_that_is_not_a_number(case):
+    Hq, Hkv, Sq, q_start, S, d = case
+    q, kc, _, R, _ = make(2, Hq, Hkv, S, d, 4, False, Sq=Sq)
+    total, tol, _ = exact(q, kc, R, q_start, causal=False)
+    rel = (tol / total).max()                                    # one factor bounds every element's error
+    clean = attention.attention_weights(q, kc, R, q_start)
+    end = q_start + Sq
+    places = {0, q_start, end - 1, end - 2, min(end // 2 + 1, end - 1)} | {t for t in (end, end + 3, end + 40, S - 1) if t < S}
+    for at in sorted(places):
+        other = make(2, Hq, Hkv, S, d, 4, False, Sq=Sq)[1]
+        spoil(other, 1, Hkv - 1, at, NAN)
+        got = attention.attention_weights(q, other, R, q_start)
+        same(got, visible64(q, other, R, q_start), rel)
+        if at >= end:                                            # no row sees it
+            assert torch.equal(got, clean)
+        got = attention.attention_weights(q, other, R, q_start, causal=False)
+        same(got, visible64(q, other, R, q_start, False), rel)
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+@pytest.mark.parametrize("case", CHUNKS, ids=["Hq{}_Hkv{}_Sq{}_at{}_S{}_d{}".format(*c) for c in CHUNKS])
+def test_chunk_weights_with_a_query_that_is_not_a_number(case, value):
+    """A row that is not a number spoils the positions that it sees and no others."""
+    Hq, Hkv, Sq, q_start, S, d = case
+    q, kc, _, R, _ = make(2, Hq, Hkv, S, d, 4, False, Sq=Sq)
+    total, tol, _ = exact(q, kc, R, q_start, causal=False)
+    rel = (tol / total).max()
+    for row in sorted({0, Sq // 2, Sq - 1}):
+        broken = q.clone()
+        broken[1, Hq - 1, row, 5] = value
+        got = attention.attention_weights(broken, kc, R, q_start)
+        assert bool(torch.isnan(got[1, Hkv - 1, :q_start + row + 1]).all())
+        assert not torch.isnan(got[1, Hkv - 1, q_start + row + 1:]).any()
+        same(got, visible64(broken, kc, R, q_start), rel)
+        assert bool(torch.isnan(attention.attention_weights(broken, kc, R, q_start, causal=False)[1, Hkv - 1]).all())
