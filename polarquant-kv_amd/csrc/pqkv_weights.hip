@@ -453,7 +453,9 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
   copy_stage(s0, (lds_u8 *)qb[s0 & 1]);
 
   // ---- this wave's keys, 16 TT tokens: lane (col, grp) holds coordinates
-  // 32 ks + 8 grp .. + 7 of token 16 tt + col ----
+  // 32 ks + 8 grp .. + 7 of token 16 tt + col; those that no row of the pass sees
+  // are zeros, so that they neither set the block's scale nor meet padding rows ----
+  const int seen = a.causal ? min(a.S, a.q_start + (int)k.group.div((uint32_t)(a.rows - 1 + a.row0)) + 1) : a.S;
   const int vb = vector_bytes(D, a.bits);
   const uint8_t *kv[TT], *sv[TT];
   float radius[TT], rmax = 0.0f;
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
       sv[tt] = QJL ? a.qjl + (stream * a.S_max + t) * (D / 8) : nullptr;
     }
     const float r = half_bits_to_float(*(const uint16_t *)kv[tt]);
-    radius[tt] = tw0 + 16 * tt + col < a.S ? r : 0.0f;
+    radius[tt] = tw0 + 16 * tt + col < seen ? r : 0.0f;
     rmax = fmaxf(rmax, fabsf(radius[tt]));
   }
   uint32_t code[TT][KS];
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
         __builtin_memcpy(&w[i], sv[tt] + 4 * i, 4);
         ones = ones && w[i] == 0xFFFFFFFFu;
       }
-      const half_t one = (half_t)(ones || tw0 + 16 * tt + col >= a.S ? 0.0f : kscale);
+      const half_t one = (half_t)(ones || tw0 + 16 * tt + col >= seen ? 0.0f : kscale);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -591,12 +593,9 @@ __global__ void __launch_bounds__(64 * kWW, QJL || TT == 4 ? 2 : 3) attn_weights
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float f = info.f[rt] * kundo;
-      int last = a.S - 1;   // the last token the lane's row sees; none where the pass has no such row
-      if (kMasked) {
-        const int r = kStage * s + 16 * rt + col;
-        if (a.causal) last = min(last, a.q_start + (int)k.group.div((uint32_t)(r + a.row0)));
-        if (r >= a.rows) last = -1;
-      }
+      int last = a.S - 1;   // the last token the lane's row sees
+      if (kMasked && a.causal)
+        last = min(last, a.q_start + (int)k.group.div((uint32_t)(kStage * s + 16 * rt + col + a.row0)));
       const int rel = last - tw0 - 4 * grp;
       if constexpr (STATS) {
         float m = -INFINITY;

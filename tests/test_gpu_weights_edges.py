@@ -155,3 +155,16 @@ def test_chunk_weights_with_a_query_that_is_not_a_number(case, value):
         assert not torch.isnan(got[1, Hkv - 1, q_start + row + 1:]).any()
         same(got, visible64(broken, kc, R, q_start), rel)
         assert bool(torch.isnan(attention.attention_weights(broken, kc, R, q_start, causal=False)[1, Hkv - 1]).all())
+
+
+@pytest.mark.parametrize("value", [NAN, INF, 60000.0])
+@pytest.mark.parametrize("qjl", [False, True])
+def test_chunk_weights_do_not_depend_on_keys_that_no_row_sees(value, qjl):
+    """Later positions in the same block of tokens: equal, not near."""
+    q, kc, _, R, jl = make(2, 12, 4, 600, 128, 4, qjl, Sq=43)
+    clean = attention.attention_weights(q, kc, R, 100, jl_rot=jl)
+    for at in (143, 144, 150, 255, 256, 599):
+        _, other, _, _, _ = make(2, 12, 4, 600, 128, 4, qjl, Sq=43)
+        for h in range(4):
+            spoil(other, 1, h, at, value)
+        assert torch.equal(attention.attention_weights(q, other, R, 100, jl_rot=jl), clean)
