@@ -407,10 +407,10 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * S = 0 writes nothing. A row with a logit that is not a number gives NaN to
  * every position that it sees and nothing to the others; what stands at
  * positions that no row sees is of no effect. Groups Hq / Hkv of up to 1024,
- * S < 2^24. The workspace
- * (qjl: with signs) needs no initialisation; past the rotated queries and their
- * projections, which only signs need, it stays below 1 GB up to a thousand
- * (batch, kv-head) streams (long chunks run in passes). */
+ * S < 2^24. The workspace (qjl: with signs) needs no initialisation; past the
+ * rotated queries and their projections, which only signs need, it stays below
+ * 1 GB + 4 bytes per position and 128 KB per (batch, kv-head) stream, however
+ * long the chunk (long ones run in passes). */
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
                       int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,

@@ -89,7 +89,8 @@ WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl)
   const int64_t streams = (int64_t)B * Hkv, total = (int64_t)Sq * (Hq / Hkv);
   p.tokens = qjl || total <= kFewRows ? 128 : 256;
   p.tblocks = (S + p.tokens - 1) / p.tokens;
-  // rows of a pass: partials within 256 MB, records within 512 MB
+  // rows of a pass: partials within 256 MB, records within 512 MB, but 64 rows
+  // at least, whose partials are 4 bytes per position
   const int64_t rec_row = (int64_t)d * (qjl ? 8 : 4);
   int64_t rows = std::min((int64_t)(256 << 20) / (streams * p.tblocks * (int64_t)sizeof(float2)),
                           (int64_t)(512 << 20) / (streams * rec_row));
@@ -107,7 +108,9 @@ WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl)
   p.factor = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float));
   p.part = align256((size_t)streams * p.tblocks * p.rows * sizeof(float2));
   p.stat = align256((size_t)streams * row_tiles(p.rows) * 16 * sizeof(float2));
-  p.col = align256((size_t)streams * p.chunks(p.rows) * p.tblocks * p.tokens * sizeof(float));
+  // (one chunk's sums are the result: no room for them)
+  const int chunks = p.chunks(p.rows);
+  p.col = chunks > 1 ? align256((size_t)streams * chunks * p.tblocks * p.tokens * sizeof(float)) : 0;
   return p;
 }
 

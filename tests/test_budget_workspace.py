@@ -20,3 +20,16 @@ def test_rotated_queries_have_room_only_with_signs(B, Hq, Hkv, Sq, S, d):
     assert plain < min(1 << 30, 2 * rotated + (256 << 20))
     assert 2 * rotated < signed < 2 * rotated + (1 << 30)
     assert weights(4 * B, Hq, Hkv, 4 * Sq, S, d, 0) < 1 << 30
+
+
+@pytest.mark.parametrize("qjl", [0, 1])
+@pytest.mark.parametrize("B,Hq,Hkv", [(1, 1, 1), (1, 64, 1), (4, 32, 8), (64, 32, 8), (128, 32, 8), (400, 14, 2)])
+def test_bound_past_the_rotated_queries(B, Hq, Hkv, qjl):
+    streams = B * Hkv
+    for Sq in (1, 32, 257, 8192):
+        for S in (1, 127, 8191, 131072, 1048576):
+            for d in (64, 128):
+                n = weights(B, Hq, Hkv, Sq, S, d, qjl)
+                assert n > 0 or streams * -(-S // 128) > 1 << 24
+                rotated = 2 * qjl * (B * Hq * Sq * d * 4 + 256)
+                assert n <= rotated + (1 << 30) + streams * (4 * S + (128 << 10)), (Sq, S, d, n)
