@@ -410,8 +410,10 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * S < 2^24. The workspace (qjl: with signs) needs no initialisation; past the
  * rotated queries and their projections, which only signs need, it stays below
  * 1 GB + 4 bytes per position and 128 KB per (batch, kv-head) stream, however
- * long the chunk (long ones run in passes). */
+ * long the chunk (long ones run in passes). A smaller workspace, of _least_bytes
+ * and more, is taken too: with passes of fewer rows, which takes longer. */
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
+size_t pqkv_attn_weights_workspace_least_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,
                       int n_bits, const uint8_t *qjl_signs, const float *p_rot, int m,
                       int B, int Hq, int Hkv, int Sq, int q_start, int S, int S_max, int d, float scale, int causal,

@@ -84,7 +84,9 @@ struct WeightsPlan {
 // 8191 tokens, 1.39 ms, take 4 % more with 128).
 constexpr int kFewRows = 2048;
 int row_tiles(int rows) { return (rows + 63) / 64 * 4; }
-WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl) {
+// shrink: passes of 2^-shrink times the rows, for less room.
+constexpr int kMaxShrink = 4;
+WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl, int shrink = 0) {
   WeightsPlan p;
   const int64_t streams = (int64_t)B * Hkv, total = (int64_t)Sq * (Hq / Hkv);
   p.tokens = qjl || total <= kFewRows ? 128 : 256;
@@ -92,8 +94,8 @@ WeightsPlan weights_plan(int B, int Hq, int Hkv, int Sq, int S, int d, bool qjl)
   // rows of a pass: partials within 256 MB, records within 512 MB, but 64 rows
   // at least, whose partials are 4 bytes per position
   const int64_t rec_row = (int64_t)d * (qjl ? 8 : 4);
-  int64_t rows = std::min((int64_t)(256 << 20) / (streams * p.tblocks * (int64_t)sizeof(float2)),
-                          (int64_t)(512 << 20) / (streams * rec_row));
+  int64_t rows = std::min((int64_t)(256 << 20 >> shrink) / (streams * p.tblocks * (int64_t)sizeof(float2)),
+                          (int64_t)(512 << 20 >> shrink) / (streams * rec_row));
   rows = std::max<int64_t>(rows / 64 * 64, 64);
   p.rows = (int)std::min(rows, total);
   // rows of a workgroup: about 1024 workgroups; at least 128 rows, under which
@@ -158,7 +160,9 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
     return fail_status(PQKV_ERR_INVALID, "attn_weights: null pointer");
   if ((uintptr_t)R % 16 || (uintptr_t)p_rot % 16)
     return fail_status(PQKV_ERR_INVALID, "attn_weights: R and p_rot must be 16-byte aligned");
-  const WeightsPlan p = weights_plan(B, Hq, Hkv, Sq, S, d, has_qjl);
+  WeightsPlan p = weights_plan(B, Hq, Hkv, Sq, S, d, has_qjl);
+  for (int shrink = 1; shrink <= kMaxShrink && ws_bytes < p.bytes(); ++shrink)
+    p = weights_plan(B, Hq, Hkv, Sq, S, d, has_qjl, shrink);
   if (!ws || ws_bytes < p.bytes())
     return fail_status(PQKV_ERR_WORKSPACE, "attn_weights: workspace %zu < %zu bytes", ws_bytes, p.bytes());
   if ((uintptr_t)ws % 16) return fail_status(PQKV_ERR_INVALID, "attn_weights: workspace must be 16-byte aligned");
@@ -272,6 +276,11 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R, c
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl) {
   if (!weights_shape_ok(B, Hq, Hkv, Sq, S, d)) return 0;
   return weights_plan(B, Hq, Hkv, Sq, S, d, qjl != 0).bytes();
+}
+
+size_t pqkv_attn_weights_workspace_least_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl) {
+  if (!weights_shape_ok(B, Hq, Hkv, Sq, S, d)) return 0;
+  return weights_plan(B, Hq, Hkv, Sq, S, d, qjl != 0, kMaxShrink).bytes();
 }
 
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,

@@ -121,6 +121,7 @@ SIGNATURES = {
                                                c_int, c_float, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64,
                                                c_void_p, c_size_t, c_void_p]),
     "pqkv_attn_weights_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "pqkv_attn_weights_workspace_least_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "pqkv_attn_weights": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                   c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),

@@ -274,8 +274,9 @@ def attention_weights(query: torch.Tensor, keys, rotation_matrix: torch.Tensor, 
     q = query if query.is_contiguous() else query.contiguous()
     R, P = _lib.dense_f32(rotation_matrix), _lib.dense_f32(jl_rot)
     lib = _lib.lib()
-    ws = torch.empty(max(1, lib.pqkv_attn_weights_workspace_bytes(B, Hq, Hkv, Sq, S, d, int(P is not None))), dtype=torch.uint8,
-                     device=q.device)
+    shape = (B, Hq, Hkv, Sq, S, d, int(P is not None))
+    ws = _lib.workspace(lib.pqkv_attn_weights_workspace_bytes(*shape),
+                        lambda: lib.pqkv_attn_weights_workspace_least_bytes(*shape), q.device)
     tail = (scale, int(causal), _lib.ptr(previous), 0 if previous is None else _row_stride(previous), into.data_ptr(),
             _row_stride(into), ws.data_ptr(), ws.numel(), _lib.stream_of(q))
     head = (q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr())

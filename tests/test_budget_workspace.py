@@ -33,3 +33,25 @@ def test_bound_past_the_rotated_queries(B, Hq, Hkv, qjl):
                 assert n > 0 or streams * -(-S // 128) > 1 << 24
                 rotated = 2 * qjl * (B * Hq * Sq * d * 4 + 256)
                 assert n <= rotated + (1 << 30) + streams * (4 * S + (128 << 10)), (Sq, S, d, n)
+
+
+@pytest.mark.parametrize("qjl", [0, 1])
+def test_least_workspace(qjl):
+    """Smaller where the chunk can run in more passes; what is below it is refused
+    (and no address is read for that)."""
+    L, fake = _lib.lib(), 0x1000
+
+    def least(*a):
+        return L.pqkv_attn_weights_workspace_least_bytes(*a, qjl)
+
+    for a in ((1, 8, 2, 1, 1, 64), (1, 8, 2, 300, 1000, 128), (2, 14, 2, 65, 4096, 64), (8, 32, 8, 8192, 131072, 128),
+              (1, 64, 1, 600, 262144, 64)):
+        assert 0 < least(*a) <= weights(*a, qjl)
+        B, Hq, Hkv, Sq, S, d = a
+        for wsb in (0, least(*a) - 1):
+            assert L.pqkv_attn_weights(fake, 1, fake, fake, fake, 4, fake if qjl else None, fake if qjl else None,
+                                       d if qjl else 0, B, Hq, Hkv, Sq, S - Sq, S, S, d, 0.1, 1, None, 0, fake, S, fake, wsb,
+                                       None) == _lib.ERR_WORKSPACE
+    rotated = 2 * qjl * 8 * 32 * 8192 * 128 * 4
+    assert least(8, 32, 8, 8192, 131072, 128) - rotated < (weights(8, 32, 8, 8192, 131072, 128, qjl) - rotated) / 4
+    assert least(1, 8, 3, 4, 16, 128) == 0

@@ -6,6 +6,10 @@ import pytest
 import torch
 
 from polarquant_kv import _lib, attention
+from polarquant_kv.lloyd_max import padded_codebook_torch
+from polarquant_kv.qjl import generate_jl_matrix, rotated_jl_matrix
+from polarquant_kv.rotation import generate_rotation_matrix
+from polarquant_kv.types import PQCache
 
 from test_gpu_evict import paged_copy
 from test_gpu_weights import close, decoded, exact, make
@@ -168,3 +172,77 @@ def test_chunk_weights_do_not_depend_on_keys_that_no_row_sees(value, qjl):
         for h in range(4):
             spoil(other, 1, h, at, value)
         assert torch.equal(attention.attention_weights(q, other, R, 100, jl_rot=jl), clean)
+
+
+PASSES = [
+    # B, Hq, Hkv, Sq, q_start, d, qjl, rows of a pass with the least workspace
+    (4, 14, 2, 2400, 0, 64, False, 16384), (4, 14, 2, 2400, 37, 64, True, 8192), (8, 3, 1, 2800, 100, 128, True, 4096),
+]
+
+
+def rows_with_peaks(B, Hq, Hkv, Sq, q_start, d, qjl, rows, dev):
+    """Keys of one length in random directions; the first and last rows of each
+    pass of `rows` rows look at one key each, the others at all alike:
+    (queries, cache, R, jl_rot, [(row, its key)])."""
+    G, S = Hq // Hkv, q_start + Sq
+    assert G * Sq > rows and (rows % G or G == 1)
+    g = torch.Generator().manual_seed(rows)
+    blocks = torch.randint(0, 256, (B, Hkv, S, d // 32, 18), generator=g, dtype=torch.uint8)
+    blocks[..., :2] = torch.tensor([8.0]).half().view(torch.uint8)
+    signs = torch.randint(0, 256, (B, Hkv, S, d // 8), generator=g, dtype=torch.uint8).to(dev) if qjl else None
+    kc = PQCache(blocks=blocks.flatten(3).to(dev), head_dim=d, n_bits=4, seq_len=S, max_seq_len=S,
+                 codebooks=padded_codebook_torch(d, 4, dev), qjl_signs=signs, jl_dim=d if qjl else 0)
+    R = generate_rotation_matrix(d, seed=42, device=dev)
+    jl = rotated_jl_matrix(generate_jl_matrix(d, d, seed=43), R.cpu().numpy(), dev) if qjl else None
+    q = (0.25 * torch.randn(B, Hq, Sq, d, generator=g)).half().to(dev)
+    keys, peaks = decoded(kc), []
+    for edge in list(range(rows, G * Sq, rows)) + [G * Sq]:
+        for r in range(edge - 2, min(edge + 2, G * Sq)):
+            at = 5 + 17 * len(peaks)
+            assert at <= q_start + r // G                        # the row sees it
+            k = keys[:, :, at] @ R.double()                      # in the queries' space
+            q[:, r % G::G, r // G] = (14 * d ** 0.5 * k / k.square().sum(-1, keepdim=True)).half()
+            peaks.append((r, at))
+    return q, kc, R, jl, peaks
+
+
+@pytest.mark.parametrize("case", PASSES, ids=["B{}_Hq{}_Hkv{}_Sq{}_at{}_d{}_{}".format(*c[:6], "qjl" if c[6] else "plain")
+                                              for c in PASSES])
+def test_rows_at_the_border_of_two_passes(case, monkeypatch):
+    """Every row counts once."""
+    B, Hq, Hkv, Sq, q_start, d, qjl, rows = case
+    G, S = Hq // Hkv, q_start + Sq
+    q, kc, R, jl, peaks = rows_with_peaks(*case, DEV)
+    want, tol, w = exact(q, kc, R, q_start, jl_rot=jl)
+    w = w.view(B, Hkv, G, Sq, S)
+    for r, at in peaks:                                          # one lost or counted twice would be seen there
+        assert bool((w[:, :, r % G, r // G, at] > 2 * tol[:, :, at]).all())
+    del w
+    whole = attention.attention_weights(q, kc, R, q_start, jl_rot=jl)
+    close(whole, want, tol)
+    monkeypatch.setattr(_lib, "workspace", lambda best, least, device: torch.empty(least(), dtype=torch.uint8, device=device))
+    close(attention.attention_weights(q, kc, R, q_start, jl_rot=jl), want, tol)
+    previous = torch.rand(B, Hkv, S + 3, device=DEV)
+    into = previous.clone()
+    apart = attention.attention_weights(q, kc, R, q_start, jl_rot=jl, previous=previous)
+    attention.attention_weights(q, kc, R, q_start, jl_rot=jl, previous=into, into=into)
+    assert torch.equal(into[:, :, :S], apart) and torch.equal(into[:, :, S:], previous[:, :, S:])
+    # (each pass's addition to a sum of at most want + 1 rounds by half a step)
+    close(apart, want + previous[:, :, :S].double(), tol + 8 * (want + 1.0) * 2.0 ** -24)
+
+
+def test_no_room_for_the_workspace_of_one_pass(monkeypatch):
+    q, kc, _, R, _ = make(4, 14, 2, 2400, 64, 4, False, Sq=2400)
+    want, tol, _ = exact(q, kc, R, 0)
+    least, real, refused = _lib.lib().pqkv_attn_weights_workspace_least_bytes(4, 14, 2, 2400, 2400, 64, 0), torch.empty, []
+
+    def empty(*size, **kw):
+        if len(size) == 1 and size[0] > least:
+            refused.append(size[0])
+            raise torch.cuda.OutOfMemoryError("out of memory")
+        return real(*size, **kw)
+
+    monkeypatch.setattr(torch, "empty", empty)
+    got = attention.attention_weights(q, kc, R, 0)
+    assert refused
+    close(got, want, tol)
