@@ -10,12 +10,15 @@
 // the rank. Counts and indices are whole numbers, so no order of the atomic
 // additions changes the result. One workgroup per stream, its keys in registers
 // up to 65536 positions (KPT per thread), so that the weights are read once and
-// all their loads are in flight together (the thread counts below differ so that
-// at most half of the steps are empty); longer streams are read again in each
+// all their loads are in flight together; longer streams are read again in each
 // pass, from L2. Weights crowd into few exponents, so the first digit's
 // additions meet in few bins: there each bin has eight counters, a lane's by its
-// number. Bound by the instructions of one compute unit per stream: 21 us for 128
-// streams of 32768 positions, 13 for 32 of 16385, 6 for 2 of 1025.
+// number. Bound by the instructions of one compute unit per stream, which grow
+// with KPT, empty steps included (128 streams, launched one after the other: 11.6
+// us with 20, 13.0 with 24): KPT is the number of steps rounded up to a multiple of
+// four (2 where that is enough) up to 32768 positions, above, where few caches are,
+// to 48 or 64. 15.7 us for 128 streams of 32768 positions, 11.1 for 32 of 16385, 5.5
+// for 32 of 1025.
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
@@ -273,8 +276,10 @@ hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_s
   else if (steps <= 4) PQKV_SELECT(4);
   else if (steps <= 8) PQKV_SELECT(8);
   else if (steps <= 12) PQKV_SELECT(12);
-  else if (steps <= 18) PQKV_SELECT(18);
+  else if (steps <= 16) PQKV_SELECT(16);
+  else if (steps <= 20) PQKV_SELECT(20);
   else if (steps <= 24) PQKV_SELECT(24);
+  else if (steps <= 28) PQKV_SELECT(28);
   else if (steps <= 32) PQKV_SELECT(32);
   else if (steps <= 48) PQKV_SELECT(48);
   else if (steps <= 64) PQKV_SELECT(64);
