@@ -247,6 +247,13 @@ def on_device(t):
     return torch.cuda.device(t.device)
 
 
+def lasting():
+    """Context for making tensors that later calls write in whatever mode those
+    run: never inference tensors."""
+    import torch
+    return torch.inference_mode(False) if torch.is_inference_mode_enabled() else contextlib.nullcontext()
+
+
 def workspace(best: int, least, device):
     """A workspace of `best` bytes, the size a call is fastest with, or of
     least(), the smallest it takes, where the device has no room for that."""

@@ -44,7 +44,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import attention, quantizer
+from . import _lib, attention, quantizer
 from .types import PagedPQCache
 
 
@@ -109,7 +109,7 @@ class KVCacheManager:
             self._values = quantizer.allocate_paged_cache(B, H, d, bits, self.device, page_tokens=self.page_tokens)
         else:
             shape = (self.batch, self.num_heads, self.max_seq_len, self.head_dim)
-            with torch.inference_mode(False):   # written by later calls in whatever mode
+            with _lib.lasting():
                 self._key_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
                 self._value_cache = torch.zeros(shape, dtype=torch.float16, device=self.device)
 
@@ -194,14 +194,13 @@ class KVCacheManager:
         self._next_position += T
 
     def _track(self, T: int) -> None:
-        """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions.
-        (Not inference tensors: later calls write them in whatever mode.)"""
+        """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions."""
         S, need = self._seq_len, self._seq_len + T
         room = 0 if self._weights is None else self._weights.shape[2]
         if need > room:
             room = min(max(need, 2 * room, self.page_tokens), self.max_seq_len)
             shape = (self.batch, self.num_heads, room)
-            with torch.inference_mode(False):
+            with _lib.lasting():
                 w = torch.zeros(shape, dtype=torch.float32, device=self.device)
                 p = torch.zeros(shape, dtype=torch.int32, device=self.device)
             if S:
@@ -243,7 +242,7 @@ class KVCacheManager:
         if self._seq_len <= keep:
             return None
         from . import eviction
-        with torch.inference_mode(False):
+        with _lib.lasting():
             r = eviction.evict(self._keys, self._values, self._weights, keep, sink=sink, recent=recent,
                                positions=self._positions)
         self._keys, self._values, self._weights, self._positions = r.keys, r.values, r.weights, r.positions

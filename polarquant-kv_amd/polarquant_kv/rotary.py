@@ -128,6 +128,8 @@ def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):
 
 def _has_tangent(*tensors) -> bool:
     """Whether any of them carries a forward-mode derivative."""
+    if forward_ad._current_level < 0:          # (none is open: 0.1 us, where asking each tensor takes 1)
+        return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
@@ -135,9 +137,10 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse):
         ctx.save_for_backward(positions, freqs)
-        ctx.save_for_forward(positions, freqs)
         ctx.how = (interleaved, amplitude, not inverse)
-        ctx.shapes, ctx.dtype = (q.shape, None if k is None else k.shape), q.dtype
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, freqs)
+            ctx.shapes, ctx.dtype = (q.shape, None if k is None else k.shape), q.dtype
         ctx.set_materialize_grads(False)
         return _turn(q, k, positions, freqs, interleaved, amplitude, inverse)
 

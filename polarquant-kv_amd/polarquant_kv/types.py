@@ -15,6 +15,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass, field
 
+from . import _lib
+
 BLOCK = 32
 
 
@@ -103,11 +105,9 @@ class PagedPQCache:
         self.table, self.sign_table = self._new_tables(self.max_pages)
 
     def _new_tables(self, width: int):
-        """Zeroed page tables of `width` pages (the second None without signs).
-        Written again by later calls in whatever mode those run, so never
-        inference tensors."""
+        """Zeroed page tables of `width` pages (the second None without signs)."""
         import torch
-        with torch.inference_mode(False):
+        with _lib.lasting():
             t = torch.zeros(self.batch * self.num_heads, width, dtype=torch.int64, device=self.device)
             return t, torch.zeros_like(t) if self.jl_dim else None
 
@@ -211,7 +211,7 @@ class PagedPQCache:
         if n == 0:
             return []
         B, H = self.batch, self.num_heads
-        with torch.inference_mode(False):      # (as _new_tables)
+        with _lib.lasting():      # (as _new_tables)
             tables = torch.empty(2 if self.jl_dim else 1, B * H, n, dtype=torch.int64, device=self.device)
         self.table, self.max_pages = tables[0], n
         blocks = torch.empty(B, H, n, self.page_tokens, self.vector_bytes, dtype=torch.uint8, device=self.device)
