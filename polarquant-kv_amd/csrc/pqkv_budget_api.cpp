@@ -81,7 +81,7 @@ struct WeightsPlan {
 // larger part of the work (32 query / 8 kv heads, d = 128: 256 rows on 32768
 // tokens 129 us against 156, 2048 rows on 16512 tokens 384 against 411); with
 // more rows each operand read serves four tiles instead of two (32764 rows on
-// 8191 tokens, 1.39 ms, take 4 % more with 128).
+// 8191 tokens take 4 % more with 128).
 constexpr int kFewRows = 2048;
 int row_tiles(int rows) { return (rows + 63) / 64 * 4; }
 // shrink: passes of 2^-shrink times the rows, for less room.

@@ -14,11 +14,11 @@
 // pass, from L2. Weights crowd into few exponents, so the first digit's
 // additions meet in few bins: there each bin has eight counters, a lane's by its
 // number. Bound by the instructions of one compute unit per stream, which grow
-// with KPT, empty steps included (128 streams, launched one after the other: 11.6
-// us with 20, 13.0 with 24): KPT is the number of steps rounded up to a multiple of
-// four (2 where that is enough) up to 32768 positions, above, where few caches are,
-// to 48 or 64. 15.7 us for 128 streams of 32768 positions, 11.1 for 32 of 16385, 5.5
-// for 32 of 1025.
+// with KPT, empty steps included (128 streams of unequal weights: 11.6 us with 20,
+// 13.0 with 24): KPT is the number of steps rounded up to a multiple of four (2 where
+// that is enough) up to 32768 positions, above, where few caches are, to 48 or 64.
+// 15.7 us for 128 such streams of 32768 positions, 21 where a quarter of the weights
+// are zeros; 11 and 14 for 32 of 16385, 5.5 for 32 of 1025.
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 

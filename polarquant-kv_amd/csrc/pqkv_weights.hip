@@ -47,7 +47,7 @@ __device__ __forceinline__ float row16_sum(float x) {
 // Bound by those rows: 4 (G + 2) bytes per token and kv head. The same launch
 // joins the output's splits (decode_merge_body, the workgroups after them),
 // which needs nothing of the weights: a launch less. 8 sequences of 32768 tokens,
-// 32 query / 8 kv heads: 14 us for 50 MB.
+// 32 query / 8 kv heads: 13 us for 50 MB.
 constexpr int kDwTokens = 1024;
 
 template <bool VEC>
@@ -151,11 +151,13 @@ __global__ void __launch_bounds__(256) decode_merge_weights_kernel(const DecodeA
 // keys' power of two against the projections (two more products; +-0 where the
 // sketch is all ones, a zero residual).
 //
-// Bound by the matrix cores: 8191 tokens of 32 query / 8 kv heads (d = 128) on
-// themselves take 700-750 us per pass, 825 GFLOP of products each, 1.1-1.2
-// PFLOP/s (a library product of two 8192 x 8192 fp16 matrices reaches 1.13). With
-// few rows the decoding of the keys and the first loads of each workgroup weigh
-// more: 32 rows x 4 heads on 131072 tokens 128 and 150 us (103 GFLOP, 0.7-0.8).
+// Bound by the products: 8191 tokens of 32 query / 8 kv heads (d = 128) on
+// themselves take 700 and 680 us in the two passes, 825 GFLOP of products each, 1.2
+// PFLOP/s (a library product of two 8192 x 8192 fp16 matrices reaches 1.13; the
+// matrix cores are busy 55 % of the cycles, two other vector instructions stand
+// beside each product). With few rows the decoding of the keys and the first loads of
+// each workgroup weigh more: 32 rows x 4 heads on 131072 tokens 120 and 133 us (103
+// GFLOP, 0.8 PFLOP/s, 30 to 36 %).
 constexpr int kWW = 4;      // waves of a workgroup
 constexpr int kStage = 32;  // rows of a stage
 
