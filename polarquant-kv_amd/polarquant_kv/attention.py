@@ -78,11 +78,15 @@ def check_paged(B: int, Hq: int, d: int, keys: PagedPQCache, values: PagedPQCach
     for c in (keys, values):
         if c.capacity < c.seq_len:
             raise ValueError("paged cache holds fewer pages than its seq_len needs")
-    # one table width for both (the kernels take one row stride): the caches'
-    # own tables are widened once, where nothing else refers to them
+    # one table width for both (the kernels take one row stride): a cache's own
+    # table is replaced by a wider one, but not while a graph is captured (its
+    # entries would be there only after a replay, and the graph would read the old
+    # one, which a later call may replace)
     width = max(keys.max_pages, values.max_pages)
     for c in (keys, values):
-        if c.max_pages < width and not c.shared_tables():
+        if c.max_pages < width and not c.caller_managed:
+            if c.table.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("paged caches with tables of different widths: call once before a capture")
             c._widen(width)
     if Hq % Hkv:
         raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
@@ -93,8 +97,8 @@ def check_paged(B: int, Hq: int, d: int, keys: PagedPQCache, values: PagedPQCach
 
 def page_tables(keys: PagedPQCache, values: PagedPQCache):
     """(keys' table, values' table, keys' sign table or None, pages per row) of a
-    checked pair, for one call: rows of one width. Where a narrower table is not
-    the cache's to replace (shared_tables), the call has a copy of its own."""
+    checked pair, for one call: rows of one width. Where the narrower table is the
+    caller's, the call has a copy of its own."""
     width = max(keys.max_pages, values.max_pages)
 
     def wide(t):

@@ -152,13 +152,11 @@ class PagedPQCache:
     def head_bits(self) -> list:
         return [self.n_bits] * self.num_heads
 
-    def shared_tables(self) -> bool:
-        """Whether the tables may not be replaced by an attention call: they are
-        the caller's own (adopt: their owner may write further entries), or a
-        graph is being captured (the new ones would hold nothing before its
-        first replay)."""
-        import torch
-        return self._adopted is not None or (self.table.is_cuda and torch.cuda.is_current_stream_capturing())
+    @property
+    def caller_managed(self) -> bool:
+        """Whether pages and tables are the caller's own (adopt): their owner may
+        write further entries, so the tables are never replaced."""
+        return self._adopted is not None
 
     def _widen(self, width: int) -> None:
         """Tables of `width` pages where they are narrower."""

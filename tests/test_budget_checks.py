@@ -71,17 +71,3 @@ def test_tables_of_the_caller_stay_the_callers(widths):
         assert torch.equal(k[:, :kt.shape[1]], kt) and torch.equal(v[:, :vt.shape[1]], vt)
         assert torch.equal(s[:, :ks.shape[1]], ks)
         kt[1, 1], vt[1, 1], ks[1, 1] = 77, 78, 79               # the owner's next page
-
-
-def test_tables_are_not_replaced_within_a_capture(monkeypatch):
-    keys, values = (PagedPQCache(1, 2, D, 4, torch.zeros(16), "cpu", 64, max_pages=n) for n in (3, 7))
-    for c in (keys, values):
-        c.ensure(100)
-        c.seq_len = 70
-    monkeypatch.setattr(PagedPQCache, "shared_tables", lambda self: True)
-    before = keys.table
-    attention.check_paged(1, 4, D, keys, values)
-    assert keys.table is before and attention.page_tables(keys, values)[0].shape == (2, 7)
-    monkeypatch.undo()
-    attention.check_paged(1, 4, D, keys, values)
-    assert keys.table.shape == (2, 7) and attention.page_tables(keys, values)[0] is keys.table

@@ -9,7 +9,7 @@ from polarquant_kv import _lib, attention
 from polarquant_kv.lloyd_max import padded_codebook_torch
 from polarquant_kv.qjl import generate_jl_matrix, rotated_jl_matrix
 from polarquant_kv.rotation import generate_rotation_matrix
-from polarquant_kv.types import PQCache
+from polarquant_kv.types import PagedPQCache, PQCache
 
 from test_gpu_evict import paged_copy
 from test_gpu_weights import close, decoded, exact, make
@@ -246,3 +246,27 @@ def test_no_room_for_the_workspace_of_one_pass(monkeypatch):
     got = attention.attention_weights(q, kc, R, 0)
     assert refused
     close(got, want, tol)
+
+
+def test_tables_are_not_replaced_within_a_capture(monkeypatch):
+    q, kc, vc, R, _ = make(1, 4, 2, 150, 64, 4, False)
+    want, w = attention.decode_attention_weights(q, kc, vc, R)
+    pair = []
+    for c, pages in ((kc, 3), (vc, 7)):
+        p = PagedPQCache(1, 2, 64, 4, c.codebooks, DEV, page_tokens=64, max_pages=pages)
+        p.ensure(150)
+        for i, group in enumerate(p.groups):
+            n = min(64, 150 - 64 * i)
+            group[:, :, :n] = c.blocks[:, :, 64 * i:64 * i + n]
+        p.seq_len = 150
+        pair.append(p)
+    before = pair[0].table
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before a capture"):
+        attention.decode_attention_weights(q, *pair, R)
+    assert pair[0].table is before
+    monkeypatch.undo()
+    for capturing in (False, True):                              # widths are one after the first call
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+        out, got = attention.decode_attention_weights(q, *pair, R)
+        assert torch.equal(out, want) and torch.equal(got, w)
