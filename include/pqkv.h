@@ -411,7 +411,8 @@ int pqkv_decode_attn_weights_paged(const void *q, int q_dtype, const float *R,
  * rotated queries and their projections, which only signs need, it stays below
  * 1 GB + 4 bytes per position and 128 KB per (batch, kv-head) stream, however
  * long the chunk (long ones run in passes). A smaller workspace, of _least_bytes
- * and more, is taken too: with passes of fewer rows, which takes longer. */
+ * and more, is taken too: with passes of fewer rows, which take longer and add
+ * the rows up in other groups. */
 size_t pqkv_attn_weights_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 size_t pqkv_attn_weights_workspace_least_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int qjl);
 int pqkv_attn_weights(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const float *k_codebook,

@@ -149,6 +149,7 @@ class _Rotary(torch.autograd.Function):
         # y = M x: the tangent is M times x's (which may be of another type)
         interleaved, amplitude, back = ctx.how
         turn = _Rotary.apply if torch.is_grad_enabled() else _turn
+        _lib.require_one_device(tq, tk, *ctx.saved_tensors)            # (make_dual takes any)
         moving = [t.to(ctx.dtype) for t in (tq, tk) if t is not None]
         out = list(turn(*(moving + [None])[:2], *ctx.saved_tensors, interleaved, amplitude, not back))
         return tuple(None if shape is None else moving[0].new_zeros(shape) if t is None else out.pop(0)

@@ -85,6 +85,14 @@ def test_tangent_of_another_type(launches):
     assert torch.equal(got[1], formula(tk.bfloat16().float(), pos, f, False, 1.0, False))
 
 
+def test_tangent_on_another_device_is_refused(launches, doubles):
+    """(forward_ad takes such a pair; the launch would read a foreign address)"""
+    q, k, tq, tk, pos, f = inputs()
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="several devices"):
+            rotary.apply_rotary(q, forward_ad.make_dual(k, tk.to("meta")), pos, f)
+
+
 def test_tangents_of_gradients_and_gradients_of_tangents(launches, doubles):
     q, k, tq, tk, pos, f = inputs()
     q1 = q.clone().requires_grad_(True)
