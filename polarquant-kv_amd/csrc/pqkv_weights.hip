@@ -266,11 +266,11 @@ __global__ void __launch_bounds__(2 * D) weights_rows_kernel(const WeightsKernel
 }
 
 // Without QJL, from the queries themselves (a.x): y = R x on the matrix cores, so
-// that the rotated queries are never written. A = R, split hi / lo once per workgroup into registers (a wave's D /
-// 4 outputs), B = 16 queries as they lie in memory: fp16 queries are their own
-// high part (two products), fp32 ones are scaled and split (three). Queries off a
-// 16-byte boundary (ALIGNED false) are read in the pieces that their type's
-// alignment allows.
+// that the rotated queries are never written. A = R, split hi / lo once per
+// workgroup into registers (a wave's D / 4 outputs), B = 16 queries as they lie in
+// memory: fp16 queries are their own high part (two products), fp32 ones are scaled
+// and split (three). Queries off a 16-byte boundary (ALIGNED false) are read in the
+// pieces that their type's alignment allows.
 // 32764 x 8 rows (d = 128): 58 us (200 MB, 3.5 TB/s) where rotating first (75)
 // and making records of the result (48) took 123.
 template <int D, typename T, bool ALIGNED>

@@ -54,6 +54,8 @@ def check_shapes(B: int, Hq: int, d: int, keys: PQCache, values: PQCache, rotati
             per_batch = Hkv * c.max_seq_len * vector_bytes(d, c.n_bits)
         if c.blocks.numel() < B * per_batch:
             raise ValueError(f"{name}: {c.blocks.numel()} cache bytes, the shape needs {B * per_batch}")
+        if not c.blocks.is_contiguous():
+            raise ValueError(f"{name}: blocks must be contiguous")
     if keys.qjl_signs is not None and keys.qjl_signs.numel() < B * Hkv * keys.max_seq_len * (d // 8):
         raise ValueError("keys: QJL sign array smaller than the cache shape")
     return Hkv
@@ -114,6 +116,8 @@ def check_signs(jl_rot, keys, d: int) -> None:
         return
     if keys.qjl_signs is None:
         raise ValueError("QJL correction requested but the key cache has no signs")
+    if not keys.qjl_signs.is_contiguous():
+        raise ValueError("the keys' signs must be contiguous")
     if tuple(jl_rot.shape) != (d, d):
         raise ValueError(f"jl_rot must be ({d}, {d}), got {tuple(jl_rot.shape)}")
     if keys.jl_dim not in (0, d):

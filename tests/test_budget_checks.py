@@ -71,3 +71,19 @@ def test_tables_of_the_caller_stay_the_callers(widths):
         assert torch.equal(k[:, :kt.shape[1]], kt) and torch.equal(v[:, :vt.shape[1]], vt)
         assert torch.equal(s[:, :ks.shape[1]], ks)
         kt[1, 1], vt[1, 1], ks[1, 1] = 77, 78, 79               # the owner's next page
+
+
+def test_caches_that_are_views():
+    """Rows that do not follow each other would be read as if they did."""
+    kc, vc = caches(False)
+    wide = torch.zeros(1, 2, 20, 36, dtype=torch.uint8)
+    view = PQCache(blocks=wide[:, :, :8], head_dim=D, n_bits=4, seq_len=8, max_seq_len=8, codebooks=torch.zeros(16))
+    signs = PQCache(blocks=kc.blocks, head_dim=D, n_bits=4, seq_len=8, max_seq_len=8, codebooks=torch.zeros(16), jl_dim=D,
+                    qjl_signs=torch.zeros(1, 2, 20, 8, dtype=torch.uint8)[:, :, :8])
+    for bad, jl_rot in ((view, None), (signs, torch.zeros(D, D))):
+        for call in calls(bad, vc, jl_rot):
+            with pytest.raises(ValueError, match="contiguous"):
+                call()
+    for call in calls(signs, vc, None):                          # nothing reads them: on to the next check
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
