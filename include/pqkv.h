@@ -474,6 +474,47 @@ int pqkv_rotary(const void *q, const int64_t q_strides[3], void *q_out, int Hq, 
                 const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
                 int64_t positions_stride, const double *freqs, int B, int T, int d, int rot_dim, int interleaved,
                 float amplitude, int inverse, void *stream);
+/* The same with n_axes rows of positions (time, height, width): pair i turns by
+ * positions[axes[i]][b][t] * freqs[i]. axes: rot_dim / 2 bytes in host memory,
+ * below n_axes (at most 256), read by the call; axis a's positions start
+ * a * positions_axis_stride integers in. */
+int pqkv_rotary_axes(const void *q, const int64_t q_strides[3], void *q_out, int Hq, const void *k,
+                     const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
+                     int64_t positions_axis_stride, int64_t positions_stride, int n_axes, const uint8_t *axes,
+                     const double *freqs, int B, int T, int d, int rot_dim, int interleaved, float amplitude,
+                     int inverse, void *stream);
+
+/* ---- attention behind a window ----------------------------------------------
+ * No counterpart in the reference. The Sq query rows of sequence b stand at
+ * positions start_b .. start_b + Sq - 1 of a cache that holds them, and the one at
+ * p attends to the positions t <= p with t > p - window or t < sinks (the first
+ * few, which stay visible). Only the tiles of 64 positions that a row sees are
+ * read, so a call's work is that of the window, not of the cache.
+ *
+ * starts: int64 [B] on the device, or NULL: `start` for every sequence. counts:
+ * int64 [B] on the device, or NULL: Sq; the rows of a padded chunk that sequence b
+ * has. Both are read by the kernels, so a captured call follows them. A row past
+ * its sequence's count gives zeros, as does every row of a sequence whose start
+ * is outside 0 .. S - 1 and one at a position S or more (S: the positions that the
+ * caches have room for; with starts NULL start + Sq <= S is required). What stands
+ * at positions that no row sees, and past the last row, has no effect.
+ * q, out [B][Hq][Sq][d]. Keys and values of one width n_bits (2 or 4) with S_max
+ * = S vectors per stream, window >= 1, sinks >= 0, S < 2^24, B * Hkv <= 65535;
+ * Sq = 0 does nothing. Sq > 1: groups Hq / Hkv of up to 256 (128 with signs). The
+ * workspace is 16-byte aligned and needs no initialisation. */
+size_t pqkv_window_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int window, int sinks, int qjl);
+int pqkv_window_attn(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const uint8_t *v_cache,
+                     const float *k_codebook, const float *v_codebook, int n_bits, const uint8_t *qjl_signs,
+                     const float *p_rot, int m, int B, int Hq, int Hkv, int Sq, int64_t start, const int64_t *starts,
+                     const int64_t *counts, int window, int sinks, int S, int d, float scale, void *out,
+                     int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* The same on a paged cache (as pqkv_decode_attn_paged) whose pages hold S positions. */
+int pqkv_window_attn_paged(const void *q, int q_dtype, const float *R, const uint8_t *const *k_pages,
+                           const uint8_t *const *v_pages, int page_tokens, int max_pages, const float *k_codebook,
+                           const float *v_codebook, int n_bits, const uint8_t *const *qjl_pages, const float *p_rot,
+                           int m, int B, int Hq, int Hkv, int Sq, int64_t start, const int64_t *starts,
+                           const int64_t *counts, int window, int sinks, int S, int d, float scale, void *out,
+                           int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- dequantise -----------------------------------------------------------
  * out = (r16 c[code]) R for n block-encoded vectors: the stored radius times

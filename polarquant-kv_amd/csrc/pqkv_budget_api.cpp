@@ -237,7 +237,76 @@ int attn_weights_run(const void *q, int q_dtype, const float *R, const uint8_t *
   return PQKV_OK;
 }
 
+int rotary_run(const char *what, const void *q, const int64_t q_strides[3], void *q_out, int Hq, const void *k,
+               const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
+               int64_t positions_stride, const double *freqs, int B, int T, int d, int rot_dim, int interleaved,
+               float amplitude, int inverse, void *stream, const pqkv::RotaryAxes *axes) {
+  if (B < 0 || T < 0 || Hq < 0 || Hkv < 0)
+    return fail_status(PQKV_ERR_INVALID, "%s: B=%d T=%d Hq=%d Hkv=%d", what, B, T, Hq, Hkv);
+  if (d < 2 || d > 1024 || rot_dim < 2 || rot_dim > d || rot_dim % 2)
+    return fail_status(PQKV_ERR_UNSUPPORTED, "%s: rot_dim=%d of d=%d", what, rot_dim, d);
+  if (dtype != PQKV_F32 && dtype != PQKV_F16 && dtype != PQKV_BF16)
+    return fail_status(PQKV_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+  if (!std::isfinite(amplitude)) return fail_status(PQKV_ERR_INVALID, "%s: amplitude must be finite", what);
+  if (B == 0 || T == 0 || (Hq == 0 && Hkv == 0)) return PQKV_OK;
+  if ((Hq && (!q || !q_out || !q_strides)) || (Hkv && (!k || !k_out || !k_strides)) || !positions || !freqs)
+    return fail_status(PQKV_ERR_INVALID, "%s: null pointer", what);
+  const uintptr_t size = dtype == PQKV_F32 ? 4 : 2;
+  if ((Hq && ((uintptr_t)q | (uintptr_t)q_out) % size) || (Hkv && ((uintptr_t)k | (uintptr_t)k_out) % size) ||
+      (uintptr_t)positions % 8 || (uintptr_t)freqs % 8)
+    return fail_status(PQKV_ERR_INVALID, "%s: unaligned pointer", what);
+  if (positions_stride < 0) return fail_status(PQKV_ERR_INVALID, "%s: positions_stride < 0", what);
+  if ((int64_t)B * T > kMaxGrid || (int64_t)Hq + Hkv > 65535)
+    return fail_status(PQKV_ERR_UNSUPPORTED, "%s: B=%d T=%d heads=%lld", what, B, T, (long long)Hq + Hkv);
+  pqkv::RotaryArgs a;
+  memset(&a, 0, sizeof(a));
+  if (Hq) {
+    a.q = q;
+    a.q_out = q_out;
+    std::copy(q_strides, q_strides + 3, a.q_stride);
+  }
+  if (Hkv) {
+    a.k = k;
+    a.k_out = k_out;
+    std::copy(k_strides, k_strides + 3, a.k_stride);
+  }
+  a.positions = positions;
+  a.pos_batch_stride = positions_stride;
+  a.freqs = freqs;
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.T = T;
+  a.d = d;
+  a.rot_dim = rot_dim;
+  a.interleaved = interleaved ? 1 : 0;
+  a.inverse = inverse ? 1 : 0;
+  a.amplitude = amplitude;
+  const int tok = pqkv::prof_begin("rotary", (hipStream_t)stream);
+  const hipError_t e = axes ? pqkv::launch_rotary_axes(a, *axes, dtype, (hipStream_t)stream)
+                            : pqkv::launch_rotary(a, dtype, (hipStream_t)stream);
+  pqkv::prof_end(tok, (hipStream_t)stream);
+  return report_hip_error(e, "rotary launch");
+}
+
 }  // namespace
+
+namespace pqkv {
+
+int rotary_axes(const char *what, const uint8_t *axes, int n_axes, int rot_dim, int64_t stride, RotaryAxes *out) {
+  if (n_axes < 1 || n_axes > 256 || stride < 0 || !axes || rot_dim < 2 || rot_dim > 2 * kMaxRotaryPairs)
+    return fail_status(PQKV_ERR_INVALID, "%s: n_axes=%d rot_dim=%d positions_axis_stride=%lld", what, n_axes, rot_dim,
+                       (long long)stride);
+  out->stride = stride;
+  memset(out->of, 0, sizeof(out->of));
+  for (int i = 0; i < rot_dim / 2; ++i) {
+    if (axes[i] >= n_axes) return fail_status(PQKV_ERR_INVALID, "%s: pair %d has axis %d of %d", what, i, axes[i], n_axes);
+    out->of[i] = axes[i];
+  }
+  return PQKV_OK;
+}
+
+}  // namespace pqkv
 
 extern "C" {
 
@@ -393,51 +462,20 @@ int pqkv_rotary(const void *q, const int64_t q_strides[3], void *q_out, int Hq, 
                 const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
                 int64_t positions_stride, const double *freqs, int B, int T, int d, int rot_dim, int interleaved,
                 float amplitude, int inverse, void *stream) {
-  if (B < 0 || T < 0 || Hq < 0 || Hkv < 0)
-    return fail_status(PQKV_ERR_INVALID, "rotary: B=%d T=%d Hq=%d Hkv=%d", B, T, Hq, Hkv);
-  if (d < 2 || d > 1024 || rot_dim < 2 || rot_dim > d || rot_dim % 2)
-    return fail_status(PQKV_ERR_UNSUPPORTED, "rotary: rot_dim=%d of d=%d", rot_dim, d);
-  if (dtype != PQKV_F32 && dtype != PQKV_F16 && dtype != PQKV_BF16)
-    return fail_status(PQKV_ERR_UNSUPPORTED, "rotary: dtype %d", dtype);
-  if (!std::isfinite(amplitude)) return fail_status(PQKV_ERR_INVALID, "rotary: amplitude must be finite");
-  if (B == 0 || T == 0 || (Hq == 0 && Hkv == 0)) return PQKV_OK;
-  if ((Hq && (!q || !q_out || !q_strides)) || (Hkv && (!k || !k_out || !k_strides)) || !positions || !freqs)
-    return fail_status(PQKV_ERR_INVALID, "rotary: null pointer");
-  const uintptr_t size = dtype == PQKV_F32 ? 4 : 2;
-  if ((Hq && ((uintptr_t)q | (uintptr_t)q_out) % size) || (Hkv && ((uintptr_t)k | (uintptr_t)k_out) % size) ||
-      (uintptr_t)positions % 8 || (uintptr_t)freqs % 8)
-    return fail_status(PQKV_ERR_INVALID, "rotary: unaligned pointer");
-  if (positions_stride < 0) return fail_status(PQKV_ERR_INVALID, "rotary: positions_stride < 0");
-  if ((int64_t)B * T > kMaxGrid || (int64_t)Hq + Hkv > 65535)
-    return fail_status(PQKV_ERR_UNSUPPORTED, "rotary: B=%d T=%d heads=%lld", B, T, (long long)Hq + Hkv);
-  pqkv::RotaryArgs a;
-  memset(&a, 0, sizeof(a));
-  if (Hq) {
-    a.q = q;
-    a.q_out = q_out;
-    std::copy(q_strides, q_strides + 3, a.q_stride);
-  }
-  if (Hkv) {
-    a.k = k;
-    a.k_out = k_out;
-    std::copy(k_strides, k_strides + 3, a.k_stride);
-  }
-  a.positions = positions;
-  a.pos_batch_stride = positions_stride;
-  a.freqs = freqs;
-  a.B = B;
-  a.Hq = Hq;
-  a.Hkv = Hkv;
-  a.T = T;
-  a.d = d;
-  a.rot_dim = rot_dim;
-  a.interleaved = interleaved ? 1 : 0;
-  a.inverse = inverse ? 1 : 0;
-  a.amplitude = amplitude;
-  const int tok = pqkv::prof_begin("rotary", (hipStream_t)stream);
-  const hipError_t e = pqkv::launch_rotary(a, dtype, (hipStream_t)stream);
-  pqkv::prof_end(tok, (hipStream_t)stream);
-  return report_hip_error(e, "rotary launch");
+  return rotary_run("rotary", q, q_strides, q_out, Hq, k, k_strides, k_out, Hkv, dtype, positions, positions_stride,
+                    freqs, B, T, d, rot_dim, interleaved, amplitude, inverse, stream, nullptr);
+}
+
+int pqkv_rotary_axes(const void *q, const int64_t q_strides[3], void *q_out, int Hq, const void *k,
+                     const int64_t k_strides[3], void *k_out, int Hkv, int dtype, const int64_t *positions,
+                     int64_t positions_axis_stride, int64_t positions_stride, int n_axes, const uint8_t *axes,
+                     const double *freqs, int B, int T, int d, int rot_dim, int interleaved, float amplitude,
+                     int inverse, void *stream) {
+  pqkv::RotaryAxes ax;
+  const int c = pqkv::rotary_axes("rotary_axes", axes, n_axes, rot_dim, positions_axis_stride, &ax);
+  if (c != PQKV_OK) return c;
+  return rotary_run("rotary_axes", q, q_strides, q_out, Hq, k, k_strides, k_out, Hkv, dtype, positions,
+                    positions_stride, freqs, B, T, d, rot_dim, interleaved, amplitude, inverse, stream, &ax);
 }
 
 }  // extern "C"

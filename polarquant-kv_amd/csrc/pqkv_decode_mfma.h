@@ -57,6 +57,7 @@
 
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
+#include "pqkv_window.h"
 
 namespace pqkv {
 
@@ -342,12 +343,17 @@ struct DecodeSmem {
 // four consecutive tokens of one head, one 16-byte store (8 sequences of 32768
 // tokens, 32 / 8 heads, 4 bits: 72 us where the kernel without takes 68; the
 // stores are 34 MB beside 302 read).
+// WIN (attention behind a window, a.win): one row per sequence, at a position
+// of its own. A split is a share of the tiles that the row sees (sinks first,
+// window_tiles), so a launch's work does not grow with the cache. Edge tiles
+// hide positions: their logits are -inf and their radii 0 (a hidden value that is
+// not a number would give 0 * NaN). Positions past the row read zeros.
 // FREE: the steady-state iteration has no scheduling fences between its
 // table reads, softmax weights and products (the mixed-width pair kernel and
 // the ggml layout, 3.5 % and 2.4 % faster that way; the other kernels are as
 // fast or faster with them).
 template <int D, int G, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GG = false, bool HW = false,
-          bool PG = false, bool FREE = false, bool WS = false>
+          bool PG = false, bool FREE = false, bool WS = false, bool WIN = false>
 __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem<D, G, KB, VBITS, QJL, VSH> &sm,
                                                  const int split, const int bh) {
   static_assert(!SOA || (KB == 4 && VBITS == 4 && !QJL), "the SoA layout carries 4-bit codes and no QJL signs");
@@ -355,6 +361,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   static_assert(!HW || GG, "one kv head per wave is a mode of the ggml layout (fp16 block radii, no listed heads)");
   static_assert(!PG || (!SOA && !GG), "paged caches hold block-encoded vectors, one token per vector slot");
   static_assert(!WS || (!SOA && !GG), "the logits are written for block-encoded caches");
+  static_assert(!WIN || (!SOA && !GG && !WS), "windows are over block-encoded caches");
   constexpr int VBK = SOA ? D / 2 : vector_bytes(D, KB), VBV = SOA ? D / 2 : vector_bytes(D, VBITS);
   constexpr int KK = D / 16;     // score MFMAs per 16-token tile
   constexpr int NB = D / 16;     // value n-tiles
@@ -381,8 +388,22 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   const bool listed = !GG && a.listed;  // (the ggml layout lists no heads)
   const int h = listed ? a.heads[hi_] : hi_;
   const int seq = GG ? b / a.rows_per_seq : b;   // the key / value sequence of row b
+  // WIN: the row's position, the positions that are read (those past the row
+  // as zeros), and the split's tiles
+  int row = 0, tile0 = 0, tile1 = 0;
+  WindowTiles wt{};
+  if constexpr (WIN) {
+    const WindowRows wr = window_rows(a.win, b, 1, a.S);
+    row = __builtin_amdgcn_readfirstlane(wr.start);
+    wt = window_tiles(a.win, row, row);
+    if (wr.count > 0) {
+      tile0 = (int)((int64_t)wt.tiles * split / a.splits);
+      tile1 = (int)((int64_t)wt.tiles * (split + 1) / a.splits);
+    }
+  }
+  auto S = [&] { return WIN ? row + 1 : a.S; };
   const int t_begin = split * a.tokens_per_split;
-  const int t_end = min(a.S, t_begin + a.tokens_per_split);
+  const int t_end = min(S(), t_begin + a.tokens_per_split);
   const uint8_t *kstream, *vstream;
   if (listed) {
     kstream = a.k_cache + b * a.k_batch_stride + a.k_head_off[hi_];
@@ -393,8 +414,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   }
   // bytes between consecutive tokens of a stream
   const int kts = GG ? (int)a.k_tok_stride : VBK, vts = GG ? (int)a.v_tok_stride : VBV;
-  const __amdgpu_buffer_rsrc_t kres = stream_rsrc(kstream, (uint32_t)a.S * (uint32_t)kts);
-  const __amdgpu_buffer_rsrc_t vres = stream_rsrc(vstream, (uint32_t)a.S * (uint32_t)vts);
+  const __amdgpu_buffer_rsrc_t kres = stream_rsrc(kstream, (uint32_t)S() * (uint32_t)kts);
+  const __amdgpu_buffer_rsrc_t vres = stream_rsrc(vstream, (uint32_t)S() * (uint32_t)vts);
   // GG: the mask row of row b (no mask: an empty buffer, every load reads 0)
   __amdgpu_buffer_rsrc_t mres = kres;
   if constexpr (GG) {
@@ -414,7 +435,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   auto rad = [](uint32_t bits) { return SOA ? __builtin_bit_cast(float, bits) : half_bits_to_float(bits); };
   __amdgpu_buffer_rsrc_t sres = kres;
   if constexpr (QJL && !PG)
-    sres = stream_rsrc(a.qjl + ((int64_t)(b * a.Hkv + h) * a.S_max) * (D / 8), (uint32_t)a.S * (uint32_t)(D / 8));
+    sres = stream_rsrc(a.qjl + ((int64_t)(b * a.Hkv + h) * a.S_max) * (D / 8), (uint32_t)S() * (uint32_t)(D / 8));
   // The buffer that chunk t0 loads through and t0's position in it: the
   // whole stream, or (PG) the chunk's page, over the page's valid tokens (so
   // loads past S still read 0). The page address is wave-uniform (a scalar
@@ -424,12 +445,15 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     if constexpr (PG) {
       const int pg = t0 >> a.page_shift, p0 = pg << a.page_shift;
       rel = t0 - p0;
-      return stream_rsrc(pages[prow + pg], (uint32_t)min(a.S - p0, 1 << a.page_shift) * vb);
+      return stream_rsrc(pages[prow + pg], (uint32_t)min(S() - p0, 1 << a.page_shift) * vb);
     } else {
       rel = t0;
       return whole;
     }
   };
+  // WIN: the positions that the row does not see, and the tiles that hold some
+  auto hidden = [&](int t) { return t > row || (t + a.win.size <= row && t >= a.win.sinks); };
+  auto edge = [&](int t0) { return t0 + kChunk - 1 > row || (t0 + a.win.size <= row && t0 + kChunk > a.win.sinks); };
 
   // WS: the logit rows of this launch's heads; a lane's store starts
   // l_off + 4 t0 bytes in (past the end, so dropped, where it holds no head)
@@ -761,7 +785,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
           c = __builtin_fmaf(x, 1.0f / kLoScale, c) * quad_bcast(rks, i);
         }
         if constexpr (GG) c = __builtin_fmaf(mask_val(mk, i), kLog2eF, c);  // the logits are in the exp2 domain
-        cv[i] = partial && kSub * (col >> 2) + 4 * grp + i >= ntok ? -INFINITY : c;
+        const int t = kSub * (col >> 2) + 4 * grp + i;
+        cv[i] = partial && (WIN ? hidden(t0 + t) : t >= ntok) ? -INFINITY : c;
       }
       store_logits(t0, 0, (float4_t){cv[0], cv[1], cv[2], cv[3]});
       cmax = fmaxf(fmaxf(cv[0], cv[1]), fmaxf(cv[2], cv[3]));
@@ -777,7 +802,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
         for (int st = 0; st < NSUB; ++st)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (kSub * st + 4 * grp + i >= ntok) sv[st][i] = -INFINITY;
+            if (WIN ? hidden(t0 + kSub * st + 4 * grp + i) : kSub * st + 4 * grp + i >= ntok) sv[st][i] = -INFINITY;
       }
 #pragma unroll
       for (int st = 0; st < NSUB; ++st) store_logits(t0, st, (float4_t){sv[st][0], sv[st][1], sv[st][2], sv[st][3]});
@@ -898,7 +923,11 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   auto finish = [&](const CV &v, const float4_t (&sc)[NSUB], float rks, const uint32_t (&mks)[MC],
                     int ntok, bool partial, int t0) {
     float sv[NSUB][4];
-    const float rvl = rad(v.r);
+    float rvl = rad(v.r);
+    if constexpr (WIN) {
+      partial = edge(t0);
+      if (partial && hidden(t0 + rtok)) rvl = 0.0f;
+    }
     FState f = fbegin(sv, sc, ntok, partial, rvl, rks, mks, t0);
     VTile vt[2];
     vread(v, 0, vt[0]);
@@ -922,9 +951,15 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   constexpr bool kPieceLoads = !QJL || G <= 4;
   constexpr int kStep = HW ? kChunk : kMWaves * kChunk;   // from one of the wave's chunks to the next
   auto step = [&](CK &k, CV &v, const float4_t (&sc)[NSUB], float rks, const uint32_t (&mks)[MC],
-                  float4_t (&sn)[NSUB], float &rkn, uint32_t (&mkn)[MC], int tk, int tv) {
+                  float4_t (&sn)[NSUB], float &rkn, uint32_t (&mkn)[MC], int tk, int tv, int t0) {
     float sv[NSUB][4];
-    const float rkl = rad(k.r), rvl = rad(v.r);
+    const float rkl = rad(k.r);
+    float rvl = rad(v.r);
+    bool partial = false;
+    if constexpr (WIN) {
+      partial = edge(t0);
+      if (partial && hidden(t0 + rtok)) rvl = 0.0f;
+    }
     rkn = rkl;
     // the buffers of the chunks this iteration loads
     int tkr = tk, tvr = tv;
@@ -935,7 +970,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     }
 #pragma unroll
     for (int j = 0; j < MC; ++j) mkn[j] = k.mw[j];
-    FState f = fbegin(sv, sc, kChunk, false, rvl, rks, mks, tv - kStep);
+    FState f = fbegin(sv, sc, kChunk, partial, rvl, rks, mks, WIN ? t0 : tv - kStep);
 #pragma unroll
     for (int j = 0; j < NSUB; ++j) {
       KTile kt;
@@ -979,30 +1014,34 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
   // (PG: through a scalar register, so that the chunk positions and with
   // them the page addresses are known to be wave-uniform)
   const int first = t_begin + (HW ? 0 : (PG ? __builtin_amdgcn_readfirstlane(wave) : wave) * kChunk);
-  const int nch = first < t_end ? (t_end - first + kStep - 1) / kStep : 0;
+  const int wtile = tile0 + (WIN ? __builtin_amdgcn_readfirstlane(wave) : 0);
+  const int nch = WIN ? (wtile < tile1 ? (tile1 - wtile + kMWaves - 1) / kMWaves : 0)
+                      : first < t_end ? (t_end - first + kStep - 1) / kStep : 0;
+  // position of the wave's i-th chunk
+  auto at = [&](int i) { return WIN ? wt.at(wtile + kMWaves * i) : first + i * kStep; };
   if (nch > 0) {
     CK ck;
     CV cv;
-    load_k(ck, first);
-    load_v(cv, first);
+    load_k(ck, at(0));
+    load_v(cv, at(0));
     float4_t sacc[NSUB];
     float rks;
     uint32_t mks[MC];
     scores(ck, sacc, rks, mks);
     // chunk 1 (a repeat of chunk 0 when there is none: an L2 hit)
-    load_k(ck, first + min(1, nch - 1) * kStep);
+    load_k(ck, at(min(1, nch - 1)));
     for (int i = 0; i + 1 < nch; ++i) {
       float4_t snext[NSUB];
       float rkn;
       uint32_t mkn[MC];
-      step(ck, cv, sacc, rks, mks, snext, rkn, mkn, first + min(i + 2, nch - 1) * kStep, first + (i + 1) * kStep);
+      step(ck, cv, sacc, rks, mks, snext, rkn, mkn, at(min(i + 2, nch - 1)), at(i + 1), at(i));
 #pragma unroll
       for (int st = 0; st < NSUB; ++st) sacc[st] = snext[st];
       rks = rkn;
 #pragma unroll
       for (int j = 0; j < MC; ++j) mks[j] = mkn[j];
     }
-    const int tlast = first + (nch - 1) * kStep;
+    const int tlast = at(nch - 1);
     finish(cv, sacc, rks, mks, min(kChunk, t_end - tlast), true, tlast);
   }
 
@@ -1082,14 +1121,14 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
 // HW: workgroup row y takes the pairs 4y .. 4y + 3, one per wave (n_heads a
 // multiple of 4, so the four share the batch row).
 template <int D, int G, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GG = false, bool HW = false,
-          bool PG = false, bool WS = false>
+          bool PG = false, bool WS = false, bool WIN = false>
 __global__ void __launch_bounds__(256, kMfmaBlocksPerCU) decode_mfma_kernel(const DecodeArgs a) {
   __shared__ DecodeSmem<D, G, KB, VBITS, QJL, VSH> sm;
   // (read through a scalar register: the buffer resources built from the
   // pair must be wave-uniform, or every load becomes a loop over lanes)
   const int bh = HW ? __builtin_amdgcn_readfirstlane((int)blockIdx.y * kMWaves + (int)(threadIdx.x >> 6))
                     : (int)blockIdx.y;
-  decode_mfma_body<D, G, KB, VBITS, QJL, VSH, SOA, GG, HW, PG, GG, WS>(a, sm, blockIdx.x, bh);
+  decode_mfma_body<D, G, KB, VBITS, QJL, VSH, SOA, GG, HW, PG, GG, WS, WIN>(a, sm, blockIdx.x, bh);
 }
 
 // Mixed widths whose kv heads are either 4-bit keys and values (a4, one
@@ -1129,25 +1168,26 @@ __global__ void __launch_bounds__(256, kMfmaBlocksPerCU) decode_mfma_pair_kernel
   }
 
 template <int D, int KB, int VBITS, bool QJL, bool VSH, bool SOA = false, bool GGML = false, bool HW = false,
-          bool PG = false, bool WS = false>
+          bool PG = false, bool WS = false, bool WIN = false>
 static void launch_dm(const DecodeArgs &a, int G, hipStream_t s) {
   dim3 grid(a.splits, HW ? a.B * a.n_heads / kMWaves : a.B * a.n_heads);
-#define PQKV_DM_ONE(GG, ...) decode_mfma_kernel<D, GG, KB, VBITS, QJL, VSH, SOA, GGML, HW, PG, WS><<<grid, 256, 0, s>>>(a)
+#define PQKV_DM_ONE(GG, ...) decode_mfma_kernel<D, GG, KB, VBITS, QJL, VSH, SOA, GGML, HW, PG, WS, WIN><<<grid, 256, 0, s>>>(a)
   PQKV_DM_G_SWITCH(PQKV_DM_ONE, 0)
 #undef PQKV_DM_ONE
 }
 
 // One width pair on both head dims, with or without QJL (PG: paged caches,
-// whose QJL signs come through a.s_pages; WS: the logits written too).
-template <int KB, int VBITS, bool VSH = false, bool PG = false, bool WS = false>
+// whose QJL signs come through a.s_pages; WS: the logits written too; WIN:
+// behind a window).
+template <int KB, int VBITS, bool VSH = false, bool PG = false, bool WS = false, bool WIN = false>
 static hipError_t launch_dm_widths(const DecodeArgs &a, hipStream_t s) {
   const bool qjl = PG ? a.s_pages != nullptr : a.qjl != nullptr;
   if (a.d == 128) {
-    if (qjl) launch_dm<128, KB, VBITS, true, VSH, false, false, false, PG, WS>(a, a.g, s);
-    else launch_dm<128, KB, VBITS, false, VSH, false, false, false, PG, WS>(a, a.g, s);
+    if (qjl) launch_dm<128, KB, VBITS, true, VSH, false, false, false, PG, WS, WIN>(a, a.g, s);
+    else launch_dm<128, KB, VBITS, false, VSH, false, false, false, PG, WS, WIN>(a, a.g, s);
   } else {
-    if (qjl) launch_dm<64, KB, VBITS, true, VSH, false, false, false, PG, WS>(a, a.g, s);
-    else launch_dm<64, KB, VBITS, false, VSH, false, false, false, PG, WS>(a, a.g, s);
+    if (qjl) launch_dm<64, KB, VBITS, true, VSH, false, false, false, PG, WS, WIN>(a, a.g, s);
+    else launch_dm<64, KB, VBITS, false, VSH, false, false, false, PG, WS, WIN>(a, a.g, s);
   }
   return hipGetLastError();
 }
@@ -1170,5 +1210,12 @@ hipError_t launch_dm_logits_k2v2(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_logits_paged_k4v4_shared(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_logits_paged_k4v4_own(const DecodeArgs &a, hipStream_t s);
 hipError_t launch_dm_logits_paged_k2v2(const DecodeArgs &a, hipStream_t s);
+// The same six behind a window.
+hipError_t launch_dm_window_k4v4_shared(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_window_k4v4_own(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_window_k2v2(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_window_paged_k4v4_shared(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_window_paged_k4v4_own(const DecodeArgs &a, hipStream_t s);
+hipError_t launch_dm_window_paged_k2v2(const DecodeArgs &a, hipStream_t s);
 
 }  // namespace pqkv

@@ -26,4 +26,14 @@ hipError_t launch_decode_mfma_logits(const DecodeArgs &a, int bits, hipStream_t 
   return launch_dm_logits_k2v2(a, s);
 }
 
+hipError_t launch_decode_mfma_window(const DecodeArgs &a, int bits, hipStream_t s) {
+  const bool shared = a.k_cb == a.v_cb;
+  if (a.k_pages) {
+    if (bits == 4) return shared ? launch_dm_window_paged_k4v4_shared(a, s) : launch_dm_window_paged_k4v4_own(a, s);
+    return launch_dm_window_paged_k2v2(a, s);
+  }
+  if (bits == 4) return shared ? launch_dm_window_k4v4_shared(a, s) : launch_dm_window_k4v4_own(a, s);
+  return launch_dm_window_k2v2(a, s);
+}
+
 }  // namespace pqkv

@@ -54,6 +54,14 @@ __device__ __forceinline__ uint8_t *encode_out_addr(const EncodeArgs &a, uint8_t
   return pages[o * a.max_pages + (pos >> a.page_shift)] + (pos & ((1 << a.page_shift) - 1)) * vb;
 }
 
+// Attention behind a window: the query rows of sequence b stand at starts[b] ..
+// starts[b] + counts[b] - 1 (null: `start` / `count` for every sequence), and the
+// one at p sees the positions t <= p with t > p - size or t < sinks.
+struct Window {
+  const int64_t *starts, *counts;
+  int64_t start, count;
+  int size, sinks;
+};
 // One launch of the split-K decode kernel covers B x n_heads (batch, kv-head)
 // streams with the same K and V bit widths.
 struct DecodeArgs {
@@ -96,6 +104,7 @@ struct DecodeArgs {
   int64_t logit_stride;
   int16_t heads[kMaxListHeads];
   int64_t k_head_off[kMaxListHeads], v_head_off[kMaxListHeads];
+  Window win;                    // the kernels' WIN mode (S is the cache's capacity then)
 };
 
 // One launch of the chunked-prefill kernel: workgroups of prefill_rows(qjl)
@@ -130,6 +139,7 @@ struct PrefillArgs {
   int page_shift, max_pages;
   int16_t heads[kMaxListHeads];
   int64_t k_head_off[kMaxListHeads], v_head_off[kMaxListHeads];
+  Window win;                    // the kernel's WIN mode (S is the cache's capacity, q_start unused)
 };
 
 // Workspace of one decode call whose plan has `splits` partitions per stream
@@ -274,7 +284,9 @@ hipError_t launch_decode_mfma_paged(const DecodeArgs &a, int bits, hipStream_t s
 // The same kernels writing a.logits (keys and values of `bits` each, contiguous
 // or, with a.k_pages, paged).
 hipError_t launch_decode_mfma_logits(const DecodeArgs &a, int bits, hipStream_t s);
-// The end of such a call: out as launch_decode_merge (with R), and w.out = w.in
+// The same kernels behind a window (a.win), keys and values of `bits` each.
+hipError_t launch_decode_mfma_window(const DecodeArgs &a, int bits, hipStream_t s);
+// The end of a call that writes the logits: out as launch_decode_merge (with R), and w.out = w.in
 // + the softmax weights summed over each kv head's query heads, from the logits
 // and the splits' partials.
 constexpr int kMaxGroupWeights = 1024;   // query heads per kv head
@@ -358,6 +370,8 @@ int device_compute_units();
 // Measurement: read `bytes` (a multiple of 16) from p once, XOR into sink[block].
 hipError_t launch_stream_read(const void *p, size_t bytes, uint32_t *sink, int blocks, hipStream_t s);
 hipError_t launch_prefill(const PrefillArgs &a, int k_bits, int v_bits, hipStream_t s);
+// The same behind a window (a.win), keys and values of `bits` each.
+hipError_t launch_prefill_window(const PrefillArgs &a, int bits, hipStream_t s);
 // How a prefill call runs: row blocks of `rows` query rows (qt tokens x G
 // heads), qtiles per (batch, kv-head) stream; planes: over tiles decoded once
 // per call (pqkv_prefill_planes.hip), `streams` streams at a time, else by the
@@ -371,6 +385,9 @@ struct PrefillPlan {
   size_t part_bytes(int d) const { return ((size_t)part_rows * (d + 2) * 4 + 255) & ~(size_t)255; }
   size_t bytes(int d) const { return part_bytes(d) + (planes ? (size_t)streams * stream_bytes : 0); }
 };
+// A call behind a window: never over tiles decoded once, whose rows see one tile in
+// few blocks; splits as above.
+PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w, bool extra);
 inline int64_t prefill_record_bytes(int d) { return 512 * (int64_t)d + 512; }   // one decoded 64-token tile
 // extra: the workspace holds what the plan asks for; planes_only: over tiles
 // decoded once, at any count of row blocks, where a stream's fit their budget.
@@ -425,6 +442,15 @@ struct RotaryArgs {
   float amplitude;
 };
 hipError_t launch_rotary(const RotaryArgs &a, int dtype, hipStream_t s);
+// The axis of each pair, whose positions lie `stride` integers apart.
+constexpr int kMaxRotaryPairs = 512;
+struct RotaryAxes {
+  int64_t stride;
+  uint8_t of[kMaxRotaryPairs];
+};
+// The checked table of a call's axes (host); a status.
+int rotary_axes(const char *what, const uint8_t *axes, int n_axes, int rot_dim, int64_t stride, RotaryAxes *out);
+hipError_t launch_rotary_axes(const RotaryArgs &a, const RotaryAxes &axes, int dtype, hipStream_t s);
 
 // Eviction: selection, and the move of up to PQKV_MAX_GATHER arrays' rows.
 hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_streams, int S, int keep, int sink,

@@ -38,6 +38,13 @@
 // B = pq hi / lo. The key radius then scales the code product before the
 // sign product is added (in the matrix stage instead of the softmax).
 //
+// WIN (attention behind a window, a.win): a sequence's rows stand at a position
+// of its own, and a row block walks the tiles that one of its rows sees (sinks
+// first, window_tiles), so its work is that of the window. Tiles keep two numbers:
+// `it` counts the row block's (buffers), pos(it) is where one lies. On edge
+// tiles a hidden position's weight is 0 whatever its radius holds. Rows past a
+// sequence's count give zeros.
+//
 // Precision: every fp32 operand x is split as x_hi = fp16(x),
 // x_lo = fp16(x - x_hi) (fp16 subnormals included, which the f16 MFMA keeps),
 // and each product is hi.hi + hi.lo + lo.hi in one fp32 accumulator: three
@@ -47,11 +54,13 @@
 // 0.003 .. 0.33 and queries down to ~0.002 keep normal lo parts); the exact
 // power-of-two factors come back out through the key radii (/ 2^12) and the
 // final normalisation (/ 2^6).
+#include <algorithm>
 #include <type_traits>
 
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 #include "pqkv_prefill.h"
+#include "pqkv_window.h"
 
 namespace pqkv {
 
@@ -242,7 +251,7 @@ __device__ __forceinline__ void decode_v(const uint8_t *raw, uint8_t *tile, floa
   if (gtid < kPT) rad[kPT + gtid] = half_bits_to_float(*(const uint16_t *)(raw + gtid * VB));
 }
 
-template <int D, int KB, int VBITS, bool QJL>
+template <int D, int KB, int VBITS, bool QJL, bool WIN = false>
 __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const PrefillArgs a) {
   using PT = PrefillTile<D>;
   constexpr int KS = PT::KS, NB = PT::NB;
@@ -275,8 +284,23 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   const int b = bh / a.n_heads, hl = bh - b * a.n_heads;
   const int h = a.listed ? a.heads[hl] : hl;
   const int q0 = qtile * a.qt;                       // first query token of the block
-  const int q_last = min(a.Sq, q0 + a.qt) - 1;       // last valid query token
-  const int kv_end = a.causal ? min(a.S, a.q_start + q_last + 1) : a.S;
+  // WIN: the sequence's rows; the tiles of the block's, none where it has no row
+  WindowRows wr{};
+  WindowTiles wt{};
+  if constexpr (WIN) {
+    wr = window_rows(a.win, b, a.Sq, a.S);
+    wr.start = __builtin_amdgcn_readfirstlane(wr.start);
+    wr.count = __builtin_amdgcn_readfirstlane(wr.count);
+  }
+  auto Sq = [&] { return WIN ? wr.count : a.Sq; };   // rows of this sequence
+  auto S = [&] { return WIN ? wr.start + wr.count : a.S; };
+  auto q_start = [&] { return WIN ? wr.start : a.q_start; };
+  const int q_last = min(Sq(), q0 + a.qt) - 1;       // last valid query token
+  const int kv_end = WIN ? 0 : a.causal ? min(a.S, a.q_start + q_last + 1) : a.S;
+  if constexpr (WIN) {
+    if (q_last >= q0) wt = window_tiles(a.win, wr.start + q0, wr.start + q_last);
+  }
+  auto pos = [&](int it) { return WIN ? wt.at(it) : it * kPT; };
 
   const uint8_t *kstream, *vstream;
   if (a.listed) {
@@ -286,11 +310,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     kstream = a.k_cache + b * a.k_batch_stride + h * a.k_head_stride;
     vstream = a.v_cache + b * a.v_batch_stride + h * a.v_head_stride;
   }
-  const __amdgpu_buffer_rsrc_t kres = stream_rsrc(kstream, (uint32_t)a.S * (uint32_t)VBK);
-  const __amdgpu_buffer_rsrc_t vres = stream_rsrc(vstream, (uint32_t)a.S * (uint32_t)VBV);
+  const __amdgpu_buffer_rsrc_t kres = stream_rsrc(kstream, (uint32_t)S() * (uint32_t)VBK);
+  const __amdgpu_buffer_rsrc_t vres = stream_rsrc(vstream, (uint32_t)S() * (uint32_t)VBV);
   __amdgpu_buffer_rsrc_t sres = kres;
   if constexpr (QJL)
-    sres = stream_rsrc(a.qjl + ((int64_t)(b * a.Hkv + h) * a.S_max) * SGB, (uint32_t)a.S * (uint32_t)SGB);
+    sres = stream_rsrc(a.qjl + ((int64_t)(b * a.Hkv + h) * a.S_max) * SGB, (uint32_t)S() * (uint32_t)SGB);
 
   // code unit (a byte of two 4-bit codes, a nibble of two 2-bit codes) ->
   // (c_hi, c_hi' | c_lo, c_lo') of its two codes
@@ -324,8 +348,8 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   for (int rt = 0; rt < RT; ++rt) {
     const int row = 16 * RT * wave + 16 * rt + col;
     const int tok = q0 + row / G, head = row % G;
-    const bool row_ok = row < a.qt * G && tok < a.Sq;
-    row_pos[rt] = a.q_start + tok;
+    const bool row_ok = row < a.qt * G && tok < Sq();
+    row_pos[rt] = q_start() + tok;
     const int64_t qrow = ((int64_t)(b * a.Hq + h * G + head) * a.Sq) + (row_ok ? tok : 0);
     const float *qr = a.q + qrow * D;
     // (loaded for every row, a valid one for those past the end: with the load
@@ -469,9 +493,12 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   };
   // online softmax of tile it's scores -> weights p * r_v as the A operand
   auto softmax = [&](int it) {
-    const int t0 = it * kPT;
+    const int t0 = pos(it);
     const float *rk = rads[it & 1], *rv = rads[it & 1] + kPT;
-    const bool need_mask = t0 + kPT > a.S || (a.causal && t0 + kPT - 1 > a.q_start + q0);
+    // WIN: what the first row does not see yet, what the last one sees no more
+    const bool need_mask = WIN ? t0 + kPT - 1 > wr.start + q0 ||
+                                     (t0 + a.win.size <= wr.start + q_last && t0 + kPT > a.win.sinks)
+                               : t0 + kPT > a.S || (a.causal && t0 + kPT - 1 > a.q_start + q0);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float s[4][4];
@@ -488,7 +515,9 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t0 + 16 * tt + 4 * grp + i;
-            if (t >= a.S || (a.causal && t > row_pos[rt])) s[tt][i] = -INFINITY;
+            if (WIN ? t > row_pos[rt] || (t + a.win.size <= row_pos[rt] && t >= a.win.sinks)
+                    : t >= a.S || (a.causal && t > row_pos[rt]))
+              s[tt][i] = -INFINITY;
           }
       }
       float cmax = s[0][0];
@@ -506,7 +535,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         const float4 r4 = *(const float4 *)&rv[16 * tt + 4 * grp];
-        const float rr[4] = {r4.x, r4.y, r4.z, r4.w};
+        float rr[4] = {r4.x, r4.y, r4.z, r4.w};
+        if (WIN && need_mask) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rr[i] = s[tt][i] == -INFINITY ? 0.0f : rr[i];
+        }
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
           const float p0 = __builtin_amdgcn_exp2f(s[tt][i] - ref), p1 = __builtin_amdgcn_exp2f(s[tt][i + 1] - ref);
@@ -551,7 +584,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   // group 1's values of tile it - 1 (stage 2 it + 1). Each is read from the
   // stage after its decode on, and radii follow their half.
   // this workgroup's tiles: all of the row block's, or its split's share
-  const int all = (kv_end + kPT - 1) / kPT;
+  const int all = WIN ? wt.tiles : (kv_end + kPT - 1) / kPT;
   const int it0 = share_begin(all, sp, splits), it1 = share_begin(all, sp + 1, splits);
   uint8_t(&graw)[2][RawTile<D>::kAlloc] = raw[group];
   // The buffer tile t0 is copied from and t0's position in it: the whole
@@ -565,7 +598,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     }
     const int pg = t0 >> a.page_shift, p0 = pg << a.page_shift;
     rel = t0 - p0;
-    return stream_rsrc(pages[prow + pg], (uint32_t)min(a.S - p0, 1 << a.page_shift) * (uint32_t)vb);
+    return stream_rsrc(pages[prow + pg], (uint32_t)min(S() - p0, 1 << a.page_shift) * (uint32_t)vb);
   };
   auto decode = [&](int it) {  // this group's half of tile it, from graw[it & 1]
     if (group == 0) decode_k<D, KB>(graw[it & 1], tiles[it & 1], rads[it & 1], lut_k, gtid);
@@ -576,15 +609,15 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   auto dma = [&](int it) {
     int rel;
     if (group == 0) {
-      dma_raw<VBK>(tile_rsrc(a.k_pages, kres, it * kPT, VBK, rel), graw[it & 1], rel, gw, lane);
+      dma_raw<VBK>(tile_rsrc(a.k_pages, kres, pos(it), VBK, rel), graw[it & 1], rel, gw, lane);
       if constexpr (QJL) {
-        const __amdgpu_buffer_rsrc_t sr = tile_rsrc(a.s_pages, sres, it * kPT, SGB, rel);
+        const __amdgpu_buffer_rsrc_t sr = tile_rsrc(a.s_pages, sres, pos(it), SGB, rel);
         if (gw == 0 && 16 * lane < kPT * SGB)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (__attribute__((address_space(3))) void *)raw_s[it % 3], 16,
                                                    rel * SGB + 16 * lane, 0, 0, 0);
       }
     } else {
-      dma_raw<VBV>(tile_rsrc(a.v_pages, vres, it * kPT, VBV, rel), graw[it & 1], rel, gw, lane);
+      dma_raw<VBV>(tile_rsrc(a.v_pages, vres, pos(it), VBV, rel), graw[it & 1], rel, gw, lane);
     }
   };
   auto wait_dma = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
@@ -643,7 +676,10 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   const int64_t prow0 = ((int64_t)bh * a.qtiles + qtile) * (16 * RT * kPW);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float l = rows_sum(l_run[rt]);
+    float l = rows_sum(l_run[rt]);
+    if constexpr (WIN) {
+      if (q0 + (16 * RT * wave + 16 * rt + col) / G >= wr.count) l = 0.0f;
+    }
     if (splits > 1 && grp == 0)
       ((float2 *)a.part_ml)[(prow0 + 16 * RT * wave + 16 * rt + col) * splits + sp] = make_float2(m_run[rt], l);
     float f[4];
@@ -658,7 +694,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       else if (row < a.qt * G && tok < a.Sq) dst = a.o + (((int64_t)(b * a.Hq + h * G + head) * a.Sq) + tok) * D;
       else continue;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) dst[16 * nb + col] = oacc[rt][nb][i] * f[i];
+      for (int nb = 0; nb < NB; ++nb) {
+        // (a row past the count: 0 even where a position holds no number)
+        const float o = oacc[rt][nb][i] * f[i];
+        dst[16 * nb + col] = WIN && tok >= wr.count ? 0.0f : o;
+      }
     }
   }
 }
@@ -711,6 +751,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs a,
   for (s = 0; s + 8 <= splits; s += 8) join(eight, s);
   for (; s < splits; ++s) join(one, s);
   const float inv = L > 0.0f ? 1.0f / (L * kPlaneScale) : 0.0f;
+  if (a.win.size && L == 0.0f) o = (float4_t){0.f, 0.f, 0.f, 0.f};   // (a row past the count, as above)
   const int64_t head = h * a.G + rw % a.G;
   const int64_t orow = a.token_major ? ((int64_t)b * a.Sq + tk) * a.Hq + head : (b * a.Hq + head) * a.Sq + tk;
   *((float4_t *)(a.o + orow * D) + threadIdx.x % TR) = o * inv;
@@ -817,6 +858,46 @@ hipError_t launch_prefill(const PrefillArgs &a, int k_bits, int v_bits, hipStrea
   const dim3 grid(a.qtiles * a.splits * a.B * a.n_heads);
   if (a.d == 128) launch_pd<128>(a, k_bits, v_bits, grid, s);
   else launch_pd<64>(a, k_bits, v_bits, grid, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  return launch_prefill_merge(a, 0, a.B * a.n_heads, prefill_rows_per_block(a.qjl != nullptr || a.s_pages != nullptr), s);
+}
+
+template <int D, int BITS>
+static void launch_pwin(const PrefillArgs &a, dim3 grid, hipStream_t s) {
+  if (a.qjl != nullptr || a.s_pages != nullptr) prefill_mfma_kernel<D, BITS, BITS, true, true><<<grid, kPW * 64, 0, s>>>(a);
+  else prefill_mfma_kernel<D, BITS, BITS, false, true><<<grid, kPW * 64, 0, s>>>(a);
+}
+
+PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w, bool extra) {
+  PrefillPlan p{};
+  p.rows = prefill_rows_per_block(qjl);
+  p.qt = p.rows / (Hq / Hkv);
+  p.qtiles = (Sq - 1) / p.qt + 1;
+  p.splits = 1;
+  p.streams = B * Hkv;
+  if (!extra) return p;
+  // the most tiles that a row block can see
+  const int64_t seen = (int64_t)w.size + p.qt + 126, all = ((int64_t)S + kPT - 1) / kPT;
+  const int64_t tiles = std::min(seen / kPT + (w.sinks + kPT - 1) / kPT, all);
+  const int64_t blocks = (int64_t)p.qtiles * p.streams;
+  const int64_t splits = std::min<int64_t>(kTargetBlocks / blocks, tiles / 4);
+  if (splits > 1) {
+    p.splits = (int)splits;
+    p.part_rows = blocks * p.rows * splits;
+  }
+  return p;
+}
+
+hipError_t launch_prefill_window(const PrefillArgs &a, int bits, hipStream_t s) {
+  const dim3 grid(a.qtiles * a.splits * a.B * a.n_heads);
+  if (a.d == 128) {
+    if (bits == 4) launch_pwin<128, 4>(a, grid, s);
+    else launch_pwin<128, 2>(a, grid, s);
+  } else {
+    if (bits == 4) launch_pwin<64, 4>(a, grid, s);
+    else launch_pwin<64, 2>(a, grid, s);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   return launch_prefill_merge(a, 0, a.B * a.n_heads, prefill_rows_per_block(a.qjl != nullptr || a.s_pages != nullptr), s);

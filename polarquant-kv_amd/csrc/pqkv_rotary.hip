@@ -1,9 +1,15 @@
-// Rotary positions of queries and keys in one launch (pqkv_rotary).
+// Rotary positions of queries and keys in one launch (pqkv_rotary, pqkv_rotary_axes).
 //
 // Pair i of a head's first rot_dim coordinates turns by t = position * freq[i]:
 //   y_a = m (x_a cos t - x_b sin t),  y_b = m (x_a sin t + x_b cos t)
 // with (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) interleaved; the other
 // coordinates are copied. The gradient is the same with -t.
+//
+// With several axes of positions (time, height, width) each pair has one of
+// them; the table of the pairs' axes comes as a kernel argument, so nothing is
+// copied for it and a call can be captured. It is read once per sine and cosine,
+// not once per head: 64 + 8 heads x 32768 tokens on three axes take what they
+// take on one.
 //
 // The angle is a product in 64 bits, reduced to a fraction of a turn there
 // (a position of 10^6 turns the first pair 1.6 10^5 times: in 32 bits the
@@ -19,6 +25,8 @@
 // follows. 64 query and 8 key heads x 32768 tokens (d = 128, bf16): 240 us, 5.0
 // TB/s, what a copy of 1 GiB moves; 40 heads of 8 single tokens: 3.1 us, the
 // launch's own.
+#include <type_traits>
+
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
@@ -57,9 +65,12 @@ struct RotaryKernelArgs {
   int n_rot, n_rest;         // items of the turned and of the copied part
 };
 
+struct OneAxis {};
+
 // V elements of each of a pair's two sides per item (of a copied item: V in all).
-template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryKernelArgs k) {
+// AX: OneAxis, or RotaryAxes.
+template <typename T, int V, bool INTER, typename AX>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryKernelArgs k, const AX axes) {
   extern __shared__ __align__(8) float2 turn[];   // [tokens][rot_dim / 2]: m cos, m sin
   const RotaryArgs &a = k.a;
   const int half = a.rot_dim / 2;
@@ -69,7 +80,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryKernelArgs k) {
   const int nt = min(k.tokens, a.T - t0);
   for (int i = threadIdx.x; i < nt * half; i += 256) {
     const int t = i / half, p = i - t * half;
-    const double pos = (double)a.positions[(int64_t)b * a.pos_batch_stride + t0 + t];
+    int64_t row = (int64_t)b * a.pos_batch_stride;
+    if constexpr (!std::is_empty<AX>::value) row += axes.of[p] * axes.stride;
+    const double pos = (double)a.positions[row + t0 + t];
     const double turns = pos * (a.freqs[p] * 0.15915494309189533577);   // 1 / (2 pi)
     const float frac = (float)(turns - __builtin_rint(turns));
     float s, c;
@@ -116,8 +129,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryKernelArgs k) {
   }
 }
 
-template <typename T, int V>
-hipError_t launch(const RotaryArgs &a, hipStream_t s) {
+template <typename T, int V, typename AX>
+hipError_t launch(const RotaryArgs &a, const AX &axes, hipStream_t s) {
   const int H = a.Hq + a.Hkv, half = a.rot_dim / 2;
   const int n_rot = half / V, n_rest = (a.d - a.rot_dim) / V, per_head = n_rot + n_rest;
   // tokens of a workgroup: as many as leave 2048 workgroups, up to four; heads:
@@ -132,28 +145,35 @@ hipError_t launch(const RotaryArgs &a, hipStream_t s) {
   const RotaryKernelArgs k{a, FastDiv(per_head), FastDiv(heads), tokens, heads, n_rot, n_rest};
   const dim3 grid((unsigned)((int64_t)((a.T + tokens - 1) / tokens) * a.B), (H + heads - 1) / heads);
   const size_t lds = (size_t)tokens * half * sizeof(float2);
-  if (a.interleaved) rotary_kernel<T, V, true><<<grid, 256, lds, s>>>(k);
-  else rotary_kernel<T, V, false><<<grid, 256, lds, s>>>(k);
+  if (a.interleaved) rotary_kernel<T, V, true><<<grid, 256, lds, s>>>(k, axes);
+  else rotary_kernel<T, V, false><<<grid, 256, lds, s>>>(k, axes);
   return hipGetLastError();
 }
 
 // 16-byte items where every item of every row starts on a 16-byte boundary,
 // else an element at a time.
-template <typename T>
-hipError_t launch_type(const RotaryArgs &a, hipStream_t s) {
+template <typename T, typename AX>
+hipError_t launch_type(const RotaryArgs &a, const AX &axes, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.k | (uintptr_t)a.k_out;
   int64_t el = a.d | (a.rot_dim / 2);
   for (int i = 0; i < 3; ++i) el |= a.q_stride[i] | (a.Hkv ? a.k_stride[i] : 0);
-  return at % 16 == 0 && el % V == 0 ? launch<T, V>(a, s) : launch<T, 1>(a, s);
+  return at % 16 == 0 && el % V == 0 ? launch<T, V>(a, axes, s) : launch<T, 1>(a, axes, s);
+}
+
+template <typename AX>
+hipError_t launch_any(const RotaryArgs &a, const AX &axes, int dtype, hipStream_t s) {
+  if (dtype == PQKV_F32) return launch_type<float>(a, axes, s);
+  if (dtype == PQKV_F16) return launch_type<half_t>(a, axes, s);
+  return launch_type<bf16_t>(a, axes, s);
 }
 
 }  // namespace
 
-hipError_t launch_rotary(const RotaryArgs &a, int dtype, hipStream_t s) {
-  if (dtype == PQKV_F32) return launch_type<float>(a, s);
-  if (dtype == PQKV_F16) return launch_type<half_t>(a, s);
-  return launch_type<bf16_t>(a, s);
+hipError_t launch_rotary(const RotaryArgs &a, int dtype, hipStream_t s) { return launch_any(a, OneAxis{}, dtype, s); }
+
+hipError_t launch_rotary_axes(const RotaryArgs &a, const RotaryAxes &axes, int dtype, hipStream_t s) {
+  return launch_any(a, axes, dtype, s);
 }
 
 }  // namespace pqkv

@@ -410,6 +410,96 @@ def _prefill_paged(query, keys, values, rotation_matrix, q_start, causal, scale,
     return out
 
 
+def row_starts(starts, n: int, B: int, device) -> tuple:
+    """(start, starts) of a call's n new positions: a number for every sequence,
+    or int64 [B] on the device (a tensor of integers; the kernels read it)."""
+    if not isinstance(starts, torch.Tensor):
+        return int(starts), None
+    if tuple(starts.shape) != (B,) or starts.dtype.is_floating_point or starts.dtype.is_complex or \
+            starts.dtype == torch.bool:
+        raise ValueError(f"starts must be an integer or [{B}] integers, got {tuple(starts.shape)} {starts.dtype}")
+    if starts.device != device:
+        raise ValueError(f"starts are on {starts.device}, the call's tensors on {device}")
+    return 0, starts.to(torch.int64).contiguous()
+
+
+def row_counts(counts, B: int, device):
+    """int64 [B] on the device, or None."""
+    if counts is None:
+        return None
+    if not isinstance(counts, torch.Tensor) or tuple(counts.shape) != (B,) or counts.dtype.is_floating_point or \
+            counts.dtype.is_complex or counts.dtype == torch.bool:
+        raise ValueError(f"counts must be [{B}] integers on the device")
+    if counts.device != device:
+        raise ValueError(f"counts are on {counts.device}, the call's tensors on {device}")
+    return counts.to(torch.int64).contiguous()
+
+
+def window_attention(query: torch.Tensor, keys, values, rotation_matrix: torch.Tensor, window: int, *, sinks: int = 0,
+                     starts=None, counts: torch.Tensor | None = None, scale: float | None = None,
+                     jl_rot: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """query [B, Hq, Sq, d] against caches that already hold its tokens -> out
+    [B, Hq, Sq, d]: the row at position p attends to the `window` positions up to
+    p and to the first `sinks` ones (pqkv_window_attn, _paged). Its work is that of
+    the window, however long the cache.
+
+    starts: the position of each sequence's first row: a number for all, by
+    default the one that makes the cache's last positions the rows' (seq_len -
+    Sq), or a tensor of integers [B] on the device, for sequences of different
+    lengths: the kernels read it, so that a captured call follows it, and the
+    caches' own seq_len is not looked at. counts ([B], device): how many of the Sq
+    rows each sequence has, in a padded chunk. Rows past them, and rows at
+    positions that the caches have no room for, give zeros.
+
+    keys / values: PQCache or PagedPQCache of one and the same width."""
+    if query.dim() != 4:
+        raise ValueError(f"query must be [B, Hq, Sq, d], got {tuple(query.shape)}")
+    B, Hq, Sq, d = query.shape
+    paged = isinstance(keys, PagedPQCache) or isinstance(values, PagedPQCache)
+    Hkv = (check_paged if paged else check_shapes)(B, Hq, d, keys, values, rotation_matrix)
+    if keys.mixed or values.mixed or keys.n_bits != values.n_bits:
+        raise ValueError("a window takes keys and values of one and the same width")
+    if window != int(window) or window < 1 or sinks != int(sinks) or sinks < 0:
+        raise ValueError(f"window={window} must be at least 1, sinks={sinks} at least 0")
+    check_signs(jl_rot, keys, d)
+    _lib.require_device(query, rotation_matrix, jl_rot)
+    _lib.require_one_device(query, rotation_matrix, jl_rot, keys.codebooks, keys.table if paged else keys.blocks,
+                            values.codebooks, values.table if paged else values.blocks)
+    start, starts = row_starts(keys.seq_len - Sq if starts is None else starts, Sq, B, query.device)
+    counts = row_counts(counts, B, query.device)
+    if starts is None and not 0 <= start <= keys.seq_len - Sq:
+        raise ValueError(f"rows at positions {start}..{start + Sq - 1} of a cache of {keys.seq_len}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    out_dtype = query.dtype if out_dtype is None else out_dtype
+    q = query if query.is_contiguous() else query.contiguous()
+    R, P = _lib.dense_f32(rotation_matrix), _lib.dense_f32(jl_rot)
+    out = torch.empty_like(q, dtype=out_dtype)
+    if out.numel() == 0:
+        return out
+    lib = _lib.lib()
+    # positions that there is room for
+    S = min(keys.capacity, values.capacity) if paged else keys.max_seq_len
+    window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+    need = lib.pqkv_window_attn_workspace_bytes(B, Hq, Hkv, Sq, S, d, window, sinks, int(P is not None))
+    ws = torch.empty(need or 1, dtype=torch.uint8, device=q.device)
+    kcb, vcb = (keys.codebooks, values.codebooks) if paged else _codebook_tables(keys, values, False, Hkv)
+    tail = (_lib.ptr(P), d if P is not None else 0, B, Hq, Hkv, Sq, start, _lib.ptr(starts), _lib.ptr(counts), window,
+            sinks, S, d, scale, out.data_ptr(), _lib.dtype_code(out_dtype), ws.data_ptr(), ws.numel(),
+            _lib.stream_of(q))
+    head = (q.data_ptr(), _lib.dtype_code(q.dtype), R.data_ptr())
+    with _lib.on_device(q):
+        if paged:
+            ktab, vtab, stab, max_pages = page_tables(keys, values)
+            _lib.check(lib.pqkv_window_attn_paged(
+                *head, ktab.data_ptr(), vtab.data_ptr(), keys.page_tokens, max_pages, kcb.data_ptr(), vcb.data_ptr(),
+                keys.n_bits, stab.data_ptr() if P is not None else None, *tail))
+        else:
+            _lib.check(lib.pqkv_window_attn(
+                *head, keys.blocks.data_ptr(), values.blocks.data_ptr(), kcb.data_ptr(), vcb.data_ptr(), keys.n_bits,
+                keys.qjl_signs.data_ptr() if P is not None else None, *tail))
+    return out
+
+
 def _codebook_tables(keys: PQCache, values: PQCache, mixed: bool, Hkv: int):
     """The codebook pointers the kernels take: one [16] table each, or per-head
     [Hkv, 16] tables with mixed widths."""

@@ -7,8 +7,10 @@ differ.
 
   rotary_frequencies  radians per position of each pair, in 64 bits, with the
                       usual scalings for contexts longer than trained for
-  apply_rotary        q and k turned in one launch (pqkv_rotary), with its
-                      gradient
+  axis_of_pairs       which of several axes of positions (time, height,
+                      width) each pair turns by
+  apply_rotary        q and k turned in one launch (pqkv_rotary,
+                      pqkv_rotary_axes), with its gradient
   RotaryEmbedding     both for one head shape; what an attention layer takes
 """
 
@@ -92,6 +94,46 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
     return freqs * (1.0 - ramp + ramp / f), float(given) if given is not None else 0.1 * math.log(f) + 1.0
 
 
+def axis_of_pairs(sections, spread: bool = False) -> tuple:
+    """The axis of each of sum(sections) pairs, of which axis a has sections[a]:
+    in runs (the first sections[0] pairs turn by axis 0, the next ones by axis
+    1, ...) or, with spread, dealt out in turn: axis a has the pairs a, a + n,
+    a + 2 n, ... of n axes, and axis 0 all that the others leave."""
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0 or sum(sections) < 1 or len(sections) > 256:
+        raise ValueError(f"sections must be counts of pairs, got {sections}")
+    if not spread:
+        return tuple(a for a, s in enumerate(sections) for _ in range(s))
+    n, out = len(sections), [0] * sum(sections)
+    for a in range(1, n):
+        if sections[a] and a + n * (sections[a] - 1) >= len(out):
+            raise ValueError(f"sections {sections}: {len(out)} pairs dealt out in turn leave axis {a} fewer than "
+                             f"{sections[a]}")
+        for j in range(sections[a]):
+            out[a + n * j] = a
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=64)
+def _axis_table(axes: tuple) -> bytes:
+    """A call's table of axes, a byte per pair."""
+    if any(a != int(a) or not 0 <= a < 256 for a in axes):
+        raise ValueError(f"axes must be the numbers of axes, got {axes}")
+    return bytes(int(a) for a in axes)
+
+
+def check_axes(axes, positions: torch.Tensor, pairs: int, B: int, T: int) -> bytes:
+    """The table of axes (one number per pair) that goes with positions [axes, T]
+    or [axes, B, T]."""
+    table = _axis_table(tuple(axes))
+    if len(table) != pairs:
+        raise ValueError(f"{len(table)} axes for {pairs} frequencies")
+    n = max(table) + 1
+    if positions.dim() not in (2, 3) or tuple(positions.shape[1:]) not in ((T,), (B, T)) or positions.shape[0] < n:
+        raise ValueError(f"positions must be [>= {n}, {T}] or [>= {n}, {B}, {T}], got {tuple(positions.shape)}")
+    return table
+
+
 def _code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return _lib.BF16
@@ -107,9 +149,19 @@ def _strides(x: torch.Tensor):
     return _int64_3(*x.stride()[:3])       # (read-only to the call)
 
 
-def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):
+def position_strides(positions: torch.Tensor, axes):
+    """(integers between axes, between sequences, axes) of positions with dense
+    rows [T] or [B, T], with axes [A, T] or [A, B, T]; 0 between sequences that share
+    a row."""
+    if axes is None:
+        return 0, positions.stride(0) if positions.dim() == 2 else 0, 1
+    return positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0, positions.shape[0]
+
+
+def _turn(q, k, positions, freqs, interleaved, amplitude, inverse, *axes):
     """The launch: q [B, Hq, T, d] and k [B, Hkv, T, d] (or None) -> contiguous
-    turned copies."""
+    turned copies. axes: the table of axes, where there are several."""
+    axes = axes[0] if axes else None
     q = q if q.stride(-1) == 1 or q.numel() == 0 else q.contiguous()
     qo = torch.empty_like(q, memory_format=torch.contiguous_format)    # (half of torch.empty's host time)
     ko, ks, Hkv = None, None, 0
@@ -118,11 +170,15 @@ def _turn(q, k, positions, freqs, interleaved, amplitude, inverse):
         ko = torch.empty_like(k, memory_format=torch.contiguous_format)
         ks, Hkv = _strides(k), k.shape[1]
     B, Hq, T, d = q.shape
+    by_axis, by_row, n_axes = position_strides(positions, axes)
+    head = (q.data_ptr(), _strides(q), qo.data_ptr(), Hq, _lib.ptr(k), ks, _lib.ptr(ko), Hkv, _code(q),
+            positions.data_ptr())
+    tail = (freqs.data_ptr(), B, T, d, 2 * freqs.numel(), int(interleaved), amplitude, int(inverse), _lib.stream_of(q))
     with _lib.on_device(q):
-        _lib.check(_lib.lib().pqkv_rotary(
-            q.data_ptr(), _strides(q), qo.data_ptr(), Hq, _lib.ptr(k), ks, _lib.ptr(ko), Hkv, _code(q),
-            positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0, freqs.data_ptr(), B, T, d,
-            2 * freqs.numel(), int(interleaved), amplitude, int(inverse), _lib.stream_of(q)))
+        if axes is None:
+            _lib.check(_lib.lib().pqkv_rotary(*head, by_row, *tail))
+        else:
+            _lib.check(_lib.lib().pqkv_rotary_axes(*head, by_axis, by_row, n_axes, axes, *tail))
     return qo, ko
 
 
@@ -135,23 +191,23 @@ def _has_tangent(*tensors) -> bool:
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse):
+    def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse, *axes):
         ctx.save_for_backward(positions, freqs)
-        ctx.how = (interleaved, amplitude, not inverse)
+        ctx.how = (interleaved, amplitude, not inverse, *axes)
         if forward_ad._current_level >= 0:
             ctx.save_for_forward(positions, freqs)
             ctx.shapes, ctx.dtype = (q.shape, None if k is None else k.shape), q.dtype
         ctx.set_materialize_grads(False)
-        return _turn(q, k, positions, freqs, interleaved, amplitude, inverse)
+        return _turn(q, k, positions, freqs, interleaved, amplitude, inverse, *axes)
 
     @staticmethod
     def jvp(ctx, tq, tk, *_):
         # y = M x: the tangent is M times x's (which may be of another type)
-        interleaved, amplitude, back = ctx.how
+        interleaved, amplitude, back, *axes = ctx.how
         turn = _Rotary.apply if torch.is_grad_enabled() else _turn
         _lib.require_one_device(tq, tk, *ctx.saved_tensors)            # (make_dual takes any)
         moving = [t.to(ctx.dtype) for t in (tq, tk) if t is not None]
-        out = list(turn(*(moving + [None])[:2], *ctx.saved_tensors, interleaved, amplitude, not back))
+        out = list(turn(*(moving + [None])[:2], *ctx.saved_tensors, interleaved, amplitude, not back, *axes))
         return tuple(None if shape is None else moving[0].new_zeros(shape) if t is None else out.pop(0)
                      for t, shape in zip((tq, tk), ctx.shapes))
 
@@ -164,25 +220,26 @@ class _Rotary(torch.autograd.Function):
         if not ctx.needs_input_grad[1]:
             gk = None
         if gq is None and gk is None:
-            return (None,) * 7
+            return (None,) * (4 + len(ctx.how))
         # (create_graph, or gradients with tangents: differentiable again)
         turn = _Rotary.apply if torch.is_grad_enabled() or _has_tangent(gq, gk) else _turn
         if gq is None:
             out = (None, turn(gk, None, *ctx.saved_tensors, *ctx.how)[0])
         else:
             out = turn(gq, gk, *ctx.saved_tensors, *ctx.how)
-        return *out, None, None, None, None, None
+        return *out, None, None, *[None] * len(ctx.how)
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,
-                 interleaved: bool = False, amplitude: float = 1.0):
+                 interleaved: bool = False, amplitude: float = 1.0, axes=None):
     """query [B, Hq, T, d] and key [B, Hkv, T, d] (or None) with the first
     2 * len(frequencies) coordinates of every head turned by positions *
     frequencies: -> (query, key), contiguous, in the inputs' type (fp16, bf16
     or fp32; one for both). positions: integers [T] or [B, T]; frequencies:
     radians per position, float64 (rotary_frequencies, on the device). Pairs
-    are (i, i + rot_dim / 2), or neighbours with interleaved. The inputs may
-    have any strides and may be expanded; gradients flow to both, and
+    are (i, i + rot_dim / 2), or neighbours with interleaved. axes (a sequence of
+    numbers, one per frequency; axis_of_pairs): pair i turns by the positions of
+    axis axes[i], which are [A, T] or [A, B, T] then. The inputs may have any strides and may be expanded; gradients flow to both, and
     forward-mode tangents (torch.autograd.forward_ad) through them."""
     for name, x in (("query", query), ("key", key)):
         if x is not None and x.dim() != 4:
@@ -202,43 +259,67 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"{2 * frequencies.numel()} turned coordinates of a head of {d}")
     if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
         raise ValueError(f"positions must be integers, got {positions.dtype}")
-    if tuple(positions.shape) not in ((T,), (B, T)):
+    if axes is not None:
+        axes = (check_axes(axes, positions, frequencies.numel(), B, T),)
+    elif tuple(positions.shape) not in ((T,), (B, T)):
         raise ValueError(f"positions must be [{T}] or [{B}, {T}], got {tuple(positions.shape)}")
-    args = (query, key, positions.to(torch.int64).contiguous(), frequencies.contiguous(), bool(interleaved),
-            float(amplitude))
+    positions = positions.to(torch.int64)
+    if axes is None or positions.stride(-1) != 1:      # (rows of axes may be one row seen several times)
+        positions = positions.contiguous()
+    args = (query, key, positions, frequencies.contiguous(), bool(interleaved),
+            float(amplitude), False, *(axes or ()))
     if (torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))) or \
             _has_tangent(query, key):
-        return _Rotary.apply(*args, False)
-    return _turn(*args, False)
+        return _Rotary.apply(*args)
+    return _turn(*args)
 
 
 class RotaryEmbedding:
     """apply_rotary with the frequencies of one head shape: rot_dim (default:
     the whole head) of head_dim coordinates, base, scaling and pairing as
-    rotary_frequencies and apply_rotary take them. The first call on a device
+    rotary_frequencies and apply_rotary take them. sections: how many pairs each
+    of several axes of positions has, spread as axis_of_pairs takes it; positions
+    have an axis in front then, or none where all axes are alike (text). The
+    first call on a device
     copies the frequencies to it, which a graph capture does not allow: such a
     call is refused there."""
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, base: float = 10000.0, scaling: dict | None = None,
-                 interleaved: bool = False):
+                 interleaved: bool = False, sections=None, spread: bool = False):
         self.head_dim = head_dim
         self.rot_dim = head_dim if rot_dim is None else int(rot_dim)
         if self.rot_dim > head_dim:
             raise ValueError(f"rot_dim {rot_dim} exceeds head_dim {head_dim}")
         self.interleaved = interleaved
+        self.axes = None if sections is None else axis_of_pairs(sections, spread)
+        if self.axes is not None and len(self.axes) != self.rot_dim // 2:
+            raise ValueError(f"sections {list(sections)} are {len(self.axes)} pairs of {self.rot_dim // 2}")
+        self.n_axes = 1 if sections is None else len(sections)
         with torch.inference_mode(False):
             self.frequencies, self.amplitude = rotary_frequencies(self.rot_dim, base, scaling)
         self._on: dict = {}            # the frequencies on each device used
 
-    def __call__(self, query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor):
-        freqs = self._on.get(query.device)
+    def frequencies_on(self, device: torch.device) -> torch.Tensor:
+        """The frequencies on a device."""
+        freqs = self._on.get(device)
         if freqs is None:
-            if query.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"call the embedding on {query.device} once before a capture")
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"call the embedding on {device} once before a capture")
             # they serve later calls, which may be differentiated whatever mode this one runs in
             with torch.inference_mode(False):
-                freqs = self._on[query.device] = self.frequencies.to(query.device)
-        return apply_rotary(query, key, positions, freqs, interleaved=self.interleaved, amplitude=self.amplitude)
+                freqs = self._on[device] = self.frequencies.to(device)
+        return freqs
+
+    def positions_by_axis(self, positions: torch.Tensor) -> torch.Tensor:
+        """Positions [T] with the axis in front that several axes take: of text,
+        whose axes are alike."""
+        if self.axes is None or positions.dim() != 1:
+            return positions
+        return positions.expand(self.n_axes, -1)
+
+    def __call__(self, query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor):
+        return apply_rotary(query, key, self.positions_by_axis(positions), self.frequencies_on(query.device),
+                            interleaved=self.interleaved, amplitude=self.amplitude, axes=self.axes)
 
 
-__all__ = ["rotary_frequencies", "apply_rotary", "RotaryEmbedding"]
+__all__ = ["rotary_frequencies", "axis_of_pairs", "apply_rotary", "RotaryEmbedding"]
