@@ -484,6 +484,52 @@ int pqkv_rotary_axes(const void *q, const int64_t q_strides[3], void *q_out, int
                      const double *freqs, int B, int T, int d, int rot_dim, int interleaved, float amplitude,
                      int inverse, void *stream);
 
+/* ---- appending with the rotation on the way ------------------------------------
+ * No counterpart in the reference, which has no positions and appends by
+ * concatenation (src/polarquant_kv_cuda/inference/kv_cache.py:96-116). The T new
+ * keys of every sequence are turned by their positions (as pqkv_rotary turns
+ * them, but not rounded), encoded (rotated by R, radius, nearest centroids) and
+ * written into slots start_b .. start_b + T - 1 of their streams, the values the
+ * same without the turn, in one launch. k, v [B][Hkv][T][d] with element strides
+ * {sequence, head, token} (any; the last dimension is dense) of dtype PQKV_F32,
+ * PQKV_F16 or PQKV_BF16; positions, frequencies, axes, rot_dim, interleaved and
+ * amplitude as pqkv_rotary_axes takes them (axes NULL: one axis).
+ *
+ * starts: int64 [B] on the device, or NULL: `start` for every sequence; counts:
+ * int64 [B] on the device, or NULL: T; how many of its T tokens sequence b has.
+ * Both are read by the kernel, so a captured call follows them. A token past its
+ * sequence's count, or whose slot is outside 0 .. S - 1 (S: the slots there are
+ * room for; with starts NULL start + T <= S is required) is not written, and
+ * nothing else of the cache is. Keys and values of one width n_bits (2 or 4),
+ * blocks [B][Hkv][S][vector bytes]. p_rot = P R^T and qjl_signs
+ * [B][Hkv][S][d / 8] (m = d; both or neither) also write the keys' signs.
+ *
+ * The rotation runs in fp16 parts with fp32 sums (about 2^-22 of the operands'
+ * norms): codes and radii differ from pqkv_encode's where a direction lies that
+ * close to a border, and, for 16-bit inputs, where the rounding of the turned key
+ * to them moves it across one. R is orthogonal (entries up to 1). A vector that
+ * holds a number that is not finite gets radius NaN (codes 0); norms above 65504
+ * are stored as that. q (or NULL): [B][Hq][T][d], turned and rounded to dtype into
+ * q_out as pqkv_rotary_axes does. */
+int pqkv_append_rotary(const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                       const void *q, const int64_t q_strides[3], void *q_out, int Hq, int dtype,
+                       const int64_t *positions, int64_t positions_axis_stride, int64_t positions_stride, int n_axes,
+                       const uint8_t *axes, const double *freqs, int rot_dim, int interleaved, float amplitude,
+                       const float *R, const float *k_codebook, const float *v_codebook, int n_bits,
+                       const float *p_rot, int m, int B, int Hkv, int T, int d, int64_t start, const int64_t *starts,
+                       const int64_t *counts, int S, uint8_t *k_blocks, uint8_t *v_blocks, uint8_t *qjl_signs,
+                       void *stream);
+/* The same into a paged cache (as pqkv_encode_paged) whose pages hold S slots. */
+int pqkv_append_rotary_paged(const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                             const void *q, const int64_t q_strides[3], void *q_out, int Hq, int dtype,
+                             const int64_t *positions, int64_t positions_axis_stride, int64_t positions_stride,
+                             int n_axes, const uint8_t *axes, const double *freqs, int rot_dim, int interleaved,
+                             float amplitude, const float *R, const float *k_codebook, const float *v_codebook,
+                             int n_bits, const float *p_rot, int m, int B, int Hkv, int T, int d, int64_t start,
+                             const int64_t *starts, const int64_t *counts, int S, uint8_t *const *k_pages,
+                             uint8_t *const *v_pages, int page_tokens, int max_pages, uint8_t *const *qjl_pages,
+                             void *stream);
+
 /* ---- attention behind a window ----------------------------------------------
  * No counterpart in the reference. The Sq query rows of sequence b stand at
  * positions start_b .. start_b + Sq - 1 of a cache that holds them, and the one at

@@ -452,6 +452,27 @@ struct RotaryAxes {
 int rotary_axes(const char *what, const uint8_t *axes, int n_axes, int rot_dim, int64_t stride, RotaryAxes *out);
 hipError_t launch_rotary_axes(const RotaryArgs &a, const RotaryAxes &axes, int dtype, hipStream_t s);
 
+// Appending to a cache with the rotation on the way (pqkv_append_rotary). S: the
+// cache's slots per stream; the page tables (k_pages set) or the contiguous
+// arrays.
+struct AppendArgs {
+  const void *k, *v;
+  int64_t k_stride[3], v_stride[3];
+  const int64_t *positions;
+  int64_t pos_batch_stride;
+  const double *freqs;
+  const float *R, *k_cb, *v_cb, *p_rot;
+  uint8_t *k_blocks, *v_blocks, *signs;
+  uint8_t *const *k_pages, *const *v_pages, *const *s_pages;
+  int page_shift, max_pages;
+  const int64_t *starts, *counts;
+  int64_t start;
+  int B, Hkv, T, d, S, rot_dim, interleaved, bits, vec_bytes;
+  float amplitude;
+  RotaryAxes axes;
+};
+hipError_t launch_append(const AppendArgs &a, int dtype, hipStream_t s);
+
 // Eviction: selection, and the move of up to PQKV_MAX_GATHER arrays' rows.
 hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_streams, int S, int keep, int sink,
                                int recent, int *kept, hipStream_t s);

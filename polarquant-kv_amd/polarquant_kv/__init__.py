@@ -13,6 +13,7 @@ python/polarquant_kv and src/polarquant_kv_cuda) for the codebook
   inference  PolarQuantConfig, KVCacheManager, CompressedMultiHeadAttention
   hf_integration CompressedDynamicCache, patch_model
   rotary     apply_rotary, RotaryEmbedding, rotary_frequencies    (HIP)
+  append     append_rotary                                       (HIP)
   eviction   evict, select_positions, gather_positions           (HIP)
   policies   compute_token_bitwidths, compute_layer_bitwidths, TokenMixedCache,
              differential_encode, ...                            (HIP for the cache)
@@ -30,7 +31,7 @@ def __getattr__(name):
     # GPU modules load libpqkv_hip.so lazily so the host-side API imports
     # on machines without a GPU.
     if name in ("attention", "quantizer", "turboquant", "inference", "hf_integration", "policies", "rotary",
-                "eviction"):
+                "eviction", "append"):
         import importlib
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

@@ -137,6 +137,15 @@ SIGNATURES = {
     "pqkv_rotary_axes": (c_int, [c_void_p, c_int64_p, c_void_p, c_int, c_void_p, c_int64_p, c_void_p, c_int, c_int,
                                  c_void_p, c_int64, c_int64, c_int, ctypes.c_char_p, c_void_p, c_int, c_int, c_int,
                                  c_int, c_int, c_float, c_int, c_void_p]),
+    "pqkv_append_rotary": (c_int, [c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int, c_int,
+                                   c_void_p, c_int64, c_int64, c_int, ctypes.c_char_p, c_void_p, c_int, c_int, c_float,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                   c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pqkv_append_rotary_paged": (c_int, [c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int,
+                                         c_int, c_void_p, c_int64, c_int64, c_int, ctypes.c_char_p, c_void_p, c_int,
+                                         c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
+                                         c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                         c_int, c_int, c_void_p, c_void_p]),
     "pqkv_window_attn_workspace_bytes": (c_size_t, [c_int] * 9),
     "pqkv_window_attn": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                  c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_int, c_int,
