@@ -33,7 +33,10 @@ Differences, all on purpose:
     got (track_weights) and cut its caches to the heaviest ones (evict), so a
     sequence may grow past max_seq_len cached positions;
   - the attention layer can turn its queries and keys by their positions
-    (rotary), which the manager counts apart from the slots of its caches.
+    (rotary), which the manager counts apart from the slots of its caches;
+  - it can look at a window of the last positions and the first few (window,
+    sinks): a step's work then is that of the window. Behind a window the keys
+    are turned on their way into the cache (append_rotary).
 All GPU work goes through libpqkv_hip.so.
 """
 
@@ -44,7 +47,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, attention, quantizer
+from . import _lib, append, attention, quantizer
 from .types import PagedPQCache
 
 
@@ -174,6 +177,18 @@ class KVCacheManager:
         (pages are added as the positions need them)."""
         if key.shape != value.shape or key.dim() != 4:
             raise ValueError("key and value must both be [batch, num_heads, new_seq, head_dim]")
+        T = self._prepare(key)
+        if self.config.enable_compression:
+            quantizer.compress_pq(key, self.R, cache=self._keys, start=self._seq_len, jl_rot=self.jl_rot)
+            quantizer.compress_pq(value, self.R, cache=self._values, start=self._seq_len)
+        else:
+            self._key_cache[:, :, self._seq_len:self._seq_len + T] = key.to(torch.float16)
+            self._value_cache[:, :, self._seq_len:self._seq_len + T] = value.to(torch.float16)
+        self._seq_len += T
+        self._next_position += T
+
+    def _prepare(self, key: torch.Tensor) -> int:
+        """Checks and room for the tokens of key, whose number it returns."""
         B, H, T, d = key.shape
         if (B, H, d) != (self.batch, self.num_heads, self.head_dim):
             raise ValueError(f"shape {tuple(key.shape)} does not match the cache "
@@ -184,14 +199,35 @@ class KVCacheManager:
             self._allocate()
         if self.track_weights:                 # (first: if it fails, nothing is in the caches)
             self._track(T)
-        if self.config.enable_compression:
-            quantizer.compress_pq(key, self.R, cache=self._keys, start=self._seq_len, jl_rot=self.jl_rot)
-            quantizer.compress_pq(value, self.R, cache=self._values, start=self._seq_len)
-        else:
-            self._key_cache[:, :, self._seq_len:self._seq_len + T] = key.to(torch.float16)
-            self._value_cache[:, :, self._seq_len:self._seq_len + T] = value.to(torch.float16)
+        return T
+
+    def append_rotary(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, rotary,
+                      positions: torch.Tensor | None = None) -> torch.Tensor:
+        """append() of keys that are turned on their way into the cache by a
+        rotary.RotaryEmbedding, with the query [batch, q_heads, new_seq,
+        head_dim] turned and returned: what rotary(query, key) and append() do,
+        but for the rounding of the turned keys in between
+        (append.append_rotary). positions: as the embedding takes them, by default
+        next_position .. . Any strides; fp16, bf16 or fp32."""
+        if key.shape != value.shape or key.dim() != 4:
+            raise ValueError("key and value must both be [batch, num_heads, new_seq, head_dim]")
+        if positions is None:
+            positions = torch.arange(self._next_position, self._next_position + key.shape[2], device=key.device)
+        if not self.config.enable_compression:
+            query, key = rotary(query, key, positions)
+            self.append(key, value)
+            return query
+        T = self._prepare(key)
+        with _lib.lasting():                   # (pages that this adds are written in any mode)
+            self._keys.ensure(self._seq_len + T)
+            self._values.ensure(self._seq_len + T)
+        out = append.append_rotary(key, value, self._keys, self._values, self.R, rotary.positions_by_axis(positions),
+                                   rotary.frequencies_on(key.device), query=query, starts=self._seq_len,
+                                   interleaved=rotary.interleaved, amplitude=rotary.amplitude, axes=rotary.axes,
+                                   jl_rot=self.jl_rot)
         self._seq_len += T
         self._next_position += T
+        return out
 
     def _track(self, T: int) -> None:
         """Slots seq_len .. seq_len + T - 1: no weight yet, and the next positions."""
@@ -250,12 +286,17 @@ class KVCacheManager:
         return r
 
     # ---- reads ----
-    def attend(self, query: torch.Tensor, causal: bool = True) -> torch.Tensor:
+    def attend(self, query: torch.Tensor, causal: bool = True, window: int | None = None,
+               sinks: int = 0) -> torch.Tensor:
         """query [batch, q_heads, Sq, head_dim] for the last Sq cached
         positions -> [batch, q_heads, Sq, head_dim] fp16: compressed
         attention (decode for Sq = 1, causal prefill otherwise) with the QJL
         term when the manager keeps signs. With track_weights the queries'
-        weights are added to those of the cached positions."""
+        weights are added to those of the cached positions. window: each query
+        looks at so many positions up to its own and at the first `sinks`
+        (attention.window_attention; causal, without track_weights)."""
+        if window is not None and (not causal or self.track_weights):
+            raise ValueError("a window is causal, and its weights are not tracked")
         if self._seq_len == 0:
             return torch.zeros_like(query, dtype=torch.float16)
         if not self.config.enable_compression:
@@ -265,13 +306,16 @@ class KVCacheManager:
             v = v.float().repeat_interleave(rep, 1)
             Sq, S = query.shape[2], k.shape[2]
             s = torch.matmul(query.float(), k.transpose(-1, -2).contiguous()) / math.sqrt(self.head_dim)
-            if causal and Sq > 1:
+            if causal and (Sq > 1 or window is not None):
                 pos = torch.arange(S, device=query.device)
                 qpos = torch.arange(S - Sq, S, device=query.device)
-                s = s.masked_fill(pos[None, :] > qpos[:, None], float("-inf"))
+                s = s.masked_fill(_hidden(pos, qpos, window, sinks), float("-inf"))
             return torch.matmul(torch.softmax(s, -1), v).half()
         Sq = query.shape[2]
         start = self._seq_len - Sq
+        if window is not None:
+            return attention.window_attention(query, self._keys, self._values, self.R, window, sinks=sinks,
+                                              starts=start, jl_rot=self.jl_rot, out_dtype=torch.float16)
         if self.track_weights:
             w = self._weights
             if Sq == 1:
@@ -290,15 +334,30 @@ class KVCacheManager:
                                                   causal=causal, q_start=start)
 
 
+def _hidden(pos, qpos, window, sinks):
+    """[rows, positions]: what a row does not see, of a causal or (window) a
+    windowed attention."""
+    late = pos[None, :] > qpos[:, None]
+    if window is None:
+        return late
+    return late | ((pos[None, :] <= qpos[:, None] - window) & (pos[None, :] >= sinks))
+
+
 class CompressedMultiHeadAttention(torch.nn.Module):
     """Multi-head (GQA) attention whose KV cache is the compressed one
     (src/polarquant_kv_cuda/inference/attention.py:12-95). rotary
     (rotary.RotaryEmbedding of the head's size): queries and keys turned by
-    their positions before the keys are cached."""
+    their positions before the keys are cached. window, sinks: each token looks
+    at the last `window` positions and the first `sinks`; keys are then turned on
+    their way into the cache (KVCacheManager.append_rotary)."""
 
     def __init__(self, config: PolarQuantConfig, embed_dim: int, num_heads: int, num_kv_heads: int | None = None,
-                 causal: bool = True, rotary=None):
+                 causal: bool = True, rotary=None, window: int | None = None, sinks: int = 0):
         super().__init__()
+        if window is not None and (window < 1 or sinks < 0 or not causal):
+            raise ValueError(f"window={window} (at least 1) and sinks={sinks} (at least 0) are for causal layers")
+        self.window = window
+        self.sinks = sinks
         self.config = config
         self.rotary = rotary
         self.causal = causal
@@ -313,28 +372,38 @@ class CompressedMultiHeadAttention(torch.nn.Module):
         self.v_proj = torch.nn.Linear(embed_dim, self.num_kv_heads * self.head_dim, bias=False)
         self.o_proj = torch.nn.Linear(num_heads * self.head_dim, embed_dim, bias=False)
 
-    def forward(self, x: torch.Tensor, cache_manager: KVCacheManager | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cache_manager: KVCacheManager | None = None,
+                positions: torch.Tensor | None = None) -> torch.Tensor:
         """x [batch, seq_len, embed_dim] -> [batch, seq_len, embed_dim]. With a
         cache manager the new keys and values are appended and the queries
-        attend to everything cached (causally unless causal=False)."""
+        attend to everything cached (causally unless causal=False). positions
+        of the tokens, as the rotary embedding takes them: by default the ones
+        after those cached."""
         B, T, _ = x.shape
         q = self.q_proj(x).reshape(B, T, self.num_heads, self.head_dim).transpose(1, 2).half()
         k = self.k_proj(x).reshape(B, T, self.num_kv_heads, self.head_dim).transpose(1, 2).half()
         v = self.v_proj(x).reshape(B, T, self.num_kv_heads, self.head_dim).transpose(1, 2).half()
-        if self.rotary is not None:
-            start = 0 if cache_manager is None else cache_manager.next_position
-            q, k = self.rotary(q, k, torch.arange(start, start + T, device=x.device))
+        on_the_way = self.rotary is not None and self.window is not None and cache_manager is not None
+        if self.rotary is not None and not on_the_way:
+            if positions is None:
+                start = 0 if cache_manager is None else cache_manager.next_position
+                positions = torch.arange(start, start + T, device=x.device)
+            q, k = self.rotary(q, k, positions)
         if cache_manager is not None:
-            cache_manager.append(k.contiguous(), v.contiguous())
-            out = cache_manager.attend(q.contiguous(), causal=self.causal)
+            if on_the_way:
+                q = cache_manager.append_rotary(q, k, v, self.rotary, positions)
+            else:
+                cache_manager.append(k.contiguous(), v.contiguous())
+            behind = {} if self.window is None else {"window": self.window, "sinks": self.sinks}
+            out = cache_manager.attend(q.contiguous(), causal=self.causal, **behind)
         else:
             rep = self.num_heads // self.num_kv_heads
             kk = k.float().repeat_interleave(rep, 1)
             vv = v.float().repeat_interleave(rep, 1)
             s = torch.matmul(q.float(), kk.transpose(-1, -2).contiguous()) / math.sqrt(self.head_dim)
             if self.causal:
-                mask = torch.ones(T, T, dtype=torch.bool, device=x.device).triu(1)
-                s = s.masked_fill(mask, float("-inf"))
+                pos = torch.arange(T, device=x.device)
+                s = s.masked_fill(_hidden(pos, pos, self.window, self.sinks), float("-inf"))
             out = torch.matmul(torch.softmax(s, -1), vv).half()
         out = out.transpose(1, 2).reshape(B, T, -1)
         return self.o_proj(out.to(self.o_proj.weight.dtype))
