@@ -580,6 +580,15 @@ int pqkv_dequantize_rows(const uint8_t *blocks, int64_t blocks_outer_stride, con
                          const float *R, void *out, int out_dtype, int64_t out_outer_stride, int64_t n_outer,
                          int64_t n_inner, int d, void *stream);
 
+/* The same without the rotation, out of a cache as it lies: out[s][t] = r16 c[code]
+ * for the slots t < S of n_streams streams, which start s * stride bytes into
+ * blocks or, with pages, are found through the table (as pqkv_encode_paged;
+ * blocks and stride unused). Equal to pqkv_dequantize with R = I. out
+ * [n_streams][S][d] fp32/fp16, 16-byte aligned. */
+int pqkv_dequantize_slots(const uint8_t *blocks, int64_t stride, const uint8_t *const *pages, int page_tokens,
+                          int max_pages, const float *codebook, int n_bits, void *out, int out_dtype,
+                          int64_t n_streams, int S, int d, void *stream);
+
 /* ---- layout converters ---------------------------------------------------
  * SoA (the reference kernels' format: packed u8 [n][d/2] + fp32 radius [n],
  * csrc/flash_turboquant.cu:29-32) <-> block_pq4. 4-bit codes only. */

@@ -32,7 +32,7 @@ SOURCES = ["pqkv_encode.hip", "pqkv_rotate_mfma.hip", "pqkv_encode_chain.hip", "
            "pqkv_decode_mfma_window_k2v2.hip", "pqkv_decode_mfma_window_paged_k4v4_shared.hip",
            "pqkv_decode_mfma_window_paged_k4v4_own.hip", "pqkv_decode_mfma_window_paged_k2v2.hip",
            "pqkv_weights.hip", "pqkv_evict.hip", "pqkv_rotary.hip", "pqkv_budget_api.cpp", "pqkv_window_api.cpp",
-           "pqkv_append.hip", "pqkv_append_api.cpp", "pqkv_prefill.hip", "pqkv_prefill_planes.hip", "pqkv_group.hip", "pqkv_group_gpu.hip", "pqkv_group_mfma.hip", "pqkv_group_api.cpp",
+           "pqkv_append.hip", "pqkv_append_api.cpp", "pqkv_slots.hip", "pqkv_prefill.hip", "pqkv_prefill_planes.hip", "pqkv_group.hip", "pqkv_group_gpu.hip", "pqkv_group_mfma.hip", "pqkv_group_api.cpp",
            "pqkv_api.cpp", "pqkv_compat.cpp", "pqkv_ggml.cpp", "pqkv_noalloc.hip"]
 
 

@@ -1,4 +1,4 @@
-// C ABI of appending with the rotation on the way. Host code: validation and
+// C ABI of appending with the rotation on the way, and of reading slots back. Host code: validation and
 // launches.
 #include <hip/hip_runtime.h>
 
@@ -118,6 +118,32 @@ int append_run(const char *what, const void *k, const int64_t k_strides[3], cons
 }  // namespace
 
 extern "C" {
+
+int pqkv_dequantize_slots(const uint8_t *blocks, int64_t stride, const uint8_t *const *pages, int page_tokens,
+                          int max_pages, const float *codebook, int n_bits, void *out, int out_dtype,
+                          int64_t n_streams, int S, int d, void *stream) {
+  if (n_streams < 0 || S < 0) return fail_status(PQKV_ERR_INVALID, "dequantize_slots: n_streams=%lld S=%d", (long long)n_streams, S);
+  if (d != 64 && d != 128) return fail_status(PQKV_ERR_UNSUPPORTED, "dequantize_slots: d=%d", d);
+  if (n_bits != 2 && n_bits != 4) return fail_status(PQKV_ERR_UNSUPPORTED, "dequantize_slots: n_bits=%d", n_bits);
+  if (out_dtype != PQKV_F32 && out_dtype != PQKV_F16) return fail_status(PQKV_ERR_UNSUPPORTED, "dequantize_slots: dtype");
+  int shift = 0;
+  if (pages) {
+    shift = pqkv::paged_validate("dequantize_slots", page_tokens, max_pages, S);
+    if (shift < 0) return shift;
+  }
+  if (n_streams == 0 || S == 0) return PQKV_OK;
+  if ((!blocks && !pages) || !codebook || !out) return fail_status(PQKV_ERR_INVALID, "dequantize_slots: null pointer");
+  if ((uintptr_t)blocks % 2 || (!pages && stride % 2) || (uintptr_t)out % 16)
+    return fail_status(PQKV_ERR_INVALID, "dequantize_slots: unaligned pointer");
+  if (!pages && stride < S * pqkv_vector_bytes(d, n_bits))
+    return fail_status(PQKV_ERR_INVALID, "dequantize_slots: stride %lld below a stream's bytes", (long long)stride);
+  if (n_streams > 0xFFFFFFFFll / S) return fail_status(PQKV_ERR_UNSUPPORTED, "dequantize_slots: n_streams=%lld S=%d", (long long)n_streams, S);
+  const pqkv::SlotsArgs a{blocks, stride, pages, shift, max_pages, codebook, out, n_streams * S, S};
+  const int tok = pqkv::prof_begin("dequantize_slots", (hipStream_t)stream);
+  const hipError_t e = pqkv::launch_slots(a, d, n_bits, out_dtype, (hipStream_t)stream);
+  pqkv::prof_end(tok, (hipStream_t)stream);
+  return report_hip_error(e, "dequantize_slots launch");
+}
 
 int pqkv_append_rotary(const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
                        const void *q, const int64_t q_strides[3], void *q_out, int Hq, int dtype,

@@ -153,7 +153,7 @@ __device__ __forceinline__ void build_cell_table(const float *cb, int nl, int ti
   // the range, and the first that passes closes it (keys of fp32 values
   // differ by < 2^32, so 8 steps reach a range of one; a wave with no open
   // range leaves the loop).
-  {
+  if (NT == 256 || tid < 256) {                   // (whole waves)
     const int i = tid >> 4, j = tid & 15;
     const bool act = i < nl - 1;
     const float ci = act ? cb[i] : 0.0f, cn = act ? cb[i + 1] : 0.0f;

@@ -473,6 +473,19 @@ struct AppendArgs {
 };
 hipError_t launch_append(const AppendArgs &a, int dtype, hipStream_t s);
 
+// The values of slots 0 .. S - 1 of every stream, unrotated (pqkv_dequantize_slots).
+struct SlotsArgs {
+  const uint8_t *blocks;              // streams `stride` bytes apart, or
+  int64_t stride;
+  const uint8_t *const *pages;        // pages
+  int page_shift, max_pages;
+  const float *codebook;
+  void *out;
+  int64_t vectors;                    // S times the streams, below 2^32
+  int S;
+};
+hipError_t launch_slots(const SlotsArgs &a, int d, int bits, int out_dtype, hipStream_t s);
+
 // Eviction: selection, and the move of up to PQKV_MAX_GATHER arrays' rows.
 hipError_t launch_evict_select(const float *weights, int64_t stride, int64_t n_streams, int S, int keep, int sink,
                                int recent, int *kept, hipStream_t s);

@@ -137,6 +137,8 @@ SIGNATURES = {
     "pqkv_rotary_axes": (c_int, [c_void_p, c_int64_p, c_void_p, c_int, c_void_p, c_int64_p, c_void_p, c_int, c_int,
                                  c_void_p, c_int64, c_int64, c_int, ctypes.c_char_p, c_void_p, c_int, c_int, c_int,
                                  c_int, c_int, c_float, c_int, c_void_p]),
+    "pqkv_dequantize_slots": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int,
+                                      c_int64, c_int, c_int, c_void_p]),
     "pqkv_append_rotary": (c_int, [c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int64_p, c_void_p, c_int, c_int,
                                    c_void_p, c_int64, c_int64, c_int, ctypes.c_char_p, c_void_p, c_int, c_int, c_float,
                                    c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,

@@ -205,8 +205,11 @@ def dequantize(cache: PQCache, rotation_matrix: torch.Tensor | None, out_dtype=t
     """Reconstruction r16 c[code] of the first `positions` (default seq_len)
     positions of every (batch, head), rotated back with R (pqkv_dequantize):
     [B, H, positions, d] of out_dtype. rotation_matrix None leaves the
-    rotated-space reconstruction (R = I, exact). A paged cache is gathered
-    into one array first."""
+    rotated-space reconstruction (R = I, exact), out of a cache as it lies
+    (pqkv_dequantize_slots). With a rotation a paged cache is gathered into one
+    array first."""
+    if rotation_matrix is None and _lies_in_rows(cache):
+        return _dequantize_slots(cache, out_dtype, cache.seq_len if positions is None else int(positions))
     if isinstance(cache, PagedPQCache):
         cache = cache.to_contiguous(positions)
     S = cache.seq_len if positions is None else int(positions)
@@ -246,6 +249,33 @@ def dequantize(cache: PQCache, rotation_matrix: torch.Tensor | None, out_dtype=t
         cb = cache.codebooks[h] if cache.codebooks.dim() == 2 else cache.codebooks
         rows(blocks + cache.head_offset(h), cache.blocks.stride(0), cb.data_ptr(), bits, dst + h * S * d * es,
              H * S * d, B)
+    return out
+
+
+def _lies_in_rows(cache) -> bool:
+    if isinstance(cache, PagedPQCache):
+        return not cache.caller_managed
+    return not cache.mixed and cache.blocks.dim() == 4 and cache.blocks.is_contiguous()
+
+
+def _dequantize_slots(cache, out_dtype, S: int) -> torch.Tensor:
+    paged = isinstance(cache, PagedPQCache)
+    where = cache.table if paged else cache.blocks
+    _lib.require_device(where)
+    _lib.require_one_device(where, cache.codebooks)
+    room = cache.capacity if paged else cache.max_seq_len
+    if not 0 <= S <= room:
+        raise ValueError(f"positions {S} exceed the cache capacity {room}")
+    B, H, d = cache.batch, cache.num_heads, cache.head_dim
+    out = torch.empty(B, H, S, d, dtype=out_dtype, device=where.device)
+    if out.numel() == 0:
+        return out
+    row = 0 if paged else cache.max_seq_len * vector_bytes(d, cache.n_bits)
+    with _lib.on_device(out):
+        _lib.check(_lib.lib().pqkv_dequantize_slots(
+            None if paged else cache.blocks.data_ptr(), row, cache.table.data_ptr() if paged else None,
+            cache.page_tokens if paged else 0, cache.max_pages if paged else 0, cache.codebooks.data_ptr(), cache.n_bits,
+            out.data_ptr(), _lib.dtype_code(out_dtype), B * H, S, d, _lib.stream_of(out)))
     return out
 
 

@@ -276,3 +276,36 @@ def test_growing_caches_and_refusals():
     with pytest.raises(RuntimeError, match="before"):
         with torch.cuda.graph(graph):
             append.append_rotary(k, k, keys, values, R, pos, freqs)
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d,bits,page", [(64, 4, 0), (64, 2, 64), (128, 4, 256), (128, 2, 0)])
+def test_slots_read_back(d, bits, page, out):
+    """The values of slots: to the bit what the product with a unit matrix gives."""
+    case = (2, 3, 3, 70, 150, d, d, bits, False, page, torch.float16, False, None, [80, 3], None)
+    q, k, v, keys, values, R, P, positions, freqs, _ = make(case)
+    for c in (keys, values):                        # radii of every kind among random bytes
+        blocks = c.groups[0] if page else c.blocks
+        for t, bits16 in enumerate((0x0000, 0x8000, 0x7C00, 0xFC00, 0x7E01, 0x0001, 0x7BFF, 0xFBFF)):
+            for j in range(d // 32):
+                at = j * window_ref.BLOCK_BYTES[bits]
+                blocks[:, :, t, at], blocks[:, :, t, at + 1] = bits16 & 255, bits16 >> 8
+        S = c.capacity if page else 150
+        got = quantizer.dequantize(c, None, out, S)
+        whole = c.to_contiguous(S) if page else c
+        blocks = whole.blocks.contiguous()
+        for j in range(1, d // 32):                 # (one radius a vector, as encoders write it)
+            at = j * window_ref.BLOCK_BYTES[bits]
+            blocks[..., at:at + 2] = blocks[..., :2]
+        want = quantizer.dequantize(whole, torch.eye(d, device=DEV), out, S)
+        same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+        first = torch.zeros_like(same)
+        first[..., :32] = True                      # the first block's radius is the vector's
+        assert bool((same | ~first).all())
+        if not page:
+            got = quantizer.dequantize(c, None, out, S)
+            assert bool(((got == want) | (torch.isnan(got) & torch.isnan(want))).all())
+            assert torch.equal(torch.signbit(got[~torch.isnan(got)]), torch.signbit(want[~torch.isnan(got)]))
+        assert torch.equal(quantizer.dequantize(c, None, out, 5).nan_to_num(7.0), got[:, :, :5].nan_to_num(7.0))
+        with pytest.raises(ValueError, match="capacity"):
+            quantizer.dequantize(c, None, out, S + 1)
