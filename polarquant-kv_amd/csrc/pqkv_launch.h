@@ -139,7 +139,15 @@ struct PrefillArgs {
   int page_shift, max_pages;
   int16_t heads[kMaxListHeads];
   int64_t k_head_off[kMaxListHeads], v_head_off[kMaxListHeads];
-  Window win;                    // the kernel's WIN mode (S is the cache's capacity, q_start unused)
+  // The kernel's WIN mode (S is the cache's capacity; q_start, q and pq unused):
+  // queries as they are, rotated by the kernel (times q_scale; projections times
+  // p_scale), and with splits = 1 the final outputs.
+  Window win;
+  const void *x;
+  void *out;
+  const float *R, *p_rot;
+  float q_scale, p_scale;
+  int x_f16, out_f16;
 };
 
 // Workspace of one decode call whose plan has `splits` partitions per stream

@@ -43,7 +43,17 @@
 // first, window_tiles), so its work is that of the window. Tiles keep two numbers:
 // `it` counts the row block's (buffers), pos(it) is where one lies. On edge
 // tiles a hidden position's weight is 0 whatever its radius holds. Rows past a
-// sequence's count give zeros.
+// sequence's count give zeros. Behind a window a row block has few tiles, and
+// rotating queries and outputs in launches of their own (fp32, 134 MB each way for
+// 8191 x 32 rows) is a third of a call, so the kernel does both itself, on the matrix
+// cores: R in fp16 parts (22 bits) lies in the tiles' LDS before the first tile and
+// after the last. The rows of R are ordered such that its product with the
+// queries is the score product's operand as it leaves the matrix cores; the outputs
+// pass through LDS once, row by row. 32 + 4 heads, 8191 positions: 617 -> 551 us a call
+// behind 1024 positions, 338 -> 240 behind 64. Without QJL at D = 128 46 registers
+// spill around the two rotations; both row tiles share each operand of R, one operand
+// live at a time, since a row tile at a time held them all (143 spilled, the tile loop's
+// own among them, and 600 us).
 //
 // Precision: every fp32 operand x is split as x_hi = fp16(x),
 // x_lo = fp16(x - x_hi) (fp16 subnormals included, which the f16 MFMA keeps),
@@ -251,6 +261,99 @@ __device__ __forceinline__ void decode_v(const uint8_t *raw, uint8_t *tile, floa
   if (gtid < kPT) rad[kPT + gtid] = half_bits_to_float(*(const uint16_t *)(raw + gtid * VB));
 }
 
+// A D x D matrix (times kRotScale) as 16 x 32 operands in fp16 parts, [o][ks][part]
+// [lane]: tile o's row r = lane % 16, element j of step ks column 32 ks + 8 (lane / 16)
+// + j. OUT = false: row r of tile o is the matrix's row 32 (o / 2) + 8 (r / 4) + 4 (o % 2)
+// + r % 4, so that lane group g's results are the coordinates 32 ks + 8 g .. + 7 that it
+// holds of an operand; OUT: the transposed matrix, and row D / 4 (r / 4) + 4 o + r % 4,
+// so that its results are D / 4 neighbouring coordinates.
+constexpr float kRotScale = 256.0f;
+template <int D, bool OUT>
+__device__ __forceinline__ void rotation_operands(uint8_t *to, const float *R, int tid) {
+  constexpr int KS = D / 32;
+  for (int i = tid; i < D * D / 8; i += kPW * 64) {
+    half8_t hi, lo;
+    int row, k8;   // the operand's row, and its eighth column group
+    float x[8];
+    if constexpr (OUT) {
+      row = i % D;
+      k8 = i / D;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = R[(8 * k8 + j) * D + row];
+    } else {
+      row = i / (D / 8);
+      k8 = i % (D / 8);
+      const float4_dw u = *(const float4_dw *)(R + row * D + 8 * k8), v = *(const float4_dw *)(R + row * D + 8 * k8 + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = u[j];
+        x[4 + j] = v[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      half_t h, l;
+      split2(x[j] * kRotScale, &h, &l);
+      hi[j] = h;
+      lo[j] = l;
+    }
+    int o, r;
+    if constexpr (OUT) {
+      o = (row % (D / 4)) >> 2;
+      r = 4 * (row / (D / 4)) + (row & 3);
+    } else {
+      o = 2 * (row >> 5) + ((row >> 2) & 1);
+      r = 4 * ((row >> 3) & 3) + (row & 3);
+    }
+    uint8_t *p = to + (((o * KS + (k8 >> 2)) * 2) * 64 + 16 * (k8 & 3) + r) * 16;
+    *(half8_t *)p = hi;
+    *(half8_t *)(p + 1024) = lo;
+  }
+}
+// The products of such operands and RT of 16 vectors each in parts; acc[.][o] is tile
+// o's.
+template <int D, int RT>
+__device__ __forceinline__ void rotate_parts(const uint8_t *m, const half8_t (&hi)[RT][D / 32],
+                                             const half8_t (&lo)[RT][D / 32], int lane, float4_t (&acc)[RT][D / 16]) {
+  constexpr int KS = D / 32;
+#pragma unroll
+  for (int o = 0; o < D / 16; ++o) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) acc[rt][o] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint8_t *p = m + (((o * KS + ks) * 2) * 64 + lane) * 16;
+      const half8_t ah = *(const half8_t *)p, al = *(const half8_t *)(p + 1024);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][o] = mfma16(ah, hi[rt][ks], acc[rt][o]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][o] = mfma16(al, hi[rt][ks], acc[rt][o]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][o] = mfma16(ah, lo[rt][ks], acc[rt][o]);
+    }
+  }
+}
+// Parts of a lane's share of a vector (the four lanes col, col + 16, .. hold it),
+// scaled by a power of two that puts its largest coordinate in [2^12, 2^13); what
+// undoes that and kRotScale.
+template <int N>
+__device__ __forceinline__ float scaled_parts(const float (&x)[N], half8_t *hi, half8_t *lo) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+  top = rows_max(top);
+  const int up = min(266 - (int)(__builtin_bit_cast(uint32_t, top) >> 23), 254);
+  const float scale = __builtin_bit_cast(float, (uint32_t)up << 23);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    half_t h, l;
+    split2(x[i] * scale, &h, &l);
+    hi[i >> 3][i & 7] = h;
+    lo[i >> 3][i & 7] = l;
+  }
+  return __builtin_ldexpf(1.0f / kRotScale, 127 - up);
+}
+
 template <int D, int KB, int VBITS, bool QJL, bool WIN = false>
 __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const PrefillArgs a) {
   using PT = PrefillTile<D>;
@@ -344,6 +447,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   half8_t qh[RT][KS], ql[RT][KS];
   half8_t pqh[QJL ? RT : 1][QJL ? KS : 1], pql[QJL ? RT : 1][QJL ? KS : 1];
   int row_pos[RT];
+  float undo_q[WIN ? RT : 1];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = 16 * RT * wave + 16 * rt + col;
@@ -351,6 +455,26 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     const bool row_ok = row < a.qt * G && tok < Sq();
     row_pos[rt] = q_start() + tok;
     const int64_t qrow = ((int64_t)(b * a.Hq + h * G + head) * a.Sq) + (row_ok ? tok : 0);
+    if constexpr (WIN) {
+      // the query's parts as they come; rotated below
+      float x[D / 4];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (a.x_f16) {
+          typedef _Float16 half8_h __attribute__((ext_vector_type(8), aligned(2)));
+          const half8_h v = *(const half8_h *)((const half_t *)a.x + qrow * D + 32 * ks + 8 * grp);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[8 * ks + i] = row_ok ? (float)v[i] : 0.0f;
+        } else {
+          const float *p = (const float *)a.x + qrow * D + 32 * ks + 8 * grp;
+          const float4_dw x0 = *(const float4_dw *)p, x1 = *(const float4_dw *)(p + 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[8 * ks + i] = row_ok ? (i < 4 ? x0[i & 3] : x1[i & 3]) : 0.0f;
+        }
+      }
+      undo_q[rt] = scaled_parts(x, qh[rt], ql[rt]);
+      continue;
+    }
     const float *qr = a.q + qrow * D;
     // (loaded for every row, a valid one for those past the end: with the load
     // behind row_ok each is a branch of its own, 10 us of a 35 us call)
@@ -371,6 +495,51 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) split8(pr + 32 * ks + 8 * grp, pqh[rt][ks], pql[rt][ks]);
     }
+  }
+
+  if constexpr (WIN) {
+    // q' = R q scale, and with signs P_rot q', through the tiles' LDS
+    uint8_t *m = &tiles[0][0];
+    static_assert(D * D * 4 <= 2 * PT::BYTES, "a matrix's parts in the tiles' memory");
+    rotation_operands<D, false>(m, a.R, tid);
+    __syncthreads();
+    float4_t acc[RT][D / 16];
+    rotate_parts<D, RT>(m, qh, ql, lane, acc);
+    // products times f as operands: a lane's results are the coordinates it holds
+    auto operands = [&](int rt, float f, half8_t (&hi)[KS], half8_t (&lo)[KS]) {
+#pragma unroll
+      for (int o = 0; o < D / 16; ++o)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          half_t vh, vl;
+          split2(acc[rt][o][i] * f, &vh, &vl);
+          hi[o >> 1][4 * (o & 1) + i] = vh;
+          lo[o >> 1][4 * (o & 1) + i] = vl;
+        }
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float f = undo_q[rt] * a.q_scale;
+      operands(rt, f, qh[rt], ql[rt]);
+      if constexpr (QJL) {
+        // (as parts of their own: q' may be far from 1)
+        float x[D / 4];
+#pragma unroll
+        for (int o = 0; o < D / 16; ++o)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[8 * (o >> 1) + 4 * (o & 1) + i] = acc[rt][o][i] * f;
+        undo_q[rt] = scaled_parts(x, pqh[rt], pql[rt]);
+      }
+    }
+    if constexpr (QJL) {
+      __syncthreads();
+      rotation_operands<D, false>(m, a.p_rot, tid);
+      __syncthreads();
+      rotate_parts<D, RT>(m, pqh, pql, lane, acc);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) operands(rt, undo_q[rt] * a.p_scale, pqh[rt], pql[rt]);
+    }
+    __syncthreads();   // before the first tile is decoded there
   }
 
   float m_run[RT], l_run[RT];
@@ -672,6 +841,70 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     }
   }
 
+  if constexpr (WIN) {
+    if (splits == 1) {
+      // out = R^T o of each row tile: o to LDS row by row, back as operands
+      uint8_t *m = &tiles[0][0], *rows = m + D * D * 4 + wave * 16 * D * 4;
+      static_assert(D * D * 4 + kPW * 16 * D * 4 <= 2 * PT::BYTES, "both in the tiles' memory");
+      // (a row's 16-byte pieces in an order of its own, so that 16 rows' reads of one
+      // piece fall into different banks)
+      auto at_row = [&](int r, int piece) { return rows + r * D * 4 + 16 * (piece ^ r); };
+      __syncthreads();                                  // every wave is done with the last tile
+      rotation_operands<D, true>(m, a.R, tid);
+      half8_t oh[RT][KS], ol[RT][KS];
+      float undo[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float l = rows_sum(l_run[rt]);
+        float f[4];
+        per_row(l > 0.0f ? 1.0f / (l * kPlaneScale) : 0.0f, grp, f);   // the value planes' 2^6 as well
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            *(float *)(at_row(4 * grp + i, 4 * nb + (col >> 2)) + 4 * (col & 3)) = oacc[rt][nb][i] * f[i];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own rows)
+        float x[D / 4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const float4_t u = *(const float4_t *)at_row(col, 8 * ks + 2 * grp);
+          const float4_t v = *(const float4_t *)at_row(col, 8 * ks + 2 * grp + 1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[8 * ks + i] = u[i];
+            x[8 * ks + 4 + i] = v[i];
+          }
+        }
+        undo[rt] = scaled_parts(x, oh[rt], ol[rt]);
+        asm volatile("" ::: "memory");                  // (read before the next row tile is written there)
+      }
+      __syncthreads();
+      float4_t acc[RT][D / 16];
+      rotate_parts<D, RT>(m, oh, ol, lane, acc);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int row = 16 * RT * wave + 16 * rt + col;
+        const int tok = q0 + row / G, head = row % G;
+        if (row >= a.qt * G || tok >= a.Sq) continue;
+        // (a row past the count: 0 even where a position holds no number)
+        const bool there = tok < wr.count;
+        const int64_t at = (((int64_t)(b * a.Hq + h * G + head) * a.Sq) + tok) * D + (D / 4) * grp;
+#pragma unroll
+        for (int o = 0; o < D / 16; ++o) {
+          float4_t y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = there ? acc[rt][o][i] * undo[rt] : 0.0f;
+          if (a.out_f16) {
+            typedef _Float16 half4_h __attribute__((ext_vector_type(4), aligned(2)));
+            *(half4_h *)((half_t *)a.out + at + 4 * o) = half4_h{(half_t)y[0], (half_t)y[1], (half_t)y[2], (half_t)y[3]};
+          } else {
+            *(float4_dw *)((float *)a.out + at + 4 * o) = y;
+          }
+        }
+      }
+      return;
+    }
+  }
   // ---------------- normalise and write o_rot, or the split's partial ----------------
   const int64_t prow0 = ((int64_t)bh * a.qtiles + qtile) * (16 * RT * kPW);
 #pragma unroll

@@ -155,15 +155,17 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
     return report_hip_error(e, "window merge launch");
   }
   const pqkv::PrefillPlan plan = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl, w, true);
-  const size_t arr = align256((size_t)nvec * d * 4);
   pqkv::PrefillArgs a;
   memset(&a, 0, sizeof(a));
-  float *q32 = (float *)base, *o32 = (float *)(base + arr), *pq32 = (float *)(base + 2 * arr);
-  hipError_t e = rotate("window_rotate", q32, pq32, scale * kLog2e * pqkv::kPrefillPlaneScale,
-                        1.0f / ((float)m * pqkv::kPrefillPlaneScale));
-  if (e != hipSuccess) return report_hip_error(e, "window query rotation");
-  a.q = q32;
-  a.pq = qjl ? pq32 : nullptr;
+  float *o32 = (float *)base;      // rotated outputs, where splits are joined
+  a.x = q;
+  a.x_f16 = q_dtype == PQKV_F16;
+  a.out = out;
+  a.out_f16 = out_dtype == PQKV_F16;
+  a.R = R;
+  a.p_rot = p_rot;
+  a.q_scale = scale * kLog2e * pqkv::kPrefillPlaneScale;
+  a.p_scale = 1.0f / ((float)m * pqkv::kPrefillPlaneScale);
   a.o = o32;
   a.k_cache = k_cache;
   a.v_cache = v_cache;
@@ -185,7 +187,7 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
   a.qtiles = plan.qtiles;
   a.splits = plan.splits;
   a.n_heads = Hkv;
-  a.part_o = (float *)(base + (qjl ? 3 : 2) * arr);
+  a.part_o = (float *)(base + align256((size_t)nvec * d * 4));
   a.part_ml = a.part_o + plan.part_rows * d;
   if (pg) {
     a.k_pages = pg->k_pages;
@@ -196,9 +198,9 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
   }
   a.win = w;
   int t = pqkv::prof_begin("window_attn", st);
-  e = pqkv::launch_prefill_window(a, n_bits, st);
+  hipError_t e = pqkv::launch_prefill_window(a, n_bits, st);
   pqkv::prof_end(t, st);
-  if (e != hipSuccess) return report_hip_error(e, "window launch");
+  if (e != hipSuccess || plan.splits == 1) return report_hip_error(e, "window launch");
   t = pqkv::prof_begin("window_out_rotate", st);
   e = pqkv::launch_rotate(o32, PQKV_F32, R, out, out_dtype, nvec, d, 1, 1.0f, st);
   pqkv::prof_end(t, st);
@@ -213,8 +215,9 @@ size_t pqkv_window_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, i
   if (!window_shape_ok(B, Hq, Hkv, Sq, S, d, qjl != 0) || window < 1 || sinks < 0) return 0;
   const pqkv::Window w = window_of(0, nullptr, nullptr, Sq, window, sinks, S);
   if (Sq == 1) return pqkv::decode_workspace_layout(B, Hq, row_splits(B, Hkv, S, w), d, nullptr, nullptr, nullptr);
-  const size_t arr = align256((size_t)B * Hq * Sq * d * 4);
-  return (qjl ? 3 : 2) * arr + pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl != 0, w, true).part_bytes(d);
+  // (the outputs of one split are final; 256 bytes, so that 0 means a shape that no call takes)
+  const pqkv::PrefillPlan p = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl != 0, w, true);
+  return p.splits == 1 ? 256 : align256((size_t)B * Hq * Sq * d * 4) + p.part_bytes(d);
 }
 
 int pqkv_window_attn(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const uint8_t *v_cache,
