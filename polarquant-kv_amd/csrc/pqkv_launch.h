@@ -317,6 +317,9 @@ inline bool ggml_heads_per_wave(int n_heads) { return n_heads % 4 == 0; }
 // R == nullptr: the normalised rotated output, not rotated back.
 hipError_t launch_decode_merge(const float *part, const float *R, void *out, int out_dtype, int BHq, int splits,
                                int d, hipStream_t s);
+// The merge of one split (n rows of [m, l, o[d]]) on the fp32 matrix cores.
+hipError_t launch_rotate_part_mfma(const float *part, const float *R, void *y, int y_dtype, int64_t n, int d,
+                                   hipStream_t s);
 hipError_t launch_fill_zero(void *p, size_t bytes, hipStream_t s);
 
 // Group (min / scale) format of the reference's CPU quantizer: d <= 256,

@@ -83,6 +83,24 @@ struct StridedSource {
     F32Source<D>{x}.values(w, j8, cb, o);
   }
 };
+// The decode kernels' partials of one split: rows of [m, l, o[D]], the vector o / l
+// (zeros where nothing was summed).
+template <int D>
+struct PartSource {
+  const float *part;
+  typedef float float2_t __attribute__((ext_vector_type(2)));
+  struct Raw { float2_t a[4]; float l; };
+  __device__ __forceinline__ Raw load(int64_t v, int j8) const {
+    const float *row = part + v * (D + 2);
+    const float2_t *p = (const float2_t *)(row + 2 + 8 * j8);   // (rows on 8-byte boundaries)
+    return {{p[0], p[1], p[2], p[3]}, row[1]};
+  }
+  __device__ __forceinline__ void values(const Raw &w, int, const float *, float (&o)[8]) const {
+    const float inv = w.l > 0.0f ? 1.0f / w.l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = w.a[e / 2][e % 2] * inv;
+  }
+};
 // Block-encoded vectors: r16 c[code]. A piece is one dword of qs (4-bit) or
 // half a dword (2-bit) at 2-byte alignment.
 template <int D, int BITS>
@@ -240,6 +258,15 @@ hipError_t launch_rotate_mfma(const void *x, int x_dtype, const float *R, void *
                    : rotate_d<128, false>(x, x_dtype, R, y, y_dtype, n, out_scale, s);
   return inverse ? rotate_d<64, true>(x, x_dtype, R, y, y_dtype, n, out_scale, s)
                  : rotate_d<64, false>(x, x_dtype, R, y, y_dtype, n, out_scale, s);
+}
+
+hipError_t launch_rotate_part_mfma(const float *part, const float *R, void *y, int y_dtype, int64_t n, int d,
+                                   hipStream_t s) {
+  if (d == 128)
+    return y_dtype == 0 ? launch_one<128, true, false>(PartSource<128>{part}, nullptr, R, (float *)y, n, 1.0f, s)
+                        : launch_one<128, true, false>(PartSource<128>{part}, nullptr, R, (half_t *)y, n, 1.0f, s);
+  return y_dtype == 0 ? launch_one<64, true, false>(PartSource<64>{part}, nullptr, R, (float *)y, n, 1.0f, s)
+                      : launch_one<64, true, false>(PartSource<64>{part}, nullptr, R, (half_t *)y, n, 1.0f, s);
 }
 
 hipError_t launch_rotate_rows_mfma(const float *x, int64_t s_q, int64_t s_h, int64_t s_s, int n_q, int Hq, int n_seq,

@@ -33,6 +33,12 @@ pqkv::Window window_of(int64_t start, const int64_t *starts, const int64_t *coun
   return w;
 }
 
+// One split has nothing to join: its rows are normalised and rotated back on the fp32
+// matrix cores. At d = 128 4.3 us for 1024 rows against the merge kernel's 5.3, 4.6
+// against 9.2 for 2048, 4.8 against 16.9 for 4096; 4.9 against 4.0 for 256 (few
+// workgroups there). At d = 64 the two are within 0.1 us up to 1792 rows.
+constexpr int64_t kMergeMfmaRows = 512;
+
 // One row per sequence: the splits of a stream's tiles, as many as the decode
 // kernel takes for as many tokens.
 int row_splits(int B, int Hkv, int S, const pqkv::Window &w) {
@@ -150,7 +156,9 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
       a.q_off += a.g;
     }
     const int t = pqkv::prof_begin("window_merge", st);
-    e = pqkv::launch_decode_merge(a.part, R, out, out_dtype, B * Hq, splits, d, st);
+    e = splits == 1 && nvec >= kMergeMfmaRows
+            ? pqkv::launch_rotate_part_mfma(a.part, R, out, out_dtype, nvec, d, st)
+            : pqkv::launch_decode_merge(a.part, R, out, out_dtype, B * Hq, splits, d, st);
     pqkv::prof_end(t, st);
     return report_hip_error(e, "window merge launch");
   }

@@ -86,6 +86,21 @@ def test_one_row_per_sequence(case, out):
     window_ref.check(got, want, bound)
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("B,Hq,Hkv,d,qjl", [(17, 32, 8, 128, False), (33, 16, 4, 128, True), (40, 14, 2, 64, False)])
+def test_many_sequences_in_one_split(B, Hq, Hkv, d, qjl, out):
+    # (some of them without a row)
+    S, window, sinks = 200, 40, 3
+    q, keys, values, R, jl = make(B, Hq, Hkv, 1, S, d, 4, qjl, 0)
+    at = torch.arange(B, device=DEV) * 11 % S
+    n = (torch.arange(B, device=DEV) % 5 != 3).long()
+    poison(keys, values, at, n, window, sinks)
+    want, bound = window_ref.window_attention(q, keys, values, R, window, sinks, at, n, p_rot=jl)
+    got = attention.window_attention(q, keys, values, R, window, sinks=sinks, starts=at, counts=n, jl_rot=jl,
+                                     out_dtype=out)
+    window_ref.check(got, want, bound)
+
+
 # B, Hq, Hkv, Sq, S, window, sinks, d, bits, qjl, page, starts, counts
 CHUNKS = [
     (1, 1, 1, 2, 2, 1, 0, 64, 4, False, 0, 0, None),
