@@ -49,11 +49,14 @@
 // cores: R in fp16 parts (22 bits) lies in the tiles' LDS before the first tile and
 // after the last. The rows of R are ordered such that its product with the
 // queries is the score product's operand as it leaves the matrix cores; the outputs
-// pass through LDS once, row by row. 32 + 4 heads, 8191 positions: 617 -> 551 us a call
-// behind 1024 positions, 338 -> 240 behind 64. Without QJL at D = 128 46 registers
-// spill around the two rotations; both row tiles share each operand of R, one operand
-// live at a time, since a row tile at a time held them all (143 spilled, the tile loop's
-// own among them, and 600 us).
+// pass through LDS once, row by row. 32 + 8 heads, 8191 positions, box to box within 2 %:
+// 617 -> 518 us a call behind 1024 positions, 338 -> 214 behind 64. Without QJL at D =
+// 128 44 registers spill around the two rotations; both row tiles share each operand
+// of R, one operand live at a time, since a row tile at a time held them all (143
+// spilled, the tile loop's own among them, and 600 us). Of a workgroup's 310 000
+// cycles behind 1024 positions (18 tiles) 242 000 are the tile loop, 7 300 each the
+// products of the two rotations, whose matrix instructions alone take 6 100; R's loads
+// go out with the queries', the first tiles' behind them (6 % of the call).
 //
 // Precision: every fp32 operand x is split as x_hi = fp16(x),
 // x_lo = fp16(x - x_hi) (fp16 subnormals included, which the f16 MFMA keeps),
@@ -269,47 +272,60 @@ __device__ __forceinline__ void decode_v(const uint8_t *raw, uint8_t *tile, floa
 // so that its results are D / 4 neighbouring coordinates.
 constexpr float kRotScale = 256.0f;
 template <int D, bool OUT>
-__device__ __forceinline__ void rotation_operands(uint8_t *to, const float *R, int tid) {
-  constexpr int KS = D / 32;
-  for (int i = tid; i < D * D / 8; i += kPW * 64) {
-    half8_t hi, lo;
-    int row, k8;   // the operand's row, and its eighth column group
-    float x[8];
-    if constexpr (OUT) {
-      row = i % D;
-      k8 = i / D;
+struct RotationOperands {
+  static constexpr int KS = D / 32, N = D * D / 8 / (kPW * 64);
+  float x[N][8];   // eight columns of an operand's row, N times
+
+  __device__ __forceinline__ static void place(int i, int &row, int &k8) {   // the row, and which eight columns
+    row = OUT ? i % D : i / (D / 8);
+    k8 = OUT ? i / D : i % (D / 8);
+  }
+  // (all loads before the first use: waited for one after the other they are the longest
+  // part of a short row block)
+  __device__ __forceinline__ void load(const float *R, int tid) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = R[(8 * k8 + j) * D + row];
-    } else {
-      row = i / (D / 8);
-      k8 = i % (D / 8);
-      const float4_dw u = *(const float4_dw *)(R + row * D + 8 * k8), v = *(const float4_dw *)(R + row * D + 8 * k8 + 4);
+    for (int u = 0; u < N; ++u) {
+      int row, k8;
+      place(tid + kPW * 64 * u, row, k8);
+      if constexpr (OUT) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = u[j];
-        x[4 + j] = v[j];
+        for (int j = 0; j < 8; ++j) x[u][j] = R[(8 * k8 + j) * D + row];
+      } else {
+        const float4_t v = *(const float4_t *)(R + row * D + 8 * k8), w = *(const float4_t *)(R + row * D + 8 * k8 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[u][j] = v[j];
+          x[u][4 + j] = w[j];
+        }
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      half_t h, l;
-      split2(x[j] * kRotScale, &h, &l);
-      hi[j] = h;
-      lo[j] = l;
-    }
-    int o, r;
-    if constexpr (OUT) {
-      o = (row % (D / 4)) >> 2;
-      r = 4 * (row / (D / 4)) + (row & 3);
-    } else {
-      o = 2 * (row >> 5) + ((row >> 2) & 1);
-      r = 4 * ((row >> 3) & 3) + (row & 3);
-    }
-    uint8_t *p = to + (((o * KS + (k8 >> 2)) * 2) * 64 + 16 * (k8 & 3) + r) * 16;
-    *(half8_t *)p = hi;
-    *(half8_t *)(p + 1024) = lo;
   }
-}
+  __device__ __forceinline__ void put(uint8_t *to, int tid) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      int row, k8, o, r;
+      place(tid + kPW * 64 * u, row, k8);
+      half8_t hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        half_t h, l;
+        split2(x[u][j] * kRotScale, &h, &l);
+        hi[j] = h;
+        lo[j] = l;
+      }
+      if constexpr (OUT) {
+        o = (row % (D / 4)) >> 2;
+        r = 4 * (row / (D / 4)) + (row & 3);
+      } else {
+        o = 2 * (row >> 5) + ((row >> 2) & 1);
+        r = 4 * ((row >> 3) & 3) + (row & 3);
+      }
+      uint8_t *p = to + (((o * KS + (k8 >> 2)) * 2) * 64 + 16 * (k8 & 3) + r) * 16;
+      *(half8_t *)p = hi;
+      *(half8_t *)(p + 1024) = lo;
+    }
+  }
+};
 // The products of such operands and RT of 16 vectors each in parts; acc[.][o] is tile
 // o's.
 template <int D, int RT>
@@ -448,6 +464,9 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   half8_t pqh[QJL ? RT : 1][QJL ? KS : 1], pql[QJL ? RT : 1][QJL ? KS : 1];
   int row_pos[RT];
   float undo_q[WIN ? RT : 1];
+  struct None {};
+  std::conditional_t<WIN, RotationOperands<D, false>, None> rot;
+  if constexpr (WIN) rot.load(a.R, tid);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = 16 * RT * wave + 16 * rt + col;
@@ -495,51 +514,6 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) split8(pr + 32 * ks + 8 * grp, pqh[rt][ks], pql[rt][ks]);
     }
-  }
-
-  if constexpr (WIN) {
-    // q' = R q scale, and with signs P_rot q', through the tiles' LDS
-    uint8_t *m = &tiles[0][0];
-    static_assert(D * D * 4 <= 2 * PT::BYTES, "a matrix's parts in the tiles' memory");
-    rotation_operands<D, false>(m, a.R, tid);
-    __syncthreads();
-    float4_t acc[RT][D / 16];
-    rotate_parts<D, RT>(m, qh, ql, lane, acc);
-    // products times f as operands: a lane's results are the coordinates it holds
-    auto operands = [&](int rt, float f, half8_t (&hi)[KS], half8_t (&lo)[KS]) {
-#pragma unroll
-      for (int o = 0; o < D / 16; ++o)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          half_t vh, vl;
-          split2(acc[rt][o][i] * f, &vh, &vl);
-          hi[o >> 1][4 * (o & 1) + i] = vh;
-          lo[o >> 1][4 * (o & 1) + i] = vl;
-        }
-    };
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float f = undo_q[rt] * a.q_scale;
-      operands(rt, f, qh[rt], ql[rt]);
-      if constexpr (QJL) {
-        // (as parts of their own: q' may be far from 1)
-        float x[D / 4];
-#pragma unroll
-        for (int o = 0; o < D / 16; ++o)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[8 * (o >> 1) + 4 * (o & 1) + i] = acc[rt][o][i] * f;
-        undo_q[rt] = scaled_parts(x, pqh[rt], pql[rt]);
-      }
-    }
-    if constexpr (QJL) {
-      __syncthreads();
-      rotation_operands<D, false>(m, a.p_rot, tid);
-      __syncthreads();
-      rotate_parts<D, RT>(m, pqh, pql, lane, acc);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) operands(rt, undo_q[rt] * a.p_scale, pqh[rt], pql[rt]);
-    }
-    __syncthreads();   // before the first tile is decoded there
   }
 
   float m_run[RT], l_run[RT];
@@ -795,6 +769,51 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   if (it0 < it1) dma(it0);
   if (it0 + 1 < it1) dma(it0 + 1);
+  if constexpr (WIN) {
+    // q' = R q scale, and with signs P_rot q', through the tiles' LDS
+    uint8_t *m = &tiles[0][0];
+    static_assert(D * D * 4 <= 2 * PT::BYTES, "a matrix's parts in the tiles' memory");
+    rot.put(m, tid);
+    __syncthreads();
+    if constexpr (QJL) rot.load(a.p_rot, tid);
+    float4_t acc[RT][D / 16];
+    rotate_parts<D, RT>(m, qh, ql, lane, acc);
+    // products times f as operands: a lane's results are the coordinates it holds
+    auto operands = [&](int rt, float f, half8_t (&hi)[KS], half8_t (&lo)[KS]) {
+#pragma unroll
+      for (int o = 0; o < D / 16; ++o)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          half_t vh, vl;
+          split2(acc[rt][o][i] * f, &vh, &vl);
+          hi[o >> 1][4 * (o & 1) + i] = vh;
+          lo[o >> 1][4 * (o & 1) + i] = vl;
+        }
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float f = undo_q[rt] * a.q_scale;
+      operands(rt, f, qh[rt], ql[rt]);
+      if constexpr (QJL) {
+        // (as parts of their own: q' may be far from 1)
+        float x[D / 4];
+#pragma unroll
+        for (int o = 0; o < D / 16; ++o)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[8 * (o >> 1) + 4 * (o & 1) + i] = acc[rt][o][i] * f;
+        undo_q[rt] = scaled_parts(x, pqh[rt], pql[rt]);
+      }
+    }
+    if constexpr (QJL) {
+      __syncthreads();
+      rot.put(m, tid);
+      __syncthreads();
+      rotate_parts<D, RT>(m, pqh, pql, lane, acc);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) operands(rt, undo_q[rt] * a.p_scale, pqh[rt], pql[rt]);
+    }
+    __syncthreads();   // before the first tile is decoded there
+  }
   wait_dma();
   __syncthreads();  // tables and the first two raw tiles ready
   if (it0 < it1) decode(it0);
@@ -849,8 +868,10 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       // (a row's 16-byte pieces in an order of its own, so that 16 rows' reads of one
       // piece fall into different banks)
       auto at_row = [&](int r, int piece) { return rows + r * D * 4 + 16 * (piece ^ r); };
+      RotationOperands<D, true> back;
+      back.load(a.R, tid);
       __syncthreads();                                  // every wave is done with the last tile
-      rotation_operands<D, true>(m, a.R, tid);
+      back.put(m, tid);
       half8_t oh[RT][KS], ol[RT][KS];
       float undo[RT];
 #pragma unroll
@@ -890,15 +911,19 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
         const bool there = tok < wr.count;
         const int64_t at = (((int64_t)(b * a.Hq + h * G + head) * a.Sq) + tok) * D + (D / 4) * grp;
 #pragma unroll
-        for (int o = 0; o < D / 16; ++o) {
-          float4_t y;
+        for (int o = 0; o < D / 16; o += 2) {
+          float y[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = there ? acc[rt][o][i] * undo[rt] : 0.0f;
+          for (int i = 0; i < 8; ++i) y[i] = there ? acc[rt][o + (i >> 2)][i & 3] * undo[rt] : 0.0f;
           if (a.out_f16) {
-            typedef _Float16 half4_h __attribute__((ext_vector_type(4), aligned(2)));
-            *(half4_h *)((half_t *)a.out + at + 4 * o) = half4_h{(half_t)y[0], (half_t)y[1], (half_t)y[2], (half_t)y[3]};
+            typedef _Float16 half8_h __attribute__((ext_vector_type(8), aligned(2)));
+            half8_h v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (half_t)y[i];
+            *(half8_h *)((half_t *)a.out + at + 4 * o) = v;
           } else {
-            *(float4_dw *)((float *)a.out + at + 4 * o) = y;
+            *(float4_dw *)((float *)a.out + at + 4 * o) = float4_dw{y[0], y[1], y[2], y[3]};
+            *(float4_dw *)((float *)a.out + at + 4 * o + 4) = float4_dw{y[4], y[5], y[6], y[7]};
           }
         }
       }
