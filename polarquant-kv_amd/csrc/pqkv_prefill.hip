@@ -1139,7 +1139,10 @@ PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl,
   const int64_t seen = (int64_t)w.size + p.qt + 126, all = ((int64_t)S + kPT - 1) / kPT;
   const int64_t tiles = std::min(seen / kPT + (w.sinks + kPT - 1) / kPT, all);
   const int64_t blocks = (int64_t)p.qtiles * p.streams;
-  const int64_t splits = std::min<int64_t>(kTargetBlocks / blocks, tiles / 4);
+  // few row blocks: down to a tile per split. 257 rows of 14 + 2 heads, d = 64, behind 512
+  // positions 46.9 us with four tiles or more, 38.4 with two, 35.8 with one; 64 rows of
+  // 32 + 8, d = 128, behind 2048 61.6, 52.8, 52.0, behind 128 53.8, 42.8, 37.1
+  const int64_t splits = std::min<int64_t>(kTargetBlocks / blocks, tiles);
   if (splits > 1) {
     p.splits = (int)splits;
     p.part_rows = blocks * p.rows * splits;
