@@ -741,7 +741,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     }
     const int pg = t0 >> a.page_shift, p0 = pg << a.page_shift;
     rel = t0 - p0;
-    return stream_rsrc(pages[prow + pg], (uint32_t)min(S() - p0, 1 << a.page_shift) * (uint32_t)vb);
+    // (a page's address through the scalar cache: a vector load's wait is also one for the
+    // raw-tile copies before it; 4 x 512 rows with signs behind 4096 positions 565 -> 558
+    // us, d = 64 424 -> 394)
+    const uint8_t *page = *(const uint8_t *const __attribute__((address_space(4))) *)(uintptr_t)(pages + prow + pg);
+    return stream_rsrc(page, (uint32_t)min(S() - p0, 1 << a.page_shift) * (uint32_t)vb);
   };
   auto decode = [&](int it) {  // this group's half of tile it, from graw[it & 1]
     if (group == 0) decode_k<D, KB>(graw[it & 1], tiles[it & 1], rads[it & 1], lut_k, gtid);
@@ -832,12 +836,18 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     __builtin_amdgcn_s_setprio(0);
     wait_dma();
   };
+  // Behind a window: the next tile's decode before this one's softmax, so that the copy
+  // after it is on its way a softmax longer (d = 128: 512 rows of 4 x 32 + 8 heads
+  // behind 4096 positions 416 -> 380 us; with signs, whose wave has half the rows,
+  // 559 -> 588, and d = 64 341 -> 346: softmax first).
+  constexpr bool kEarly = WIN && RT == 2 && D == 128;
   auto y_stage = [&](int it) {
-    softmax(it);
+    if (!kEarly) softmax(it);
     if (it + 1 < it1) {
       decode(it + 1);
       if (it + 2 < it1) dma(it + 2);
     }
+    if (kEarly) softmax(it);
   };
   if (it0 < it1) {
     if (group == 0) {
