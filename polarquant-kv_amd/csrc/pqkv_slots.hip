@@ -5,8 +5,8 @@
 // thread takes eight coordinates (the codes that one 16-byte store of fp16 needs),
 // neighbouring threads neighbouring ones, so that stores and the reads of a vector's
 // bytes are dense; the codebook is in LDS, one bank an entry. 8 streams of 32768
-// vectors of 128 to fp16: 30 us where the product with a unit matrix took 82 behind
-// a copy out of the pages of 29.
+// vectors of 128 to fp16: 34 us (86 MB, 2.5 TB/s) where the product with a unit matrix
+// took 82 behind a copy out of the pages of 29.
 #include "pqkv_device.h"
 #include "pqkv_launch.h"
 
