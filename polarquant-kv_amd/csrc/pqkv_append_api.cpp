@@ -58,10 +58,11 @@ int append_run(const char *what, const void *k, const int64_t k_strides[3], cons
       (Hkv && ((uintptr_t)k | (uintptr_t)v) % size) || (Hq && ((uintptr_t)q | (uintptr_t)q_out) % size))
     return fail_status(PQKV_ERR_INVALID, "%s: unaligned pointer", what);
   hipStream_t st = (hipStream_t)stream;
-  if (Hkv) {
+  // (a cache without a slot: there is nothing to write, and no page to find)
+  if (Hkv && S > 0) {
     if (!k || !v || !k_strides || !v_strides || !R || !k_cb || !v_cb)
       return fail_status(PQKV_ERR_INVALID, "%s: null pointer", what);
-    if (S > 0 && (pg ? (!pg->k || !pg->v) : (!k_blocks || !v_blocks)))
+    if (pg ? (!pg->k || !pg->v) : (!k_blocks || !v_blocks))
       return fail_status(PQKV_ERR_INVALID, "%s: null cache", what);
     if (((uintptr_t)k_blocks | (uintptr_t)v_blocks) % 2 || (uintptr_t)signs % 4 || (uintptr_t)R % 4 ||
         (uintptr_t)p_rot % 4)

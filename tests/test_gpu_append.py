@@ -222,6 +222,19 @@ def test_slots_that_there_is_no_room_for(page):
     assert torch.equal(window_ref.rows_of(keys)[0], before[0][0])
 
 
+@pytest.mark.parametrize("T", [1, 40])
+def test_a_cache_without_a_page(T):
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v = (torch.randn(2, h, T, 128, generator=g, device=DEV).half() for h in (4, 2, 2))
+    R = rotation.generate_rotation_matrix(128, seed=42, device=DEV)
+    keys, values = (quantizer.allocate_paged_cache(2, 2, 128, 4, DEV, page_tokens=64) for _ in range(2))
+    freqs, _ = rotary.rotary_frequencies(128)
+    freqs, positions = freqs.to(DEV), torch.arange(T, device=DEV)
+    out = append.append_rotary(k, v, keys, values, R, positions, freqs, query=q, starts=expand([0, 3], 2))
+    assert torch.equal(out, rotary.apply_rotary(q, None, positions, freqs)[0])
+    assert keys.capacity == values.capacity == keys.seq_len == 0
+
+
 def test_captured_appends_follow_their_starts():
     case = (3, 4, 2, 1, 200, 128, 128, 4, False, 64, torch.float16, False, None, [10, 63, 150], None)
     q, k, v, keys, values, R, P, positions, freqs, _ = make(case)
