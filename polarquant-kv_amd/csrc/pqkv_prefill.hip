@@ -51,7 +51,7 @@
 // queries is the score product's operand as it leaves the matrix cores; the outputs
 // pass through LDS once, row by row. 32 + 8 heads, 8191 positions, box to box within 2 %:
 // 617 -> 518 us a call behind 1024 positions, 338 -> 214 behind 64. Without QJL at D =
-// 128 44 registers spill around the two rotations; both row tiles share each operand
+// 128 29 registers spill around the two rotations; both row tiles share each operand
 // of R, one operand live at a time, since a row tile at a time held them all (143
 // spilled, the tile loop's own among them, and 600 us). Of a workgroup's 310 000
 // cycles behind 1024 positions (18 tiles) 242 000 are the tile loop, 7 300 each the
@@ -940,7 +940,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       return;
     }
   }
-  // ---------------- normalise and write o_rot, or the split's partial ----------------
+  // ---------------- normalise and write o_rot, or the split's partial (WIN: that) ----------------
   const int64_t prow0 = ((int64_t)bh * a.qtiles + qtile) * (16 * RT * kPW);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -948,17 +948,17 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     if constexpr (WIN) {
       if (q0 + (16 * RT * wave + 16 * rt + col) / G >= wr.count) l = 0.0f;
     }
-    if (splits > 1 && grp == 0)
+    if ((WIN || splits > 1) && grp == 0)
       ((float2 *)a.part_ml)[(prow0 + 16 * RT * wave + 16 * rt + col) * splits + sp] = make_float2(m_run[rt], l);
     float f[4];
-    per_row(splits > 1 ? 1.0f : l > 0.0f ? 1.0f / (l * kPlaneScale) : 0.0f, grp, f);   // the value planes' 2^6 as well
+    per_row(WIN || splits > 1 ? 1.0f : l > 0.0f ? 1.0f / (l * kPlaneScale) : 0.0f, grp, f);   // the value planes' 2^6 as well
     // output rows 4 grp + i of this row tile
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * RT * wave + 16 * rt + 4 * grp + i;
       const int tok = q0 + row / G, head = row % G;
       float *dst;
-      if (splits > 1) dst = a.part_o + ((prow0 + row) * splits + sp) * D;
+      if (WIN || splits > 1) dst = a.part_o + ((prow0 + row) * splits + sp) * D;
       else if (row < a.qt * G && tok < a.Sq) dst = a.o + (((int64_t)(b * a.Hq + h * G + head) * a.Sq) + tok) * D;
       else continue;
 #pragma unroll
