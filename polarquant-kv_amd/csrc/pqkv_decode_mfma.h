@@ -398,7 +398,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
     const WindowRows wr = window_rows(a.win, b, 1, a.S);
     row = __builtin_amdgcn_readfirstlane(wr.start);
     wt = window_tiles(a.win, row, row);
-    if (wr.count > 0) {
+    // (known to be wave-uniform, or a page's loads become loops over lanes)
+    if (__builtin_amdgcn_readfirstlane(wr.count) > 0) {
       tile0 = (int)((int64_t)wt.tiles * split / a.splits);
       tile1 = (int)((int64_t)wt.tiles * (split + 1) / a.splits);
     }
