@@ -348,7 +348,7 @@ struct DecodeSmem {
 // window_tiles), so a launch's work does not grow with the cache. Edge tiles
 // hide positions: their logits are -inf and their radii 0 (a hidden value that is
 // not a number would give 0 * NaN). Positions past the row read zeros. 64 sequences
-// behind 4096 positions (32 + 8 heads, d = 128, 4 bits): 70-73 us, 303 MB at 4.2 TB/s;
+// behind 4096 positions (32 + 8 heads, d = 128, 4 bits): 66-73 us, 303 MB at 4.2 to 4.6 TB/s;
 // the kernel without it takes as long on a cache of as many.
 // FREE: the steady-state iteration has no scheduling fences between its
 // table reads, softmax weights and products (the mixed-width pair kernel and
