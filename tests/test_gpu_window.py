@@ -242,3 +242,22 @@ def test_strided_queries_and_rotations():
     assert not wide.is_contiguous()
     assert torch.equal(attention.window_attention(wide, keys, values, R.t().contiguous().t(), 30, sinks=1), want)
     assert attention.window_attention(q[:, :, :0], keys, values, R, 30).shape == (2, 8, 0, 64)
+
+
+@pytest.mark.parametrize("S", [60, 300], ids=["one_split", "splits"])
+@pytest.mark.parametrize("d,bits,qjl", [(128, 4, False), (64, 2, False), (128, 4, True)])
+def test_queries_of_any_size(S, d, bits, qjl):
+    # rows of very different sizes side by side in a matrix operand
+    q, keys, values, R, jl = make(2, 8, 2, 24, S, d, bits, qjl, 0, dtype=torch.float32)
+    sizes = torch.tensor([0.0, 1e-30, 2.0 ** -6, 1.0, 8.0, 20.0], device=DEV)
+    q = q * sizes[torch.arange(24, device=DEV) % 6][:, None]
+    at, n = per_sequence([S - 24, 5], 2), per_sequence(24, 2)
+    want, bound = window_ref.window_attention(q, keys, values, R, 33, 2, at, n, p_rot=jl)
+    window_ref.check(attention.window_attention(q, keys, values, R, 33, sinks=2, starts=at, jl_rot=jl), want, bound)
+    q[0, 3, 7] = float("inf")
+    q[1, 5, 20, 3] = float("nan")
+    got = attention.window_attention(q, keys, values, R, 33, sinks=2, starts=at, jl_rot=jl)
+    hit = torch.zeros(2, 8, 24, dtype=torch.bool, device=DEV)
+    hit[0, 3, 7] = hit[1, 5, 20] = True
+    assert torch.isnan(got[hit]).all()
+    window_ref.check(got[~hit], want[~hit], bound[~hit])
