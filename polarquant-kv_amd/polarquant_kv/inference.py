@@ -221,7 +221,8 @@ class KVCacheManager:
         with _lib.lasting():                   # (pages that this adds are written in any mode)
             self._keys.ensure(self._seq_len + T)
             self._values.ensure(self._seq_len + T)
-        out = append.append_rotary(key, value, self._keys, self._values, self.R, rotary.positions_by_axis(positions),
+        out = append.append_rotary(key, value, self._keys, self._values, self.R,
+                                   rotary.positions_by_axis(positions, key.shape[0]),
                                    rotary.frequencies_on(key.device), query=query, starts=self._seq_len,
                                    interleaved=rotary.interleaved, amplitude=rotary.amplitude, axes=rotary.axes,
                                    jl_rot=self.jl_rot)

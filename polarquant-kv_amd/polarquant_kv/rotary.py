@@ -279,8 +279,8 @@ class RotaryEmbedding:
     the whole head) of head_dim coordinates, base, scaling and pairing as
     rotary_frequencies and apply_rotary take them. sections: how many pairs each
     of several axes of positions has, spread as axis_of_pairs takes it; positions
-    have an axis in front then, or none where all axes are alike (text). The
-    first call on a device
+    have an axis in front then, or none where all axes are alike (text;
+    positions_by_axis). The first call on a device
     copies the frequencies to it, which a graph capture does not allow: such a
     call is refused there."""
 
@@ -310,16 +310,34 @@ class RotaryEmbedding:
                 freqs = self._on[device] = self.frequencies.to(device)
         return freqs
 
-    def positions_by_axis(self, positions: torch.Tensor) -> torch.Tensor:
-        """Positions [T] with the axis in front that several axes take: of text,
-        whose axes are alike."""
-        if self.axes is None or positions.dim() != 1:
+    def positions_by_axis(self, positions: torch.Tensor, batch: int | None = None) -> torch.Tensor:
+        """Positions of `batch` sequences with the axis in front that several axes
+        take: those of text, whose axes are alike, are [T] or a row per sequence
+        [batch, T]. [n_axes, T] has its axes already, the same for all sequences;
+        where batch is n_axes too, it could be either and is refused (with the
+        axes in front it is [n_axes, batch, T]). Any other number of rows is
+        refused. Without batch only [T] is expanded."""
+        if self.axes is None:
             return positions
-        return positions.expand(self.n_axes, -1)
+        if positions.dim() == 1:
+            return positions.expand(self.n_axes, -1)
+        if batch is None:
+            return positions
+        rows = positions.shape[0]
+        if positions.dim() == 2 and rows == batch:
+            if rows == self.n_axes > 1:
+                raise ValueError(f"positions {tuple(positions.shape)} could be of {batch} sequences or on {rows} axes: "
+                                 f"give [{rows}, {batch}, T]")
+            return positions.expand(self.n_axes, -1, -1)
+        if rows != self.n_axes:
+            raise ValueError(f"positions must be [T], [{batch}, T], [{self.n_axes}, T] or [{self.n_axes}, {batch}, T], "
+                             f"got {tuple(positions.shape)}")
+        return positions
 
     def __call__(self, query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor):
-        return apply_rotary(query, key, self.positions_by_axis(positions), self.frequencies_on(query.device),
-                            interleaved=self.interleaved, amplitude=self.amplitude, axes=self.axes)
+        return apply_rotary(query, key, self.positions_by_axis(positions, query.shape[0]),
+                            self.frequencies_on(query.device), interleaved=self.interleaved, amplitude=self.amplitude,
+                            axes=self.axes)
 
 
 __all__ = ["rotary_frequencies", "axis_of_pairs", "apply_rotary", "RotaryEmbedding"]
