@@ -46,18 +46,18 @@ __global__ void __launch_bounds__(256) slots_kernel(const SlotsArgs a, const Fas
       const uint32_t s = by_s.div((uint32_t)v), t = (uint32_t)v - s * by_s.d;
       if (a.pages) p[u] = a.pages[(int64_t)s * a.max_pages + (t >> a.page_shift)] + (t & ((1u << a.page_shift) - 1)) * VB;
       else p[u] = a.blocks + (int64_t)s * a.stride + (int64_t)t * VB;
-      p[u] += (g / 4) * block_bytes(BITS);
     }
     uint32_t w[U];
     uint16_t h[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      h[u] = *(const uint16_t *)p[u];
+      h[u] = *(const uint16_t *)p[u];            // (the vector's radius is its first block's)
+      const uint8_t *codes = p[u] + (g / 4) * block_bytes(BITS) + 2;
       if constexpr (BITS == 4) {
-        const uint16_t *q = (const uint16_t *)(p[u] + 2) + 2 * (g % 4);
+        const uint16_t *q = (const uint16_t *)codes + 2 * (g % 4);
         w[u] = q[0] | (uint32_t)q[1] << 16;
       } else {
-        w[u] = ((const uint16_t *)(p[u] + 2))[g % 4];
+        w[u] = ((const uint16_t *)codes)[g % 4];
       }
     }
 #pragma unroll

@@ -253,9 +253,11 @@ def dequantize(cache: PQCache, rotation_matrix: torch.Tensor | None, out_dtype=t
 
 
 def _lies_in_rows(cache) -> bool:
+    """Whether pqkv_dequantize_slots takes the cache as it lies."""
     if isinstance(cache, PagedPQCache):
         return not cache.caller_managed
-    return not cache.mixed and cache.blocks.dim() == 4 and cache.blocks.is_contiguous()
+    return not cache.mixed and cache.blocks.dim() == 4 and cache.blocks.is_contiguous() and \
+        cache.blocks.data_ptr() % 2 == 0
 
 
 def _dequantize_slots(cache, out_dtype, S: int) -> torch.Tensor:
