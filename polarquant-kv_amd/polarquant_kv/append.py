@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .attention import _codebook_tables, check_paged, check_shapes, check_signs, page_tables, row_counts, row_starts
-from .rotary import _code, _strides, check_axes, position_strides
+from .rotary import _code, _has_tangent, _strides, apply_rotary, check_axes, position_strides
 from .types import PagedPQCache
 
 
@@ -25,8 +25,9 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, keys, values, rotation
     """key and value [B, Hkv, T, d] into the caches `keys` and `values` (both
     PQCache, or both PagedPQCache; one width), the keys turned by positions *
     frequencies on the way; query [B, Hq, T, d] is turned too and returned
-    (contiguous, in its type), else None. fp16, bf16 or fp32, one for all; any
-    strides. positions, frequencies, interleaved, amplitude and axes as
+    (contiguous, in its type), else None; gradients and forward-mode tangents flow
+    through it as through rotary.apply_rotary (not through what is cached). fp16, bf16
+    or fp32, one for all; any strides. positions, frequencies, interleaved, amplitude and axes as
     rotary.apply_rotary takes them. jl_rot = P R^T adds the keys' QJL signs.
 
     starts: the slot of each sequence's first token: a number for all, by default
@@ -52,6 +53,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, keys, values, rotation
         raise ValueError(f"{2 * frequencies.numel()} turned coordinates of a head of {d}")
     if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
         raise ValueError(f"positions must be integers, got {positions.dtype}")
+    given_axes = axes
     if axes is not None:
         axes = check_axes(axes, positions, frequencies.numel(), B, T)
     elif tuple(positions.shape) not in ((T,), (B, T)):
@@ -81,6 +83,11 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, keys, values, rotation
             keys.ensure(start + T)
             values.ensure(start + T)
             check_paged(B, Hkv, d, keys, values)        # (one width of tables again)
+    turned = None
+    if query is not None and ((torch.is_grad_enabled() and query.requires_grad) or _has_tangent(query)):
+        turned, _ = apply_rotary(query, None, positions, frequencies, interleaved=interleaved, amplitude=amplitude,
+                                 axes=given_axes)
+        query = None
     k, v, q = (x if x is None or x.stride(-1) == 1 or x.numel() == 0 else x.contiguous() for x in (key, value, query))
     positions = positions.to(torch.int64)
     if axes is None or positions.stride(-1) != 1:
@@ -109,7 +116,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, keys, values, rotation
     if starts is None:
         for c in (keys, values):
             c.seq_len = max(c.seq_len, start + T)
-    return out
+    return out if turned is None else turned
 
 
 __all__ = ["append_rotary"]
