@@ -380,6 +380,8 @@ class CompressedMultiHeadAttention(torch.nn.Module):
         attend to everything cached (causally unless causal=False). positions
         of the tokens, as the rotary embedding takes them: by default the ones
         after those cached."""
+        if self.window is not None and cache_manager is not None and cache_manager.track_weights:
+            raise ValueError("the weights of a window are not tracked")      # (before anything is appended)
         B, T, _ = x.shape
         q = self.q_proj(x).reshape(B, T, self.num_heads, self.head_dim).transpose(1, 2).half()
         k = self.k_proj(x).reshape(B, T, self.num_kv_heads, self.head_dim).transpose(1, 2).half()
