@@ -296,6 +296,8 @@ class KVCacheManager:
         weights are added to those of the cached positions. window: each query
         looks at so many positions up to its own and at the first `sinks`
         (attention.window_attention; causal, without track_weights)."""
+        if window is None and sinks:
+            raise ValueError(f"sinks={sinks} go with a window")
         if window is not None and (not causal or self.track_weights):
             raise ValueError("a window is causal, and its weights are not tracked")
         if self._seq_len == 0:
@@ -355,6 +357,8 @@ class CompressedMultiHeadAttention(torch.nn.Module):
     def __init__(self, config: PolarQuantConfig, embed_dim: int, num_heads: int, num_kv_heads: int | None = None,
                  causal: bool = True, rotary=None, window: int | None = None, sinks: int = 0):
         super().__init__()
+        if window is None and sinks:
+            raise ValueError(f"sinks={sinks} go with a window")
         if window is not None and (window < 1 or sinks < 0 or not causal):
             raise ValueError(f"window={window} (at least 1) and sinks={sinks} (at least 0) are for causal layers")
         self.window = window
@@ -380,6 +384,8 @@ class CompressedMultiHeadAttention(torch.nn.Module):
         attend to everything cached (causally unless causal=False). positions
         of the tokens, as the rotary embedding takes them: by default the ones
         after those cached."""
+        if positions is not None and self.rotary is None:
+            raise ValueError("positions are for layers with a rotary embedding")
         if self.window is not None and cache_manager is not None and cache_manager.track_weights:
             raise ValueError("the weights of a window are not tracked")      # (before anything is appended)
         B, T, _ = x.shape

@@ -15,3 +15,17 @@ def test_a_window_over_tracked_weights_leaves_the_cache_as_it_was():
         with pytest.raises(ValueError, match="not tracked"):
             layer(torch.zeros(1, 3, 64), m)
         assert m.seq_len == m.next_position == 0 and m._key_cache is None
+
+
+def test_sinks_go_with_a_window():
+    with pytest.raises(ValueError, match="sinks=2 go with a window"):
+        CompressedMultiHeadAttention(PolarQuantConfig(), 64, 2, sinks=2)
+    m = KVCacheManager(PolarQuantConfig(enable_compression=False), 20, 1, 1, 32, "cpu")
+    with pytest.raises(ValueError, match="sinks=2 go with a window"):
+        m.attend(torch.zeros(1, 1, 1, 32), sinks=2)
+
+
+def test_positions_without_an_embedding():
+    layer = CompressedMultiHeadAttention(PolarQuantConfig(enable_compression=False), 64, 2, 1)
+    with pytest.raises(ValueError, match="rotary embedding"):
+        layer(torch.zeros(1, 3, 64), positions=torch.arange(3))
