@@ -296,10 +296,9 @@ class KVCacheManager:
         weights are added to those of the cached positions. window: each query
         looks at so many positions up to its own and at the first `sinks`
         (attention.window_attention; causal, without track_weights)."""
-        if window is None and sinks:
-            raise ValueError(f"sinks={sinks} go with a window")
-        if window is not None and (not causal or self.track_weights):
-            raise ValueError("a window is causal, and its weights are not tracked")
+        _check_window(window, sinks, causal)
+        if window is not None and self.track_weights:
+            raise ValueError("the weights of a window are not tracked")
         if self._seq_len == 0:
             return torch.zeros_like(query, dtype=torch.float16)
         if not self.config.enable_compression:
@@ -337,6 +336,13 @@ class KVCacheManager:
                                                   causal=causal, q_start=start)
 
 
+def _check_window(window, sinks, causal) -> None:
+    if window is None and sinks:
+        raise ValueError(f"sinks={sinks} go with a window")
+    if window is not None and (window != int(window) or window < 1 or sinks != int(sinks) or sinks < 0 or not causal):
+        raise ValueError(f"window={window} (at least 1) and sinks={sinks} (at least 0) are for causal attention")
+
+
 def _hidden(pos, qpos, window, sinks):
     """[rows, positions]: what a row does not see, of a causal or (window) a
     windowed attention."""
@@ -357,10 +363,7 @@ class CompressedMultiHeadAttention(torch.nn.Module):
     def __init__(self, config: PolarQuantConfig, embed_dim: int, num_heads: int, num_kv_heads: int | None = None,
                  causal: bool = True, rotary=None, window: int | None = None, sinks: int = 0):
         super().__init__()
-        if window is None and sinks:
-            raise ValueError(f"sinks={sinks} go with a window")
-        if window is not None and (window < 1 or sinks < 0 or not causal):
-            raise ValueError(f"window={window} (at least 1) and sinks={sinks} (at least 0) are for causal layers")
+        _check_window(window, sinks, causal)
         self.window = window
         self.sinks = sinks
         self.config = config

@@ -29,3 +29,13 @@ def test_positions_without_an_embedding():
     layer = CompressedMultiHeadAttention(PolarQuantConfig(enable_compression=False), 64, 2, 1)
     with pytest.raises(ValueError, match="rotary embedding"):
         layer(torch.zeros(1, 3, 64), positions=torch.arange(3))
+
+
+@pytest.mark.parametrize("cached", [0, 3])
+@pytest.mark.parametrize("kw", [dict(window=0), dict(window=-3), dict(window=2.5), dict(window=3, sinks=-1),
+                                dict(window=3, sinks=0.5)])
+def test_windows_of_an_uncompressed_cache(kw, cached):
+    m = KVCacheManager(PolarQuantConfig(enable_compression=False), 20, 1, 1, 32, "cpu")
+    m.append(torch.zeros(1, 1, cached, 32), torch.zeros(1, 1, cached, 32))
+    with pytest.raises(ValueError, match="window="):
+        m.attend(torch.zeros(1, 1, 1, 32), **kw)
