@@ -40,8 +40,7 @@ int append_run(const char *what, const void *k, const int64_t k_strides[3], cons
   if (qjl != (p_rot != nullptr)) return fail_status(PQKV_ERR_INVALID, "%s: qjl and p_rot go together", what);
   if (qjl && m != d) return fail_status(PQKV_ERR_UNSUPPORTED, "%s: QJL needs m == d", what);
   if (!starts && (start < 0 || start > S || T > S - start))
-    return fail_status(PQKV_ERR_INVALID, "%s: slots %lld..%lld of %d", what, (long long)start,
-                       (long long)start + T - 1, S);
+    return fail_status(PQKV_ERR_INVALID, "%s: %d slots from %lld on, of %d", what, T, (long long)start, S);
   pqkv::RotaryAxes ax;
   const uint8_t one[pqkv::kMaxRotaryPairs] = {};
   const int c = pqkv::rotary_axes(what, axes ? axes : one, axes ? n_axes : 1, rot_dim, axes ? axis_stride : 0, &ax);

@@ -77,9 +77,9 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
   if (qjl != (p_rot != nullptr)) return fail_status(PQKV_ERR_INVALID, "%s: qjl and p_rot go together", what);
   if (qjl && m != d) return fail_status(PQKV_ERR_UNSUPPORTED, "%s: QJL needs m == d", what);
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail_status(PQKV_ERR_INVALID, "%s: scale must be > 0", what);
-  if (!starts && (start < 0 || start + Sq > S))
-    return fail_status(PQKV_ERR_INVALID, "%s: rows at %lld..%lld are not all in the cache (S=%d)", what,
-                       (long long)start, (long long)start + Sq - 1, S);
+  if (!starts && (start < 0 || start > S || Sq > S - start))
+    return fail_status(PQKV_ERR_INVALID, "%s: %d rows from %lld on are not all in the cache (S=%d)", what, Sq,
+                       (long long)start, S);
   if (Sq == 0) return PQKV_OK;
   if (!window_shape_ok(B, Hq, Hkv, Sq, S, d, qjl))
     return fail_status(PQKV_ERR_UNSUPPORTED, "%s: B=%d Hq=%d Hkv=%d Sq=%d S=%d", what, B, Hq, Hkv, Sq, S);
