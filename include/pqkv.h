@@ -546,7 +546,8 @@ int pqkv_append_rotary_paged(const void *k, const int64_t k_strides[3], const vo
  * at positions that no row sees, and past the last row, has no effect.
  * q, out [B][Hq][Sq][d]. Keys and values of one width n_bits (2 or 4) with S_max
  * = S vectors per stream, window >= 1, sinks >= 0, S < 2^24, B * Hkv <= 65535;
- * Sq = 0 does nothing. Sq > 1: groups Hq / Hkv of up to 256 (128 with signs). The
+ * Sq = 0 does nothing. Sq > 1: groups Hq / Hkv of up to 256 (128 with signs). R is
+ * orthogonal; queries and p_rot are of any size whose logits are finite in 32 bits. The
  * workspace is 16-byte aligned and needs no initialisation. */
 size_t pqkv_window_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, int d, int window, int sinks, int qjl);
 int pqkv_window_attn(const void *q, int q_dtype, const float *R, const uint8_t *k_cache, const uint8_t *v_cache,

@@ -520,6 +520,46 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
       }
   }
 
+  // WIN: a row whose query (or projections) passes what fp16 holds is kept 2^k times
+  // smaller, and its logits multiplied by 2^k again (q_more, of the head whose logits
+  // the lane holds; 1 elsewhere)
+  float q_more = 1.0f;
+  if constexpr (WIN) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+      top = fmaxf(top, fabsf(qrow[grp * (D / 4) + i]));
+      if constexpr (QJL) top = fmaxf(top, fabsf(a.pq[qrow_i * D + grp * (D / 4) + i]));
+    }
+    if (__builtin_amdgcn_ballot_w64(top >= 32768.0f) != 0) {
+      const int k = max((int)(__builtin_bit_cast(uint32_t, rows_max(top)) >> 23) - 141, 0);   // below 2^15
+      const float less = __builtin_ldexpf(qmask, -k);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          half_t vh, vl;
+          split_hi_lo(qrow[grp * (D / 4) + 4 * kk + j] * less, &vh, &vl);
+          qb[kk][2 * j] = qlo ? vl : vh;
+          qb[kk][2 * j + 1] = qlo ? vh : (half_t)0.0f;
+        }
+      if constexpr (QJL) {
+#pragma unroll
+        for (int kq = 0; kq < KQ; ++kq)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            half_t vh, vl;
+            split_hi_lo(a.pq[qrow_i * D + grp * (D / 4) + 8 * kq + i] * less, &vh, &vl);
+            pb[kq][i] = qlo ? vl : vh;
+          }
+      }
+      q_more = __builtin_ldexpf(1.0f, k);
+      if constexpr (G <= 4)
+        q_more = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * (16 * grp + (col & 3)),
+                                                                        __builtin_bit_cast(int, q_more)));
+    }
+  }
+
   // Running softmax state: lanes with col < 8 own head col (replicated over
   // the four rows).
   float m_run = -INFINITY, l_run = 0.0f;
@@ -788,6 +828,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
           c = __builtin_fmaf(x, 1.0f / kLoScale, c) * quad_bcast(rks, i);
         }
         if constexpr (GG) c = __builtin_fmaf(mask_val(mk, i), kLog2eF, c);  // the logits are in the exp2 domain
+        if constexpr (WIN) c *= q_more;
         const int t = kSub * (col >> 2) + 4 * grp + i;
         cv[i] = partial && (WIN ? hidden(t0 + t) : t >= ntok) ? -INFINITY : c;
       }
@@ -799,7 +840,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
 #pragma unroll
       for (int st = 0; st < NSUB; ++st)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sv[st][i] = sc[st][i];
+        for (int i = 0; i < 4; ++i) sv[st][i] = WIN ? sc[st][i] * q_more : sc[st][i];
       if (partial) {
 #pragma unroll
         for (int st = 0; st < NSUB; ++st)

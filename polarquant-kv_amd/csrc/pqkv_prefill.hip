@@ -300,7 +300,16 @@ struct RotationOperands {
       }
     }
   }
-  __device__ __forceinline__ void put(uint8_t *to, int tid) const {
+  // the largest of this lane's and of three others' entries (l ^ 16, l ^ 32, l ^ 48)
+  __device__ __forceinline__ float top() const {
+    float t = 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t = fmaxf(t, fabsf(x[u][j]));
+    return rows_max(t);
+  }
+  __device__ __forceinline__ void put(uint8_t *to, int tid, float scale = kRotScale) const {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       int row, k8, o, r;
@@ -309,7 +318,7 @@ struct RotationOperands {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         half_t h, l;
-        split2(x[u][j] * kRotScale, &h, &l);
+        split2(x[u][j] * scale, &h, &l);
         hi[j] = h;
         lo[j] = l;
       }
@@ -464,6 +473,13 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   half8_t pqh[QJL ? RT : 1][QJL ? KS : 1], pql[QJL ? RT : 1][QJL ? KS : 1];
   int row_pos[RT];
   float undo_q[WIN ? RT : 1];
+  // WIN: a row whose rotated query may pass what fp16 holds is kept 2^k times smaller, one
+  // whose projections may, those 2^j times; row_factor has {2^(k - j), 2^j}: what the
+  // scores are multiplied by before the sign products are added and after. `wide`: one of
+  // the wave's rows has factors; only then they are read.
+  __shared__ float2 row_factor[WIN ? 16 * RT * kPW : 1];
+  __shared__ uint32_t p_top;                           // of P_rot's entries, as bits
+  bool wide = false;
   struct None {};
   std::conditional_t<WIN, RotationOperands<D, false>, None> rot;
   if constexpr (WIN) rot.load(a.R, tid);
@@ -526,6 +542,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     for (int nb = 0; nb < NB; ++nb) oacc[rt][nb] = (float4_t){0.f, 0.f, 0.f, 0.f};
   }
   float4_t sacc[RT][4];                // scores of the tile between X and Y
+  float4_t zacc[QJL && WIN ? 4 : 1];   // and its sign products, where they are summed apart
   half8_t ph[RT][2], pl[RT][2];        // softmax weights between Y and the next X
 
   // ---- stage bodies ----
@@ -564,18 +581,21 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     }
     if constexpr (QJL) {
       // s = r_k (q . c) + [e != 0] sum_i (2 s_i - 1) pq_i: the radius
-      // scaling moves here, then the sign products accumulate on top
+      // scaling moves here, then the sign products accumulate on top (WIN: in a sum of
+      // their own, and the softmax adds the two)
       const float *rk = rads[it & 1];
       const uint8_t *sg = raw_s[it % 3];
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
+        if constexpr (!WIN) {
+          const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          sacc[rt][tt][0] *= r4.x;
-          sacc[rt][tt][1] *= r4.y;
-          sacc[rt][tt][2] *= r4.z;
-          sacc[rt][tt][3] *= r4.w;
+          for (int rt = 0; rt < RT; ++rt) {
+            sacc[rt][tt][0] *= r4.x;
+            sacc[rt][tt][1] *= r4.y;
+            sacc[rt][tt][2] *= r4.z;
+            sacc[rt][tt][3] *= r4.w;
+          }
         }
         // A: signs of token 16 tt + col, projections 32 ks + 8 grp .. + 7
         // (sign byte 4 ks + grp); the zero half of the table for an all-ones
@@ -599,8 +619,9 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
           const half8_t as = pack8u((u32x2){lo.x, lo.y}, (u32x2){hi.x, hi.y});
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            sacc[rt][tt] = mfma16(as, pqh[rt][ks], sacc[rt][tt]);
-            sacc[rt][tt] = mfma16(as, pql[rt][ks], sacc[rt][tt]);
+            float4_t &to = WIN ? zacc[tt] : sacc[rt][tt];            // (RT is 1)
+            to = mfma16(as, pqh[rt][ks], WIN && ks == 0 ? (float4_t){0.f, 0.f, 0.f, 0.f} : to);
+            to = mfma16(as, pql[rt][ks], to);
           }
         }
       }
@@ -650,9 +671,24 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
         const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
         const float rr[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[tt][i] = QJL ? sacc[rt][tt][i] : sacc[rt][tt][i] * rr[i];
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (QJL && WIN) s[tt][i] = __builtin_fmaf(sacc[rt][tt][i], rr[i], zacc[tt][i]);
+          else s[tt][i] = QJL ? sacc[rt][tt][i] : sacc[rt][tt][i] * rr[i];
+        }
       }
-      if (need_mask) {
+      // (one branch for both: one more in each tile costs 1 to 5 %)
+      if (WIN ? need_mask || wide : need_mask) {
+        if (WIN && wide) {
+          const float2 f = row_factor[16 * RT * wave + 16 * rt + col];
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
+            const float rr[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[tt][i] = QJL ? __builtin_fmaf(sacc[rt][tt][i], rr[i] * f.x, zacc[tt][i]) * f.y : s[tt][i] * f.y;
+          }
+        }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -778,10 +814,13 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     uint8_t *m = &tiles[0][0];
     static_assert(D * D * 4 <= 2 * PT::BYTES, "a matrix's parts in the tiles' memory");
     rot.put(m, tid);
+    if (QJL && tid == 0) p_top = 0;
     __syncthreads();
     if constexpr (QJL) rot.load(a.p_rot, tid);
     float4_t acc[RT][D / 16];
     rotate_parts<D, RT>(m, qh, ql, lane, acc);
+    // the powers of two by which products below 2^n, times f, may pass 2^15
+    auto excess = [](int n, float f) { return max((int)(__builtin_bit_cast(uint32_t, f) >> 23) - 126 + n - 15, 0); };
     // products times f as operands: a lane's results are the coordinates it holds
     auto operands = [&](int rt, float f, half8_t (&hi)[KS], half8_t (&lo)[KS]) {
 #pragma unroll
@@ -797,7 +836,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float f = undo_q[rt] * a.q_scale;
-      operands(rt, f, qh[rt], ql[rt]);
+      // (parts below 2^13, and R keeps their norm: at most sqrt(D) 2^13 2^8)
+      const int k = excess(13 + 8 + 4, f);
+      row_factor[16 * RT * wave + 16 * rt + col] = make_float2(1.0f, __builtin_ldexpf(1.0f, k));
+      wide |= __builtin_amdgcn_ballot_w64(k > 0) != 0;
+      operands(rt, __builtin_ldexpf(f, -k), qh[rt], ql[rt]);
       if constexpr (QJL) {
         // (as parts of their own: q' may be far from 1)
         float x[D / 4];
@@ -809,12 +852,26 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       }
     }
     if constexpr (QJL) {
+      const float top = rot.top();
+      if (lane < 16) atomicMax(&p_top, __builtin_bit_cast(uint32_t, top));
       __syncthreads();
-      rot.put(m, tid);
+      // P_rot is of any size: 2^8 times its entries as they are where the largest is from
+      // 2^-5 to 2^7 (a sketch's are), else with that one in [2^12, 2^13)
+      const int e = (int)(__builtin_amdgcn_readfirstlane((int)p_top) >> 23);
+      const int up = e == 0 || e == 255 || (e >= 127 - 5 && e < 127 + 7) ? 0 : e - 131;
+      rot.put(m, tid, __builtin_ldexpf(kRotScale, -up));
       __syncthreads();
       rotate_parts<D, RT>(m, pqh, pql, lane, acc);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) operands(rt, undo_q[rt] * a.p_scale, pqh[rt], pql[rt]);
+      for (int rt = 0; rt < RT; ++rt) {
+        const float f = __builtin_ldexpf(undo_q[rt] * a.p_scale, up);
+        // (parts below 2^13, D entries of P_rot below 2^(e - 126))
+        const int j = excess(13 + (D == 128 ? 7 : 6) + e - 126 + 8 - up, f);
+        float2 &r = row_factor[16 * RT * wave + 16 * rt + col];
+        r = make_float2(__builtin_ldexpf(r.y, -j), __builtin_ldexpf(1.0f, j));
+        wide |= __builtin_amdgcn_ballot_w64(j > 0) != 0;
+        operands(rt, __builtin_ldexpf(f, -j), pqh[rt], pql[rt]);
+      }
     }
     __syncthreads();   // before the first tile is decoded there
   }
