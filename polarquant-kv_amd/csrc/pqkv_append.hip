@@ -591,9 +591,21 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
     // coordinate NC g + 8 ks + j
     for (int i = tid; i < D * KS * 4; i += kAW * 64) {
       const int row = i / (KS * 4), c = 8 * (i % (KS * 4)), gg = c / NC, ks = (c % NC) >> 3;
-      float x[8];
+      float x[8], top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = a.p_rot[row * D + c + j];
+      for (int j = 0; j < 8; ++j) {
+        x[j] = a.p_rot[row * D + c + j];
+        top = fmaxf(top, fabsf(x[j]));
+      }
+      // only the sign of a projection counts: a row (of KS * 4 neighbouring threads) whose
+      // largest entry is not from 2^-5 to 2^7 (a sketch's are) is scaled to [2^4, 2^5)
+#pragma unroll
+      for (int n = 1; n < KS * 4; n *= 2) top = fmaxf(top, __shfl_xor(top, n));
+      const int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+      if (ex != 0 && ex != 255 && (ex < 127 - 5 || ex >= 127 + 7)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __builtin_ldexpf(x[j], 131 - ex);
+      }
       put(sm.p, row, ks, gg, x);
     }
   }
