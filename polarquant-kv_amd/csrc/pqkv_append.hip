@@ -149,7 +149,6 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
   using SM = AppendSmem<D, QJL>;
   constexpr int OT = SM::OT, KS = SM::KS, NM = KS / 2;
   constexpr int NC = D / 4;                       // coordinates of a vector that a lane ends with
-  constexpr int AT = 1;                           // tiles of a wave's step
   __shared__ SM sm;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
       else __builtin_amdgcn_raw_buffer_store_b32(word[0], r, ca, 0, 0);
     }
   };
-  // (wave-uniform) the slots of a run: first, behind the last, and its stream
+  // (wave-uniform) the first slot of a run, and its stream
   struct Run {
     int first, stream;
   };
@@ -479,9 +478,9 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
     }
   };
 
-  // A step: AT tiles of an item for each wave, `wave` + 8 v of those from `tile` on
-  // (the item's keys', then its values'; one past its last is the last again,
-  // without slots). All waves make the same steps.
+  // A step: a tile of an item for each wave, number `tile` + wave (the item's keys',
+  // then its values'; one past its last is the last again, without slots). All waves
+  // make the same steps.
   struct Step {
     int item, tile, pairs, kind_tiles, buf;
   };
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
     p.kind_tiles = (p.pairs + per - 1) / per;
   };
   auto after = [&](Step p) {
-    p.tile += AT * kAW;
+    p.tile += kAW;
     if (p.tile >= 2 * p.kind_tiles) {
       p.item += gridDim.x;
       p.buf ^= 1;
@@ -499,31 +498,25 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
     }
     return p;
   };
-  Vec w[AT], wn[AT];
-  Raw raw[AT];
-  half8_t hi[AT][KS], lo[AT][KS];
-  float undo[AT];
+  Vec w, wn;
+  Raw raw;
+  half8_t hi[KS], lo[KS];
+  float undo;
+  auto tile_of = [&](const Step &p) { return min(p.tile + wave, 2 * p.kind_tiles - 1); };
   auto request = [&](const Step &p) {
-#pragma unroll
-    for (int v = 0; v < AT; ++v) {
-      const int tv = min(p.tile + wave + kAW * v, 2 * p.kind_tiles - 1);
-      wn[v] = locate(p.item, tv, tv < p.kind_tiles, p.kind_tiles, p.pairs);
-    }
-#pragma unroll
-    for (int v = 0; v < AT && VEC; ++v) fetch(wn[v], raw[v]);
+    const int tile = tile_of(p);
+    wn = locate(p.item, tile, tile < p.kind_tiles, p.kind_tiles, p.pairs);
+    if constexpr (VEC) fetch(wn, raw);
   };
-  auto is_key = [&](const Step &p, int v) { return min(p.tile + wave + kAW * v, 2 * p.kind_tiles - 1) < p.kind_tiles; };
+  auto is_key = [&](const Step &p) { return tile_of(p) < p.kind_tiles; };
   auto take = [&](const Step &p) {                // the requested inputs as operands
-#pragma unroll
-    for (int v = 0; v < AT; ++v) {
-      w[v] = wn[v];
-      if constexpr (!RUNS) {
-        w[v].slot = w[v].row >= 0 ? sm.slot[p.buf][w[v].row] : -1;
-        w[v].row = max(w[v].row, 0);
-      }
-      if (p.tile + wave + kAW * v >= 2 * p.kind_tiles) w[v].slot = -1;
-      parts(raw[v], is_key(p, v), w[v], p.buf, hi[v], lo[v], undo[v]);
+    w = wn;
+    if constexpr (!RUNS) {
+      w.slot = w.row >= 0 ? sm.slot[p.buf][w.row] : -1;
+      w.row = max(w.row, 0);
     }
+    if (p.tile + wave >= 2 * p.kind_tiles) w.slot = -1;
+    parts(raw, is_key(p), w, p.buf, hi, lo, undo);
   };
 
   // The first step's loads go out before the operands are made.
@@ -627,32 +620,25 @@ __global__ void __launch_bounds__(kAW * 64, 1) append_kernel(const AppendKernelA
     take(cur);
     const Step nx = after(cur);
     if (nx.item < k.items) request(nx);
-    float4_t acc[AT][OT];
+    float4_t acc[OT];
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
-#pragma unroll
-      for (int v = 0; v < AT; ++v) acc[v][o] = (float4_t){0.f, 0.f, 0.f, 0.f};
+      acc[o] = (float4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const half8_t rh = sm.r[o][ks][0][lane], rl = sm.r[o][ks][1][lane];
-#pragma unroll
-        for (int v = 0; v < AT; ++v) acc[v][o] = mfma16(rh, hi[v][ks], acc[v][o]);
-#pragma unroll
-        for (int v = 0; v < AT; ++v) acc[v][o] = mfma16(rl, hi[v][ks], acc[v][o]);
-#pragma unroll
-        for (int v = 0; v < AT; ++v) acc[v][o] = mfma16(rh, lo[v][ks], acc[v][o]);
+        acc[o] = mfma16(rh, hi[ks], acc[o]);
+        acc[o] = mfma16(rl, hi[ks], acc[o]);
+        acc[o] = mfma16(rh, lo[ks], acc[o]);
       }
     }
-#pragma unroll
-    for (int v = 0; v < AT; ++v) {
-      uint32_t word[NC / 8];
-      uint16_t radius;
-      float e[QJL ? NC : 1];
-      const bool key = is_key(cur, v);
-      quantise(acc[v], key, undo[v], word, radius, e);
-      store(w[v], key, word, radius);
-      if (QJL && key) sketch(w[v], e);
-    }
+    uint32_t word[NC / 8];
+    uint16_t radius;
+    float e[QJL ? NC : 1];
+    const bool key = is_key(cur);
+    quantise(acc, key, undo, word, radius, e);
+    store(w, key, word, radius);
+    if (QJL && key) sketch(w, e);
     if (nx.item >= k.items) return;
     if (nx.item != cur.item) {
       table(nx.item, nx.buf);

@@ -398,7 +398,7 @@ struct PrefillPlan {
 };
 // A call behind a window: never over tiles decoded once, whose rows see one tile in
 // few blocks; splits as above.
-PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w, bool extra);
+PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w);
 inline int64_t prefill_record_bytes(int d) { return 512 * (int64_t)d + 512; }   // one decoded 64-token tile
 // extra: the workspace holds what the plan asks for; planes_only: over tiles
 // decoded once, at any count of row blocks, where a stream's fit their budget.

@@ -1194,14 +1194,13 @@ static void launch_pwin(const PrefillArgs &a, dim3 grid, hipStream_t s) {
   else prefill_mfma_kernel<D, BITS, BITS, false, true><<<grid, kPW * 64, 0, s>>>(a);
 }
 
-PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w, bool extra) {
+PrefillPlan prefill_window_plan(int B, int Hq, int Hkv, int Sq, int S, bool qjl, const Window &w) {
   PrefillPlan p{};
   p.rows = prefill_rows_per_block(qjl);
   p.qt = p.rows / (Hq / Hkv);
   p.qtiles = (Sq - 1) / p.qt + 1;
   p.splits = 1;
   p.streams = B * Hkv;
-  if (!extra) return p;
   // the most tiles that a row block can see
   const int64_t seen = (int64_t)w.size + p.qt + 126, all = ((int64_t)S + kPT - 1) / kPT;
   const int64_t tiles = std::min(seen / kPT + (w.sinks + kPT - 1) / kPT, all);

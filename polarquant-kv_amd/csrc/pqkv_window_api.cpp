@@ -34,9 +34,10 @@ pqkv::Window window_of(int64_t start, const int64_t *starts, const int64_t *coun
 }
 
 // One split has nothing to join: its rows are normalised and rotated back on the fp32
-// matrix cores. At d = 128 4.3 us for 1024 rows against the merge kernel's 5.3, 4.6
-// against 9.2 for 2048, 4.8 against 16.9 for 4096; 4.9 against 4.0 for 256 (few
-// workgroups there). At d = 64 the two are within 0.1 us up to 1792 rows.
+// matrix cores. Single launches between two events (which are most of the smallest), us, against
+// the merge kernel's: d = 128 6.8 and 6.6 for 256 rows, 6.8 and 7.0 for 512, 7.0 and 8.0 for
+// 1024, 7.2 and 11.9 for 2048, 7.1 and 19.5 for 4096; d = 64 within 0.1 up to 768, 6.1 and
+// 6.4 for 1024, 6.0 and 6.5 for 2048, 6.2 and 8.4 for 4096.
 constexpr int64_t kMergeMfmaRows = 512;
 
 // One row per sequence: the splits of a stream's tiles, as many as the decode
@@ -162,7 +163,7 @@ int window_run(const char *what, const void *q, int q_dtype, const float *R, con
     pqkv::prof_end(t, st);
     return report_hip_error(e, "window merge launch");
   }
-  const pqkv::PrefillPlan plan = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl, w, true);
+  const pqkv::PrefillPlan plan = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl, w);
   pqkv::PrefillArgs a;
   memset(&a, 0, sizeof(a));
   float *o32 = (float *)base;      // rotated outputs, where splits are joined
@@ -224,7 +225,7 @@ size_t pqkv_window_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int S, i
   const pqkv::Window w = window_of(0, nullptr, nullptr, Sq, window, sinks, S);
   if (Sq == 1) return pqkv::decode_workspace_layout(B, Hq, row_splits(B, Hkv, S, w), d, nullptr, nullptr, nullptr);
   // (the outputs of one split are final; 256 bytes, so that 0 means a shape that no call takes)
-  const pqkv::PrefillPlan p = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl != 0, w, true);
+  const pqkv::PrefillPlan p = pqkv::prefill_window_plan(B, Hq, Hkv, Sq, S, qjl != 0, w);
   return p.splits == 1 ? 256 : align256((size_t)B * Hq * Sq * d * 4) + p.part_bytes(d);
 }
 

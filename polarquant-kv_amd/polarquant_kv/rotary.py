@@ -239,8 +239,9 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     radians per position, float64 (rotary_frequencies, on the device). Pairs
     are (i, i + rot_dim / 2), or neighbours with interleaved. axes (a sequence of
     numbers, one per frequency; axis_of_pairs): pair i turns by the positions of
-    axis axes[i], which are [A, T] or [A, B, T] then. The inputs may have any strides and may be expanded; gradients flow to both, and
-    forward-mode tangents (torch.autograd.forward_ad) through them."""
+    axis axes[i], which are [A, T] or [A, B, T] then. The inputs may have any
+    strides and may be expanded; gradients flow to both, and forward-mode
+    tangents (torch.autograd.forward_ad) through them."""
     for name, x in (("query", query), ("key", key)):
         if x is not None and x.dim() != 4:
             raise ValueError(f"{name} must be [B, H, T, d], got {tuple(x.shape)}")
