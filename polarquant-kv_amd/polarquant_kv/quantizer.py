@@ -272,7 +272,7 @@ def _dequantize_slots(cache, out_dtype, S: int) -> torch.Tensor:
     out = torch.empty(B, H, S, d, dtype=out_dtype, device=where.device)
     if out.numel() == 0:
         return out
-    row = 0 if paged else cache.max_seq_len * vector_bytes(d, cache.n_bits)
+    row = 0 if paged else cache.blocks.shape[2] * cache.blocks.shape[3]
     with _lib.on_device(out):
         _lib.check(_lib.lib().pqkv_dequantize_slots(
             None if paged else cache.blocks.data_ptr(), row, cache.table.data_ptr() if paged else None,

@@ -37,3 +37,17 @@ def test_the_first_radius_of_a_vector(d, bits, page):
     got = quantizer.dequantize(cache, None, torch.float32)
     assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -24 + 2.0 ** -149).all())
     assert torch.equal(got, quantizer.dequantize(cache, torch.eye(d, device=DEV), torch.float32))
+
+
+@pytest.mark.parametrize("H", [1, 3])
+def test_blocks_longer_than_the_cache_says(H):
+    """Streams lie where the blocks have them, also where max_seq_len is less than their length."""
+    B, S, d = 2, 40, 64
+    g = torch.Generator(device=DEV).manual_seed(6)
+    cache = quantizer.compress_pq(torch.randn(B, H, S, d, generator=g, device=DEV), torch.eye(d, device=DEV), 4)
+    whole = quantizer.dequantize(cache, None, torch.float32)
+    cache.max_seq_len = cache.seq_len = 25
+    assert torch.equal(quantizer.dequantize(cache, None, torch.float32), whole[:, :, :25])
+    assert torch.equal(quantizer.dequantize(cache, torch.eye(d, device=DEV), torch.float32), whole[:, :, :25])
+    cache.blocks = cache.blocks.transpose(0, 1).contiguous().transpose(0, 1)    # (H = 1: dense, with strides of its own)
+    assert torch.equal(quantizer.dequantize(cache, None, torch.float32), whole[:, :, :25])
