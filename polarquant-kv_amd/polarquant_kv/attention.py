@@ -414,6 +414,8 @@ def row_starts(starts, n: int, B: int, device) -> tuple:
     """(start, starts) of a call's n new positions: a number for every sequence,
     or int64 [B] on the device (a tensor of integers; the kernels read it)."""
     if not isinstance(starts, torch.Tensor):
+        if starts != int(starts):
+            raise ValueError(f"starts must be a whole number, got {starts}")
         return int(starts), None
     if tuple(starts.shape) != (B,) or starts.dtype.is_floating_point or starts.dtype.is_complex or \
             starts.dtype == torch.bool:
