@@ -531,6 +531,19 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs &a, DecodeSmem
       top = fmaxf(top, fabsf(qrow[grp * (D / 4) + i]));
       if constexpr (QJL) top = fmaxf(top, fabsf(a.pq[qrow_i * D + grp * (D / 4) + i]));
     }
+    // (the operands as they are, or the compiler makes them after the branch for both ways)
+    auto made = [](half8_t &x) {
+      typedef uint32_t u32x4r __attribute__((ext_vector_type(4)));
+      u32x4r y = __builtin_bit_cast(u32x4r, x);
+      asm("" : "+v"(y));
+      x = __builtin_bit_cast(half8_t, y);
+    };
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) made(qb[kk]);
+    if constexpr (QJL) {
+#pragma unroll
+      for (int kq = 0; kq < KQ; ++kq) made(pb[kq]);
+    }
     if (__builtin_amdgcn_ballot_w64(top >= 32768.0f) != 0) {
       const int k = max((int)(__builtin_bit_cast(uint32_t, rows_max(top)) >> 23) - 141, 0);   // below 2^15
       const float less = __builtin_ldexpf(qmask, -k);

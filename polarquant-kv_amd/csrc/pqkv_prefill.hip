@@ -474,9 +474,10 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
   int row_pos[RT];
   float undo_q[WIN ? RT : 1];
   // WIN: a row whose rotated query may pass what fp16 holds is kept 2^k times smaller, one
-  // whose projections may, those 2^j times; row_factor has {2^(k - j), 2^j}: what the
-  // scores are multiplied by before the sign products are added and after. `wide`: one of
-  // the wave's rows has factors; only then they are read.
+  // whose projections may, those 2^j times; row_factor has {2^k, 2^j}, which the sums are
+  // multiplied by again. `wide`: one of the wave's rows has factors; only then they are
+  // read, at the end of the matrix stage (in the softmax, where more is live, that costs
+  // registers: 2 bits, D = 128 479 -> 518 us for 8191 rows behind 1024).
   __shared__ float2 row_factor[WIN ? 16 * RT * kPW : 1];
   __shared__ uint32_t p_top;                           // of P_rot's entries, as bits
   bool wide = false;
@@ -542,7 +543,12 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
     for (int nb = 0; nb < NB; ++nb) oacc[rt][nb] = (float4_t){0.f, 0.f, 0.f, 0.f};
   }
   float4_t sacc[RT][4];                // scores of the tile between X and Y
-  float4_t zacc[QJL && WIN ? 4 : 1];   // and its sign products, where they are summed apart
+  // Behind a window, D = 128: the sign products are summed apart, and the softmax adds the
+  // two (4 x 512 rows behind 4096 positions: 4 bits 583 us where one sum takes 600, 2 bits
+  // 566 and 577; at D = 64, where the softmax's stage is the longer one, 415 against 398:
+  // one sum).
+  constexpr bool kApart = WIN && QJL && D == 128;
+  float4_t zacc[kApart ? 4 : 1];
   half8_t ph[RT][2], pl[RT][2];        // softmax weights between Y and the next X
 
   // ---- stage bodies ----
@@ -579,15 +585,24 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       ah = ah_n;
       al = al_n;
     }
+    auto widen_rows = [&](bool queries, float4_t (&sum)[4], int rt) {
+      const float2 f = row_factor[16 * RT * wave + 16 * rt + col];
+      const float x = !queries ? f.y : QJL && !kApart ? f.x / f.y : f.x;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) sum[tt] *= x;
+    };
+    if (WIN && wide) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) widen_rows(true, sacc[rt], rt);
+    }
     if constexpr (QJL) {
       // s = r_k (q . c) + [e != 0] sum_i (2 s_i - 1) pq_i: the radius
-      // scaling moves here, then the sign products accumulate on top (WIN: in a sum of
-      // their own, and the softmax adds the two)
+      // scaling moves here, then the sign products accumulate on top (kApart: neither)
       const float *rk = rads[it & 1];
       const uint8_t *sg = raw_s[it % 3];
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        if constexpr (!WIN) {
+        if constexpr (!kApart) {
           const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
@@ -619,11 +634,15 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
           const half8_t as = pack8u((u32x2){lo.x, lo.y}, (u32x2){hi.x, hi.y});
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            float4_t &to = WIN ? zacc[tt] : sacc[rt][tt];            // (RT is 1)
-            to = mfma16(as, pqh[rt][ks], WIN && ks == 0 ? (float4_t){0.f, 0.f, 0.f, 0.f} : to);
+            float4_t &to = kApart ? zacc[tt] : sacc[rt][tt];         // (RT is 1)
+            to = mfma16(as, pqh[rt][ks], kApart && ks == 0 ? (float4_t){0.f, 0.f, 0.f, 0.f} : to);
             to = mfma16(as, pql[rt][ks], to);
           }
         }
+      }
+      if (WIN && wide) {
+        if constexpr (kApart) widen_rows(false, zacc, 0);
+        else widen_rows(false, sacc[0], 0);
       }
     }
   };
@@ -672,23 +691,11 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
         const float rr[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (QJL && WIN) s[tt][i] = __builtin_fmaf(sacc[rt][tt][i], rr[i], zacc[tt][i]);
+          if constexpr (kApart) s[tt][i] = __builtin_fmaf(sacc[rt][tt][i], rr[i], zacc[tt][i]);
           else s[tt][i] = QJL ? sacc[rt][tt][i] : sacc[rt][tt][i] * rr[i];
         }
       }
-      // (one branch for both: one more in each tile costs 1 to 5 %)
-      if (WIN ? need_mask || wide : need_mask) {
-        if (WIN && wide) {
-          const float2 f = row_factor[16 * RT * wave + 16 * rt + col];
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            const float4 r4 = *(const float4 *)&rk[16 * tt + 4 * grp];
-            const float rr[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[tt][i] = QJL ? __builtin_fmaf(sacc[rt][tt][i], rr[i] * f.x, zacc[tt][i]) * f.y : s[tt][i] * f.y;
-          }
-        }
+      if (need_mask) {
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -838,7 +845,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       const float f = undo_q[rt] * a.q_scale;
       // (parts below 2^13, and R keeps their norm: at most sqrt(D) 2^13 2^8)
       const int k = excess(13 + 8 + 4, f);
-      row_factor[16 * RT * wave + 16 * rt + col] = make_float2(1.0f, __builtin_ldexpf(1.0f, k));
+      row_factor[16 * RT * wave + 16 * rt + col] = make_float2(__builtin_ldexpf(1.0f, k), 1.0f);
       wide |= __builtin_amdgcn_ballot_w64(k > 0) != 0;
       operands(rt, __builtin_ldexpf(f, -k), qh[rt], ql[rt]);
       if constexpr (QJL) {
@@ -867,8 +874,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
         const float f = __builtin_ldexpf(undo_q[rt] * a.p_scale, up);
         // (parts below 2^13, D entries of P_rot below 2^(e - 126))
         const int j = excess(13 + (D == 128 ? 7 : 6) + e - 126 + 8 - up, f);
-        float2 &r = row_factor[16 * RT * wave + 16 * rt + col];
-        r = make_float2(__builtin_ldexpf(r.y, -j), __builtin_ldexpf(1.0f, j));
+        row_factor[16 * RT * wave + 16 * rt + col].y = __builtin_ldexpf(1.0f, j);
         wide |= __builtin_amdgcn_ballot_w64(j > 0) != 0;
         operands(rt, __builtin_ldexpf(f, -j), pqh[rt], pql[rt]);
       }
