@@ -507,7 +507,8 @@ int pqkv_rotary_axes(const void *q, const int64_t q_strides[3], void *q_out, int
  * The rotation runs in fp16 parts with fp32 sums (about 2^-22 of the operands'
  * norms): codes and radii differ from pqkv_encode's where a direction lies that
  * close to a border, and, for 16-bit inputs, where the rounding of the turned key
- * to them moves it across one. R is orthogonal (entries up to 1). A vector that
+ * to them moves it across one. R is orthogonal (entries up to 1); p_rot is of any
+ * size. A vector that
  * holds a number that is not finite gets radius NaN (codes 0); norms above 65504
  * are stored as that. q (or NULL): [B][Hq][T][d], turned and rounded to dtype into
  * q_out as pqkv_rotary_axes does. */
@@ -584,8 +585,8 @@ int pqkv_dequantize_rows(const uint8_t *blocks, int64_t blocks_outer_stride, con
 /* The same without the rotation, out of a cache as it lies: out[s][t] = r16 c[code]
  * for the slots t < S of n_streams streams, which start s * stride bytes into
  * blocks or, with pages, are found through the table (as pqkv_encode_paged;
- * blocks and stride unused). Equal to pqkv_dequantize with R = I. out
- * [n_streams][S][d] fp32/fp16, 16-byte aligned. */
+ * blocks and stride unused). Equal to pqkv_dequantize with R = I. blocks and
+ * stride are even; out [n_streams][S][d] fp32/fp16, 16-byte aligned. */
 int pqkv_dequantize_slots(const uint8_t *blocks, int64_t stride, const uint8_t *const *pages, int page_tokens,
                           int max_pages, const float *codebook, int n_bits, void *out, int out_dtype,
                           int64_t n_streams, int S, int d, void *stream);

@@ -29,11 +29,15 @@
 // itself. The sign product takes its residuals in that order, too: nothing leaves
 // the lanes.
 //
-// Measured (bf16, d = 128, 32768 tokens of 8 heads): 80-92 us box to box, 172 MB at
-// 1.9 to 2.1 TB/s, 51 GFLOP (three products) at 560 to 640 TFLOP/s. It is bound by
-// what a vector costs beside its products: turn, parts, radius, a table lookup and a
-// compare per coordinate. Eight waves of two tiles each took 125; 64 rows to an item
-// 88 where 32 take 90 and a step's rows alone 93.
+// Measured (bf16, d = 128, 32768 tokens of 8 heads): 80-95 us box to box, 172 MB at
+// 1.8 to 2.1 TB/s, 51 GFLOP (three products) at 540 to 640 TFLOP/s. Of its cycles the
+// vector units issue for 51 % (20 instructions a coordinate: turn, parts, radius, a table
+// lookup and a compare), the matrix cores are busy for 31 %, LDS for 42 % (R's 64 KB of
+// operands a tile, lookups, sines; 14 % are bank conflicts of the lookups): no one bound,
+// the first two share a SIMD's issue. Eight waves of two tiles each took 125; 64 rows to
+// an item 88 where 32 take 90 and a step's rows alone 93. The same at 2 bits 79, with
+// signs (eight waves, 16 rows to an item) 129 and at 2 bits 127, of fp32 inputs 100 (24
+// registers spilled by sixteen waves, so eight), at d = 64 43 us, in replayed graphs.
 // One token of 8 sequences takes 16 us: of 33 000 cycles the table of codes is 10 700,
 // first loads and R's parts 9 000, the sines 4 100, the tile 10 200. Searching the
 // codebook instead, or R's loads ahead of the table, were no faster (19.4 and 15.9).

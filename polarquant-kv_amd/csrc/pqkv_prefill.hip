@@ -50,13 +50,14 @@
 // after the last. The rows of R are ordered such that its product with the
 // queries is the score product's operand as it leaves the matrix cores; the outputs
 // pass through LDS once, row by row. 32 + 8 heads, 8191 positions, box to box within 2 %:
-// 617 -> 518 us a call behind 1024 positions, 338 -> 214 behind 64. Without QJL at D =
-// 128 29 registers spill around the two rotations; both row tiles share each operand
+// 617 -> 512 us a call behind 1024 positions, 338 -> 201 behind 64. Without QJL at D =
+// 128 30 registers spill around the two rotations; both row tiles share each operand
 // of R, one operand live at a time, since a row tile at a time held them all (143
-// spilled, the tile loop's own among them, and 600 us). Of a workgroup's 310 000
-// cycles behind 1024 positions (18 tiles) 242 000 are the tile loop, 7 300 each the
-// products of the two rotations, whose matrix instructions alone take 6 100; R's loads
-// go out with the queries', the first tiles' behind them (6 % of the call).
+// spilled, the tile loop's own among them, and 600 us). Of a workgroup's 300 000
+// cycles behind 1024 positions (18 tiles) 250 000 are the tile loop, 7 800 the queries'
+// rotation, 8 000 to 10 000 the outputs' and their stores, where the matrix instructions
+// alone take 6 100; R's loads go out with the queries', the first tiles' behind them (6 %
+// of the call).
 //
 // Precision: every fp32 operand x is split as x_hi = fp16(x),
 // x_lo = fp16(x - x_hi) (fp16 subnormals included, which the f16 MFMA keeps),

@@ -1,7 +1,9 @@
 // What the slots of a cache stand for, without a rotation (pqkv_dequantize_slots):
 // out[stream][t][j] = r16 c[code_j], contiguous or through the page table.
 //
-// Bound by its output: 144 bytes of a vector pair become 512 (fp16, d = 128). A
+// 144 bytes of a vector pair become 512 (fp16, d = 128), at 3.6 TB/s; what bounds it are
+// its vector instructions, 12.5 a coordinate, 81 % of the cycles (the address of a slot in
+// its page, the codes, NaN and saturation). A
 // thread takes eight coordinates (the codes that one 16-byte store of fp16 needs),
 // neighbouring threads neighbouring ones, so that stores and the reads of a vector's
 // bytes are dense; the codebook is in LDS, one bank an entry. 8 streams of 32768
