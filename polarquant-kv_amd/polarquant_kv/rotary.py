@@ -322,7 +322,7 @@ class RotaryEmbedding:
             return positions
         if positions.dim() == 1:
             return positions.expand(self.n_axes, -1)
-        if batch is None:
+        if batch is None or positions.dim() not in (2, 3):
             return positions
         rows = positions.shape[0]
         if positions.dim() == 2 and rows == batch:
