@@ -47,7 +47,6 @@ def test_rows_that_could_be_either_or_neither_are_refused(handed_over):
 
 def test_positions_of_other_ranks_are_the_rotation_s_to_refuse():
     e = rotary.RotaryEmbedding(64, sections=(12, 10, 10))
-    q = torch.zeros(2, 2, 4, 64)
     for positions in (torch.tensor(3), torch.zeros(3, 2, 4, 1, dtype=torch.int64)):
         with pytest.raises(ValueError, match="positions must be"):
-            e(q, None, positions)
+            rotary.check_axes(e.axes, e.positions_by_axis(positions, 2), 32, 2, 4)
