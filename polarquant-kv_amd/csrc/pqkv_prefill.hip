@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(kPW * 64, 1) prefill_mfma_kernel(const Prefill
       // P_rot is of any size: 2^8 times its entries as they are where the largest is from
       // 2^-5 to 2^7 (a sketch's are), else with that one in [2^12, 2^13)
       const int e = (int)(__builtin_amdgcn_readfirstlane((int)p_top) >> 23);
-      const int up = e == 0 || e == 255 || (e >= 127 - 5 && e < 127 + 7) ? 0 : e - 131;
+      const int up = e == 0 || e == 255 || (e >= 127 - 5 && e < 127 + 7) ? 0 : max(e - 131, -110);
       rot.put(m, tid, __builtin_ldexpf(kRotScale, -up));
       __syncthreads();
       rotate_parts<D, RT>(m, pqh, pql, lane, acc);

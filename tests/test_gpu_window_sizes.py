@@ -82,3 +82,16 @@ def test_large_projections(d, bits, Sq):
     want, bound = window_ref.window_attention(q, keys, values, R, 64, 3, at, n, scale=1.0, p_rot=jl)
     got = attention.window_attention(q, keys, values, R, 64, sinks=3, starts=at, scale=1.0, jl_rot=jl, out_dtype=torch.float32)
     window_ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("power", [-140, -125, -118, -100, -60])
+@pytest.mark.parametrize("Sq", [1, 24])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiny_projections(d, Sq, power):
+    """Signs whose projections are far below everything else."""
+    q, keys, values, R, jl = make(Sq, d, 2, 4, 4, True, 0, 1.0, 1.0)
+    jl = torch.ldexp(jl, torch.tensor(float(power), device=DEV))
+    at, n = window_tests.per_sequence([300 - Sq, 5], 2), window_tests.per_sequence(Sq, 2)
+    want, bound = window_ref.window_attention(q, keys, values, R, 64, 3, at, n, scale=1.0, p_rot=jl)
+    got = attention.window_attention(q, keys, values, R, 64, sinks=3, starts=at, scale=1.0, jl_rot=jl, out_dtype=torch.float32)
+    window_ref.check(got, want, bound)
